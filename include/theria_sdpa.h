@@ -1,5 +1,6 @@
 /*
- * theria_sdpa.h - C ABI of the MI355X (gfx950) scaled-dot-product-attention operator family.
+ * theria_sdpa.h - C ABI of the MI355X (gfx950) scaled-dot-product-attention operator family and of the token-side
+ * operators of a training step (layer norm, embedding, linear cross entropy; at the end of this file).
  *
  * One shared library, libtheria_sdpa.so, exports these entry points. They take caller-owned device
  * pointers, plain integer shapes and strides, and a hipStream_t passed as void*. The library never
@@ -29,7 +30,7 @@
 extern "C" {
 #endif
 
-#define THERIA_SDPA_ABI_VERSION 10
+#define THERIA_SDPA_ABI_VERSION 11
 
 enum theria_dtype { THERIA_DTYPE_F32 = 0, THERIA_DTYPE_F16 = 1, THERIA_DTYPE_BF16 = 2 };
 enum theria_status { THERIA_OK = 0, THERIA_ERR_CONTRACT = 1, THERIA_ERR_HIP = 2 };
@@ -244,6 +245,92 @@ int theria_debug_tile_counts(uint64_t* counts, int32_t reset);
  * counter-enabled build (libtheria_sdpa_tiles.so) runs it; libtheria_sdpa.so returns THERIA_ERR_CONTRACT.
  */
 int theria_debug_atomic_probe(float* buf, int64_t n, int32_t reps, int32_t atomic, void* stream);
+
+/*
+ * Token-side operators: what a transformer's training step runs beside its attention. They have no counterpart in the
+ * reference, whose models take them from PyTorch. Matrices are (rows, width) views with an element stride from row to
+ * row and a contiguous last dimension; ids and targets are contiguous int32 or int64 arrays. Sums are float32 and every
+ * result is rounded once; nothing uses float atomics, so results repeat bit for bit.
+ */
+typedef struct {
+  void* data;
+  int64_t stride_row; /* elements */
+} theria_rows_t;
+
+/* Layer norm over the last dimension, at most 16384 wide. */
+typedef struct {
+  int32_t dtype;       /* of x, y and the other matrices */
+  int32_t param_dtype; /* of weight, bias and their gradients: dtype, or float32 */
+  int32_t width;
+  float eps;
+  int64_t rows;
+} theria_layer_norm_problem_t;
+
+/* y = (x - mean) rstd weight + bias; mean and rstd (rows floats each) are saved for the backward. weight and bias may be
+ * NULL (ones, zeros). */
+int theria_layer_norm_fwd(const theria_layer_norm_problem_t* p, const theria_rows_t* x, const void* weight, const void* bias,
+                          const theria_rows_t* y, float* mean, float* rstd, void* stream);
+/* Floats of the workspace of the two calls below (partial column sums). */
+int64_t theria_layer_norm_ws_floats(const theria_layer_norm_problem_t* p);
+/* dx, dweight, dbias; each may be absent (data == NULL, NULL). ws is needed for dweight and dbias only. */
+int theria_layer_norm_bwd(const theria_layer_norm_problem_t* p, const theria_rows_t* x, const void* weight, const theria_rows_t* dout,
+                          const float* mean, const float* rstd, const theria_rows_t* dx, void* dweight, void* dbias, float* ws,
+                          void* stream);
+/* The gradient of <gdx, dx> + <gdw, dweight> + <gdb, dbias> with respect to x, weight and dout. Cotangents and results may
+ * be absent; ws is needed for out_gw only. */
+int theria_layer_norm_bwd_bwd(const theria_layer_norm_problem_t* p, const theria_rows_t* x, const void* weight,
+                              const theria_rows_t* dout, const float* mean, const float* rstd, const theria_rows_t* gdx,
+                              const void* gdw, const void* gdb, const theria_rows_t* out_gx, void* out_gw,
+                              const theria_rows_t* out_gdout, float* ws, void* stream);
+
+/* Embedding lookup with a scale, rows of at most 2^20. */
+typedef struct {
+  int32_t dtype;
+  int32_t ids64; /* ids are int64, else int32 */
+  int32_t width;
+  float scale;
+  int64_t n;       /* ids */
+  int64_t classes; /* rows of the table, below 2^31 */
+  int64_t padding; /* id whose row gets no gradient, or -1 */
+} theria_embedding_problem_t;
+
+/* out[i] = scale table[ids[i]]. An id outside the table gives a row of NaN. zero_padding: rows of the padding id are zeros
+ * (the derivative of the gradient with respect to dout). */
+int theria_embedding_fwd(const theria_embedding_problem_t* p, const void* ids, const theria_rows_t* table, int32_t zero_padding,
+                         const theria_rows_t* out, void* stream);
+/* Bytes of the 16-byte-aligned workspace of the gradient. */
+int64_t theria_embedding_ws_bytes(const theria_embedding_problem_t* p);
+/* dtable[v] = scale times the sum of dout[i] over ids[i] == v, every row of dtable written. Ids outside the table and the
+ * padding id add nothing. */
+int theria_embedding_bwd(const theria_embedding_problem_t* p, const void* ids, const theria_rows_t* dout, const theria_rows_t* dtable,
+                         void* ws, void* stream);
+
+/* Cross entropy of the logits x weight^T + bias, rows of at most 2^20. */
+enum theria_reduction { THERIA_REDUCE_NONE = 0, THERIA_REDUCE_MEAN = 1, THERIA_REDUCE_SUM = 2 };
+typedef struct {
+  int32_t dtype;     /* of x, weight, bias and their gradients */
+  int32_t target64;  /* targets are int64, else int32 */
+  int32_t reduction; /* enum theria_reduction */
+  int32_t width;
+  int64_t n;         /* rows of x, below 2^31 */
+  int64_t classes;   /* rows of weight, below 2^31 */
+  int64_t ignore;    /* target of the rows that are left out */
+} theria_linear_ce_problem_t;
+
+/* Bytes of the 256-byte-aligned workspace of a call on these matrices. Nothing in it is kept between calls. */
+int64_t theria_linear_ce_ws_bytes(const theria_linear_ce_problem_t* p, const theria_rows_t* weight, int32_t backward,
+                                  int32_t need_dx, int32_t need_dweight, int32_t need_dbias);
+/* loss (float32: n of them, or one) and, for the backward, stats (2 n floats: of the i-th row that is not left out, the
+ * largest logit and the sum of exp(logit - largest)). Rows left out have loss 0 and are not read; a target outside
+ * [0, classes) gives a loss of NaN. The mean is over the rows that are not left out, NaN if there are none. bias may be NULL. */
+int theria_linear_ce_fwd(const theria_linear_ce_problem_t* p, const theria_rows_t* x, const theria_rows_t* weight, const void* bias,
+                         const void* target, float* loss, float* stats, void* ws, void* stream);
+/* dx, dweight, dbias for the loss's gradient dloss (float32: n, or one), from the stats of the forward on the same
+ * inputs. Each may be absent. Rows left out have zeros in dx; a row with a target outside [0, classes) has NaN there and adds
+ * nothing to dweight and dbias. */
+int theria_linear_ce_bwd(const theria_linear_ce_problem_t* p, const theria_rows_t* x, const theria_rows_t* weight, const void* bias,
+                         const void* target, const float* stats, const float* dloss, const theria_rows_t* dx,
+                         const theria_rows_t* dweight, void* dbias, void* ws, void* stream);
 
 #ifdef __cplusplus
 }

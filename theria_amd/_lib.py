@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be imported first: it loads the HIP runtime th
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtheria_sdpa.so"
 # The counter-enabled build of the same sources (theria_debug_tile_counts counts there), for measurements only.
 TILES_LIB_PATH = LIB_PATH.with_name("libtheria_sdpa_tiles.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 OK, ERR_CONTRACT, ERR_HIP = 0, 1, 2
@@ -53,7 +53,57 @@ class Problem(ctypes.Structure):
     ]
 
 
+class RowsView(ctypes.Structure):
+    """theria_rows_t: (rows, width) view; last dim contiguous."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("stride_row", ctypes.c_int64)]
+
+
+class LayerNormProblem(ctypes.Structure):
+    """theria_layer_norm_problem_t."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("param_dtype", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("rows", ctypes.c_int64),
+    ]
+
+
+class EmbeddingProblem(ctypes.Structure):
+    """theria_embedding_problem_t."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("ids64", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("n", ctypes.c_int64),
+        ("classes", ctypes.c_int64),
+        ("padding", ctypes.c_int64),
+    ]
+
+
+class LinearCeProblem(ctypes.Structure):
+    """theria_linear_ce_problem_t."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("target64", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("n", ctypes.c_int64),
+        ("classes", ctypes.c_int64),
+        ("ignore", ctypes.c_int64),
+    ]
+
+
 _TV = ctypes.POINTER(TensorView)
+_RV = ctypes.POINTER(RowsView)
+_NP = ctypes.POINTER(LayerNormProblem)
+_EP = ctypes.POINTER(EmbeddingProblem)
+_CP = ctypes.POINTER(LinearCeProblem)
 _PR = ctypes.POINTER(Problem)
 _FP = ctypes.POINTER(ctypes.c_float)
 
@@ -87,6 +137,22 @@ SIGNATURES = {
     ),
     "theria_qk_scores": ([_PR, _TV, _TV, _P, ctypes.c_int32, _P], ctypes.c_int),
     "theria_qk_softmax": ([_PR, _TV, _TV, _P, _P], ctypes.c_int),
+    "theria_layer_norm_fwd": ([_NP, _RV, _P, _P, _RV, _P, _P, _P], ctypes.c_int),
+    "theria_layer_norm_ws_floats": ([_NP], ctypes.c_int64),
+    "theria_layer_norm_bwd": ([_NP, _RV, _P, _RV, _P, _P, _RV, _P, _P, _P, _P], ctypes.c_int),
+    "theria_layer_norm_bwd_bwd": (
+        [_NP, _RV, _P, _RV, _P, _P, _RV, _P, _P, _RV, _P, _RV, _P, _P],
+        ctypes.c_int,
+    ),
+    "theria_embedding_fwd": ([_EP, _P, _RV, ctypes.c_int32, _RV, _P], ctypes.c_int),
+    "theria_embedding_ws_bytes": ([_EP], ctypes.c_int64),
+    "theria_embedding_bwd": ([_EP, _P, _RV, _RV, _P, _P], ctypes.c_int),
+    "theria_linear_ce_ws_bytes": (
+        [_CP, _RV, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32],
+        ctypes.c_int64,
+    ),
+    "theria_linear_ce_fwd": ([_CP, _RV, _RV, _P, _P, _P, _P, _P, _P], ctypes.c_int),
+    "theria_linear_ce_bwd": ([_CP, _RV, _RV, _P, _P, _P, _P, _RV, _RV, _P, _P, _P], ctypes.c_int),
     "theria_debug_tile_counts": ([ctypes.POINTER(ctypes.c_uint64), ctypes.c_int32], ctypes.c_int),
     "theria_debug_atomic_probe": ([_P, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _P], ctypes.c_int),
 }

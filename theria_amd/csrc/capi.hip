@@ -8,6 +8,7 @@
 
 #include "../../include/theria_sdpa.h"
 #include "sdpa_params.hpp"
+#include "token_params.hpp"
 
 #define THERIA_API extern "C" __attribute__((visibility("default")))
 
@@ -110,6 +111,10 @@ bool empty_problem(const theria::Shape& s) { return s.B == 0 || s.H == 0 || s.T 
 }  // namespace
 
 namespace theria {
+
+// The same for the entry points of the other files.
+int fail(int code, const char* msg) { return ::fail(code, std::string(msg)); }
+int hip_status(hipError_t e, const char* what) { return ::hip_status(e, what); }
 
 // Compute units of the current device. The per-device cache is written with the same value by any
 // thread that fills it, so concurrent first calls are harmless.

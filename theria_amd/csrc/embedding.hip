@@ -1,0 +1,463 @@
+// Embedding lookup with a scale, and its gradient by sorted tokens (gfx950).
+//
+//   lookup    out[n] = s W[ids[n]]
+//   gradient  dW[v] = s sum of dout[n] over the n with ids[n] = v, zeros for ids that no token has
+//
+// Both are bound by memory. The gradient orders the tokens by (id, n) first: every row of dW then has a known run of
+// tokens and is summed in float32 and written once, in an order that does not depend on the run (no float atomics, no
+// float32 copy of the table, no clearing pass).
+//
+//   order   up to kRankTokens tokens: one launch in which every token counts the tokens before it (n^2 comparisons out
+//           of LDS, spread over the GPU). More: a stable radix sort, digits of at most 10 bits, two launches a digit.
+//   pieces  frequent ids: every aligned run of 64 sorted tokens that holds one id alone is summed by a workgroup of its
+//           own into a float32 row of the workspace, so that an id with thousands of tokens is spread over the GPU.
+//   rows    every table row: its bounds by binary search, then the tokens before its first whole piece, the pieces,
+//           and the tokens after its last one.
+#include "token_common.hpp"
+#include "token_params.hpp"
+
+namespace theria {
+namespace {
+
+constexpr int kPiece = 64;         // sorted tokens of a piece
+constexpr int kRankTokens = 8192;  // most tokens ordered by counting
+constexpr int kSortTile = 4096;    // tokens of a radix sort's workgroup
+constexpr int kSortMost = 1024;    // digits of a radix sort's pass
+
+__device__ __forceinline__ int64_t load_id(const void* ids, bool ids64, int64_t n) {
+  return ids64 ? ((const int64_t*)ids)[n] : (int64_t)((const int32_t*)ids)[n];
+}
+
+// The sort key of an id: the id, or `classes` (behind every row) for padding and for ids outside the table.
+__device__ __forceinline__ uint32_t key_of(const EmbedParams& p, int64_t n) {
+  const int64_t id = load_id(p.ids, p.ids64, n);
+  return id < 0 || id >= p.classes || id == p.padding ? (uint32_t)p.classes : (uint32_t)id;
+}
+
+// ------------------------------------------------------------------------------------------ lookup
+// Teams of TPR threads, one for each token; a thread moves two vectors of the row (grid.y covers wide rows).
+template <typename T, int VEC, int TPR>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
+  constexpr int TEAMS = 256 / TPR;
+  const int t = threadIdx.x % TPR;
+  const int64_t n = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
+  if (n >= p.n) return;
+  const int64_t id = load_id(p.ids, p.ids64, n);
+  const bool known = id >= 0 && id < p.classes, zero = p.zero_padding && id == p.padding;
+  const T* row = (const T*)p.table.p + (known ? id : 0) * p.table.sr;
+  RawVec<T, VEC> raw[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = ((2 * blockIdx.y + i) * TPR + t) * VEC;
+    if (known && c < p.width) raw[i].load(row + c);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = ((2 * blockIdx.y + i) * TPR + t) * VEC;
+    if (c >= p.width) continue;
+    float f[VEC];
+    if (known) raw[i].get(f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = zero ? 0.f : known ? f[e] * p.scale : __builtin_nanf("");
+    raw[i].set(f);
+    raw[i].store((T*)p.out.p + n * p.out.sr + c);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ order
+// keys[r], order[r]: the token of rank r. A workgroup ranks 64 tokens, each of its 16 waves against a sixteenth of all.
+__global__ __launch_bounds__(1024) void rank_kernel(EmbedParams p, uint32_t* keys, uint32_t* order) {
+  __shared__ __align__(16) uint32_t all[kRankTokens + 64];
+  __shared__ int part[16][64];
+  const int n = (int)p.n, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int slice = (n + 63) / 64 * 4;  // tokens of a wave, a multiple of 4; 16 slices cover n
+  for (int i = threadIdx.x; i < 16 * slice; i += 1024) all[i] = i < n ? key_of(p, i) : 0xffffffffu;
+  __syncthreads();
+  const int i = blockIdx.x * 64 + lane;
+  const uint32_t mine = all[min(i, n - 1)];
+  const int j0 = wave * slice, j1 = j0 + slice;
+  // tokens of the same id count when they come earlier: compare with mine + 1 before this workgroup's tokens, mine after
+  const int own0 = blockIdx.x * 64, own1 = own0 + 64;
+  const int before = min(max(own0, j0), j1), after = min(max(own1, j0), j1);  // multiples of 4
+  int rank = 0;
+  for (int j = j0; j < before; j += 4) {
+    const u32x4_t k = *reinterpret_cast<const u32x4_t*>(all + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rank += k[e] <= mine;
+  }
+  for (int j = before; j < after; ++j) rank += all[j] < mine || (all[j] == mine && j < i);
+  for (int j = after; j < j1; j += 4) {
+    const u32x4_t k = *reinterpret_cast<const u32x4_t*>(all + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rank += k[e] < mine;
+  }
+  part[wave][lane] = rank;
+  __syncthreads();
+  if (wave == 0 && i < n) {
+    int r = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) r += part[w][lane];
+    keys[r] = mine;
+    order[r] = (uint32_t)i;
+  }
+}
+
+// One digit of the radix sort. from == nullptr: the keys are taken from the ids, the tokens in order.
+struct SortPass {
+  const uint32_t *from_key, *from_order;
+  uint32_t *to_key, *to_order;
+  uint32_t* hist;  // [tiles][digits]
+  int shift, bits, tiles;
+};
+
+__device__ __forceinline__ uint32_t sort_key(const EmbedParams& p, const SortPass& s, int64_t n) {
+  return s.from_key ? s.from_key[n] : key_of(p, n);
+}
+
+__global__ __launch_bounds__(256) void sort_count_kernel(EmbedParams p, SortPass s) {
+  __shared__ uint32_t count[kSortMost];
+  const int digits = 1 << s.bits;
+  for (int d = threadIdx.x; d < digits; d += 256) count[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll 4
+  for (int r = 0; r < kSortTile / 256; ++r) {
+    const int64_t n = base + r * 256 + threadIdx.x;
+    if (n < p.n) atomicAdd(&count[sort_key(p, s, n) >> s.shift & (digits - 1)], 1u);  // whole numbers: any order
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += 256) s.hist[(int64_t)blockIdx.x * digits + d] = count[d];
+}
+
+// Places of a tile's tokens: the tokens of smaller digits, of the same digit in earlier tiles, in earlier waves of this
+// tile (a wave takes 1024 consecutive tokens), and before it in its wave (by ballots over the digit's bits).
+__global__ __launch_bounds__(256) void sort_place_kernel(EmbedParams p, SortPass s) {
+  __shared__ uint32_t count[4][kSortMost];  // a wave's tokens of each digit so far; then the place of its first
+  __shared__ uint32_t sums[256];
+  const int digits = 1 << s.bits, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  for (int d = threadIdx.x; d < 4 * kSortMost; d += 256) count[d / kSortMost][d % kSortMost] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kSortTile + wave * (kSortTile / 4);
+  uint32_t key[16], rank[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int64_t n = base + r * 64 + lane;
+    key[r] = n < p.n ? sort_key(p, s, n) : 0;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const bool in = base + r * 64 + lane < p.n;
+    const uint32_t d = key[r] >> s.shift & (digits - 1);
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < s.bits; ++b) {
+      const uint64_t set = __ballot(d >> b & 1);
+      same &= d >> b & 1 ? set : ~set;
+    }
+    const uint32_t earlier = __popcll(same & ((1ull << lane) - 1));
+    if (in) rank[r] = count[wave][d] + earlier;
+    __builtin_amdgcn_wave_barrier();  // every lane has read the count before one of its digit raises it
+    if (in && earlier == 0) count[wave][d] += (uint32_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+  // digits 4 t .. 4 t + 3 belong to thread t: their tokens in all tiles and in the tiles before this one
+  const int per = (digits + 255) / 256;
+  uint32_t total[4] = {0, 0, 0, 0}, before[4] = {0, 0, 0, 0}, mine = 0;
+  for (int q = 0; q < per; ++q) {
+    const int d = threadIdx.x * per + q;
+    if (d >= digits) break;
+    for (int b = 0; b < s.tiles; ++b) {
+      const uint32_t h = s.hist[(int64_t)b * digits + d];
+      total[q] += h;
+      before[q] += b < (int)blockIdx.x ? h : 0;
+    }
+    mine += total[q];
+  }
+  sums[threadIdx.x] = mine;
+  __syncthreads();
+  for (int o = 1; o < 256; o *= 2) {  // inclusive scan over the threads
+    const uint32_t add = (int)threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
+    __syncthreads();
+    sums[threadIdx.x] += add;
+    __syncthreads();
+  }
+  uint32_t place = sums[threadIdx.x] - mine;
+  for (int q = 0; q < per; ++q) {
+    const int d = threadIdx.x * per + q;
+    if (d >= digits) break;
+    uint32_t at = place + before[q];
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t c = count[w][d];
+      count[w][d] = at;
+      at += c;
+    }
+    place += total[q];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int64_t n = base + r * 64 + lane;
+    if (n < p.n) {
+      const uint32_t at = count[wave][key[r] >> s.shift & (digits - 1)] + rank[r];
+      s.to_key[at] = key[r];
+      s.to_order[at] = s.from_order ? s.from_order[n] : (uint32_t)n;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ sums
+// Tokens [s, e) of the order, every `step`-th from s + first: the thread's vectors of their rows added to acc.
+template <typename T, int VEC, int NPT, int TPR>
+__device__ __forceinline__ void add_tokens(float (&acc)[NPT][VEC], const EmbedParams& p, const uint32_t* order, int64_t s, int64_t e,
+                                           int first, int step, int c0) {
+  constexpr int U = NPT > 1 ? 2 : 4;  // rows in flight
+  for (int64_t j = s + first; j < e; j += (int64_t)U * step) {
+    RawVec<T, VEC> raw[U][NPT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = j + (int64_t)u * step;
+      const T* row = (const T*)p.dout.p + (at < e ? (int64_t)order[at] : 0) * p.dout.sr;
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        const int c = c0 + i * TPR * VEC;
+        if (at < e && c < p.width)
+          raw[u][i].load(row + c);
+        else
+          raw[u][i].zero();
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        float f[VEC];
+        raw[u][i].get(f);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[i][k] += f[k];
+      }
+  }
+}
+
+// acc summed over the TEAMS teams of a workgroup in team 0's threads, in the teams' order.
+template <int VEC, int NPT, int TPR>
+__device__ __forceinline__ void join_teams(float (&acc)[NPT][VEC], float* lds) {
+  constexpr int TEAMS = 256 / TPR, PER = VEC * NPT;
+  if constexpr (TEAMS > 1) {
+    const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NPT; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) lds[(team * TPR + t) * (PER + 1) + i * VEC + k] = acc[i][k];
+    __syncthreads();
+    if (team == 0) {
+      for (int q = 1; q < TEAMS; ++q)
+#pragma unroll
+        for (int i = 0; i < NPT; ++i)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[i][k] += lds[(q * TPR + t) * (PER + 1) + i * VEC + k];
+    }
+  }
+}
+
+template <typename T, int VEC, int NPT, int TPR>
+__global__ __launch_bounds__(256) void embed_piece_kernel(EmbedParams p, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order,
+                                                          float* __restrict__ pieces) {
+  constexpr int TEAMS = 256 / TPR;
+  __shared__ float lds[TEAMS > 1 ? 256 * (VEC * NPT + 1) : 1];
+  const int64_t s = (int64_t)blockIdx.x * kPiece;
+  const uint32_t key = keys[s];
+  if (key != keys[s + kPiece - 1] || key >= p.classes) return;
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c0 = (blockIdx.y * NPT * TPR + t) * VEC;
+  float acc[NPT][VEC] = {};
+  add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, s + kPiece, team, TEAMS, c0);
+  join_teams<VEC, NPT, TPR>(acc, lds);
+  if (team != 0) return;
+#pragma unroll
+  for (int i = 0; i < NPT; ++i) {
+    const int c = c0 + i * TPR * VEC;
+    if (c < p.width) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) pieces[(int64_t)blockIdx.x * p.width + c + k] = acc[i][k];
+    }
+  }
+}
+
+// First of n sorted keys that is not below v.
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t v) {
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (keys[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+constexpr int kRowsMost = 16;  // table rows of a workgroup
+constexpr int kTeamTokens = 8;  // most tokens that one of several teams sums alone
+
+// `rows` table rows of a workgroup, one for each team in turn; rows with more tokens take all the teams.
+template <typename T, int VEC, int NPT, int TPR>
+__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order,
+                                                         const float* __restrict__ pieces, int rows) {
+  constexpr int TEAMS = 256 / TPR;
+  __shared__ float lds[TEAMS > 1 ? 256 * (VEC * NPT + 1) : 1];
+  __shared__ int64_t bound[kRowsMost + 1];
+  const int64_t v0 = (int64_t)blockIdx.x * rows;
+  if ((int)threadIdx.x <= rows) bound[threadIdx.x] = lower_bound(keys, p.n, (uint32_t)min(v0 + threadIdx.x, p.classes));
+  __syncthreads();
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c0 = (blockIdx.y * NPT * TPR + t) * VEC;
+  auto write = [&](const float(&acc)[NPT][VEC], int64_t v) {
+#pragma unroll
+    for (int i = 0; i < NPT; ++i) {
+      const int c = c0 + i * TPR * VEC;
+      if (c >= p.width) continue;
+      float f[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = acc[i][k] * p.scale;
+      RawVec<T, VEC> out;
+      out.set(f);
+      out.store((T*)p.out.p + v * p.out.sr + c);
+    }
+  };
+  const int have = (int)min((int64_t)rows, p.classes - v0);
+  if constexpr (TEAMS > 1) {
+    for (int r = team; r < have; r += TEAMS) {
+      const int64_t s = bound[r], e = bound[r + 1];
+      if (e - s > kTeamTokens) continue;
+      float acc[NPT][VEC] = {};
+      add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, e, 0, 1, c0);
+      write(acc, v0 + r);
+    }
+  }
+  for (int r = 0; r < have; ++r) {
+    const int64_t s = bound[r], e = bound[r + 1];
+    if (TEAMS > 1 && e - s <= kTeamTokens) continue;
+    const int64_t a = (s + kPiece - 1) / kPiece, b = e / kPiece;  // whole pieces [a, b)
+    float acc[NPT][VEC] = {};
+    if (a < b) {
+      add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, a * kPiece, team, TEAMS, c0);
+      for (int64_t q = a + team; q < b; q += TEAMS) {
+#pragma unroll
+        for (int i = 0; i < NPT; ++i) {
+          const int c = c0 + i * TPR * VEC;
+          if (c < p.width) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[i][k] += pieces[q * p.width + c + k];
+          }
+        }
+      }
+      add_tokens<T, VEC, NPT, TPR>(acc, p, order, b * kPiece, e, team, TEAMS, c0);
+    } else {
+      add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, e, team, TEAMS, c0);
+    }
+    join_teams<VEC, NPT, TPR>(acc, lds);
+    if (team == 0) write(acc, v0 + r);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ launches
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+int key_bits(int64_t classes) {  // keys run from 0 to classes
+  int b = 1;
+  while (b < 32 && classes >> b) ++b;
+  return b;
+}
+
+template <typename T, int VEC, int TPR>
+hipError_t fwd(const EmbedParams& p, hipStream_t st) {
+  constexpr int TEAMS = 256 / TPR, COLS = 2 * TPR * VEC;
+  embed_fwd_kernel<T, VEC, TPR><<<dim3((unsigned)((p.n + TEAMS - 1) / TEAMS), (p.width + COLS - 1) / COLS), 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+
+struct Order {
+  uint32_t *keys, *order;
+};
+
+hipError_t sort_tokens(const EmbedParams& p, Order& o, hipStream_t st) {
+  char* ws = (char*)p.ws;
+  const int64_t each = align256(4 * p.n);
+  uint32_t *key[2] = {(uint32_t*)ws, (uint32_t*)(ws + each)}, *ord[2] = {(uint32_t*)(ws + 2 * each), (uint32_t*)(ws + 3 * each)};
+  if (p.n <= kRankTokens) {
+    rank_kernel<<<dim3((unsigned)((p.n + 63) / 64)), 1024, 0, st>>>(p, key[0], ord[0]);
+    o = {key[0], ord[0]};
+    return hipGetLastError();
+  }
+  const int bits = key_bits(p.classes), passes = (bits + 9) / 10, each_bits = (bits + passes - 1) / passes;
+  const int tiles = (int)((p.n + kSortTile - 1) / kSortTile);
+  SortPass s{nullptr, nullptr, key[0], ord[0], (uint32_t*)(ws + 4 * each), 0, each_bits, tiles};
+  for (int q = 0; q < passes; ++q) {
+    s.to_key = key[q & 1], s.to_order = ord[q & 1];
+    sort_count_kernel<<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+    sort_place_kernel<<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+    s.from_key = s.to_key, s.from_order = s.to_order;
+    s.shift += each_bits;
+  }
+  o = {s.to_key, s.to_order};
+  return hipGetLastError();
+}
+
+template <typename T, int VEC, int NPT, int TPR>
+hipError_t bwd(const EmbedParams& p, hipStream_t st) {
+  constexpr int COLS = NPT * TPR * VEC;
+  const unsigned cols = (unsigned)((p.width + COLS - 1) / COLS);
+  Order o{nullptr, nullptr};
+  float* pieces = (float*)((char*)p.ws + embed_ws_bytes(p)) - p.n / kPiece * p.width;
+  if (p.n > 0) {
+    hipError_t e = sort_tokens(p, o, st);
+    if (e != hipSuccess) return e;
+    if (p.n >= kPiece) {
+      embed_piece_kernel<T, VEC, NPT, TPR><<<dim3((unsigned)(p.n / kPiece), cols), 256, 0, st>>>(p, o.keys, o.order, pieces);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+  }
+  // several rows for a workgroup (one binary search for all) once they fill the GPU
+  const int64_t per = p.classes * cols / (8 * (int64_t)device_cu_count());
+  const int rows = (int)(per < 1 ? 1 : per < kRowsMost ? per : kRowsMost);
+  embed_rows_kernel<T, VEC, NPT, TPR><<<dim3((unsigned)((p.classes + rows - 1) / rows), cols), 256, 0, st>>>(p, o.keys, o.order, pieces, rows);
+  return hipGetLastError();
+}
+
+template <typename T, bool GRAD>
+hipError_t by_width(const EmbedParams& p, hipStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int n = p.vec ? p.width / V : p.width;
+#define THERIA_EMBED_CASE(VEC, TPR)               \
+  if constexpr (GRAD)                             \
+    return bwd<T, VEC, TPR == 256 ? 2 : 1, TPR>(p, st); \
+  else                                            \
+    return fwd<T, VEC, TPR>(p, st);
+  if (p.vec) {
+    if (n <= 16) { THERIA_EMBED_CASE(V, 16) }
+    if (n <= 128) { THERIA_EMBED_CASE(V, 64) }
+    THERIA_EMBED_CASE(V, 256)
+  }
+  if (n <= 16) { THERIA_EMBED_CASE(1, 16) }
+  if (n <= 128) { THERIA_EMBED_CASE(1, 64) }
+  THERIA_EMBED_CASE(1, 256)
+#undef THERIA_EMBED_CASE
+}
+
+template <bool GRAD>
+hipError_t by_type(const EmbedParams& p, hipStream_t st) {
+  if (p.dtype == 0) return by_width<float, GRAD>(p, st);
+  if (p.dtype == 1) return by_width<_Float16, GRAD>(p, st);
+  return by_width<__bf16, GRAD>(p, st);
+}
+
+}  // namespace
+
+// Keys and order twice, the digits' counts, and a float32 row for each piece.
+int64_t embed_ws_bytes(const EmbedParams& p) {
+  const int64_t tiles = (p.n + kSortTile - 1) / kSortTile;
+  return 4 * align256(4 * p.n) + align256(4 * kSortMost * tiles) + 4 * (p.n / kPiece) * p.width;
+}
+hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st) { return by_type<false>(p, st); }
+hipError_t launch_embed_bwd(const EmbedParams& p, hipStream_t st) { return by_type<true>(p, st); }
+
+}  // namespace theria

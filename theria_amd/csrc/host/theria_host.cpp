@@ -1,4 +1,5 @@
-// Python binding of the hot C ABI entry points (theria_sdpa_fwd, _bwd, _jvp, _bwd_bwd) for torch tensors.
+// Python binding of the hot C ABI entry points (theria_sdpa_fwd, _bwd, _jvp, _bwd_bwd, and the token-side operators)
+// for torch tensors.
 //
 // The autograd operator calls these once per forward, backward, JVP and double backward. Building the
 // theria_tensor_t views, the output tensors and the stream handle here costs about a microsecond per call,
@@ -261,6 +262,184 @@ py::tuple bwd_bwd(at::Tensor q, at::Tensor k, at::Tensor v, OptT o, const at::Te
   return py::make_tuple(oq, ok, ov, odo);
 }
 
+// ---- token-side operators: matrices (rows, width), whose leading dimensions are flattened -------------------------
+
+// A tensor's rows of `width` as a matrix; a copy only where no view with a contiguous last dimension exists.
+at::Tensor rows_of(const at::Tensor& t_in, int64_t width) {
+  at::Tensor t = plain(t_in);
+  if (t.dim() != 2) t = t.reshape({t.numel() / width, width});
+  if (width > 1 && t.stride(1) != 1) t = t.contiguous();
+  return t;
+}
+at::Tensor rows_of(const at::Tensor& t, const at::Tensor& like, const char* msg) {
+  need(t.sizes() == like.sizes() && t.device() == like.device(), msg);
+  return rows_of(t.scalar_type() == like.scalar_type() ? t : t.to(like.scalar_type()), like.size(-1));
+}
+OptT rows_of(const OptT& t, const at::Tensor& like, const char* msg) {
+  if (!t) return std::nullopt;
+  return rows_of(*t, like, msg);
+}
+theria_rows_t rows_view(const at::Tensor& t) { return {t.data_ptr(), t.stride(0)}; }
+theria_rows_t rows_view(const OptT& t) { return t ? rows_view(*t) : theria_rows_t{nullptr, 0}; }
+void* ptr(const OptT& t) { return t ? plain(*t).data_ptr() : nullptr; }
+OptT flat(const OptT& t) {
+  if (!t) return std::nullopt;
+  return plain(*t).contiguous();
+}
+py::object given(const OptT& t) { return t ? py::cast(*t) : py::none(); }
+
+theria_layer_norm_problem_t norm_problem(const at::Tensor& x, at::ScalarType param, double eps) {
+  return {dtype_code(x.scalar_type()), dtype_code(param), (int32_t)x.size(1), (float)eps, x.size(0)};
+}
+
+py::tuple layer_norm_fwd(const at::Tensor& x_in, const OptT& weight_in, const OptT& bias_in, double eps) {
+  const int64_t width = x_in.size(-1);
+  const at::Tensor x = rows_of(x_in, width);
+  const OptT weight = flat(weight_in), bias = flat(bias_in);
+  const c10::hip::HIPGuard guard(x.get_device());
+  const auto y = at::empty({x.size(0), width}, x.options());
+  const auto mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+  const auto p = norm_problem(x, weight ? weight->scalar_type() : bias ? bias->scalar_type() : x.scalar_type(), eps);
+  const auto vx = rows_view(x), vy = rows_view(y);
+  check_rc(theria_layer_norm_fwd(&p, &vx, ptr(weight), ptr(bias), &vy, fptr(mean), fptr(rstd), stream_of(x)),
+           "theria_layer_norm_fwd");
+  return py::make_tuple(y.view(x_in.sizes()), mean, rstd);
+}
+
+py::tuple layer_norm_bwd(const at::Tensor& x_in, const OptT& weight_in, const at::Tensor& dout_in, const at::Tensor& mean,
+                         const at::Tensor& rstd, double eps, bool need_dx, bool need_dw, bool need_db, at::ScalarType param) {
+  const int64_t width = x_in.size(-1);
+  const at::Tensor dout = rows_of(dout_in, x_in, "the gradient must have the shape of the input");
+  const at::Tensor x = rows_of(x_in, width);
+  const OptT weight = flat(weight_in);
+  const c10::hip::HIPGuard guard(x.get_device());
+  OptT dx, dw, db, ws;
+  if (need_dx) dx = at::empty({x.size(0), width}, x.options());
+  const auto po = x.options().dtype(param);
+  const bool none = x.size(0) == 0;
+  if (need_dw) dw = none ? at::zeros({width}, po) : at::empty({width}, po);
+  if (need_db) db = none ? at::zeros({width}, po) : at::empty({width}, po);
+  if (!none) {
+    const auto p = norm_problem(x, param, eps);
+    if (need_dw || need_db) ws = at::empty({theria_layer_norm_ws_floats(&p)}, x.options().dtype(at::kFloat));
+    const auto vx = rows_view(x), vg = rows_view(dout), vdx = rows_view(dx);
+    check_rc(theria_layer_norm_bwd(&p, &vx, ptr(weight), &vg, fptr(mean), fptr(rstd), &vdx, ptr(dw), ptr(db), fptr(ws), stream_of(x)),
+             "theria_layer_norm_bwd");
+  }
+  if (dx) dx = dx->view(x_in.sizes());
+  return py::make_tuple(given(dx), given(dw), given(db));
+}
+
+py::tuple layer_norm_bwd_bwd(const at::Tensor& x_in, const OptT& weight_in, const at::Tensor& dout_in, const at::Tensor& mean,
+                             const at::Tensor& rstd, double eps, const OptT& gdx_in, const OptT& gdw_in, const OptT& gdb_in,
+                             bool need_gx, bool need_gw, bool need_gdout, at::ScalarType param) {
+  const int64_t width = x_in.size(-1);
+  const at::Tensor dout = rows_of(dout_in, x_in, "the gradient must have the shape of the input");
+  const OptT gdx = rows_of(gdx_in, x_in, "a cotangent must have the shape of the input");
+  const at::Tensor x = rows_of(x_in, width);
+  auto param_like = [&](const OptT& t) -> OptT {
+    if (!t) return std::nullopt;
+    need(t->numel() == width && t->device() == x.device(), "a cotangent must have the shape of its parameter");
+    return flat(t->scalar_type() == param ? *t : t->to(param));
+  };
+  const OptT weight = flat(weight_in), gdw = param_like(gdw_in), gdb = param_like(gdb_in);
+  const c10::hip::HIPGuard guard(x.get_device());
+  OptT gx, gw, gg, ws;
+  const bool none = x.size(0) == 0;
+  if (need_gx) gx = at::empty({x.size(0), width}, x.options());
+  if (need_gdout) gg = at::empty({x.size(0), width}, x.options());
+  if (need_gw) gw = none ? at::zeros({width}, x.options().dtype(param)) : at::empty({width}, x.options().dtype(param));
+  if (!none) {
+    const auto p = norm_problem(x, param, eps);
+    if (need_gw) ws = at::empty({theria_layer_norm_ws_floats(&p)}, x.options().dtype(at::kFloat));
+    const auto vx = rows_view(x), vg = rows_view(dout), vu = rows_view(gdx), vgx = rows_view(gx), vgg = rows_view(gg);
+    check_rc(theria_layer_norm_bwd_bwd(&p, &vx, ptr(weight), &vg, fptr(mean), fptr(rstd), &vu, ptr(gdw), ptr(gdb), &vgx, ptr(gw),
+                                       &vgg, fptr(ws), stream_of(x)),
+             "theria_layer_norm_bwd_bwd");
+  }
+  if (gx) gx = gx->view(x_in.sizes());
+  if (gg) gg = gg->view(x_in.sizes());
+  return py::make_tuple(given(gx), given(gw), given(gg));
+}
+
+at::Tensor embedding_fwd(const at::Tensor& ids_in, const at::Tensor& table_in, double scale, int64_t padding, bool zero_padding) {
+  const int64_t width = table_in.size(1);
+  const at::Tensor table = rows_of(table_in, width), ids = plain(ids_in).contiguous();
+  const c10::hip::HIPGuard guard(table.get_device());
+  const auto out = at::empty({ids.numel(), width}, table.options());
+  const theria_embedding_problem_t p{dtype_code(table.scalar_type()), ids.scalar_type() == at::kLong, (int32_t)width,
+                                     (float)scale, ids.numel(), table.size(0), padding};
+  const auto vt = rows_view(table), vo = rows_view(out);
+  check_rc(theria_embedding_fwd(&p, ids.data_ptr(), &vt, zero_padding, &vo, stream_of(table)), "theria_embedding_fwd");
+  auto sizes = ids_in.sizes().vec();
+  sizes.push_back(width);
+  return out.view(sizes);
+}
+
+at::Tensor embedding_bwd(const at::Tensor& ids_in, const at::Tensor& dout_in, int64_t classes, double scale, int64_t padding) {
+  const int64_t width = dout_in.size(-1);
+  const at::Tensor ids = plain(ids_in).contiguous(), dout = rows_of(dout_in, width);
+  need(dout.size(0) == ids.numel() && dout.device() == ids.device(), "the gradient must have one row for each id");
+  const c10::hip::HIPGuard guard(dout.get_device());
+  const auto out = at::empty({classes, width}, dout.options());
+  const theria_embedding_problem_t p{dtype_code(dout.scalar_type()), ids.scalar_type() == at::kLong, (int32_t)width,
+                                     (float)scale, ids.numel(), classes, padding};
+  const auto ws = at::empty({theria_embedding_ws_bytes(&p)}, dout.options().dtype(at::kByte));
+  const auto vg = rows_view(dout), vo = rows_view(out);
+  check_rc(theria_embedding_bwd(&p, ids.data_ptr(), &vg, &vo, ws.data_ptr(), stream_of(dout)), "theria_embedding_bwd");
+  return out;
+}
+
+theria_linear_ce_problem_t ce_problem(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, int64_t ignore, int reduction) {
+  return {dtype_code(x.scalar_type()), target.scalar_type() == at::kLong, reduction, (int32_t)x.size(1), x.size(0), weight.size(0), ignore};
+}
+
+// A 256-byte-aligned workspace: torch's allocations are.
+at::Tensor ce_workspace(const theria_linear_ce_problem_t& p, const theria_rows_t& w, const at::Tensor& x, bool backward, bool dx, bool dw, bool db) {
+  return at::empty({theria_linear_ce_ws_bytes(&p, &w, backward, dx, dw, db)}, x.options().dtype(at::kByte));
+}
+
+py::tuple linear_ce_fwd(const at::Tensor& x_in, const at::Tensor& weight_in, const OptT& bias_in, const at::Tensor& target_in,
+                        int64_t ignore, int reduction) {
+  const int64_t width = x_in.size(-1);
+  const at::Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = plain(target_in).contiguous();
+  const OptT bias = flat(bias_in);
+  const c10::hip::HIPGuard guard(x.get_device());
+  const auto f = x.options().dtype(at::kFloat);
+  const auto loss = reduction == THERIA_REDUCE_NONE ? at::empty({x.size(0)}, f) : at::empty({}, f);
+  const auto stats = at::empty({2, x.size(0)}, f);
+  const auto p = ce_problem(x, weight, target, ignore, reduction);
+  const auto vx = rows_view(x), vw = rows_view(weight);
+  const auto ws = ce_workspace(p, vw, x, false, false, false, false);
+  check_rc(theria_linear_ce_fwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), fptr(loss), fptr(stats), ws.data_ptr(), stream_of(x)),
+           "theria_linear_ce_fwd");
+  return py::make_tuple(reduction == THERIA_REDUCE_NONE ? loss.view(target_in.sizes()) : loss, stats);
+}
+
+py::tuple linear_ce_bwd(const at::Tensor& x_in, const at::Tensor& weight_in, const OptT& bias_in, const at::Tensor& target_in,
+                        const at::Tensor& stats, const at::Tensor& dloss_in, int64_t ignore, int reduction, bool need_dx, bool need_dw,
+                        bool need_db) {
+  const int64_t width = x_in.size(-1);
+  const at::Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = plain(target_in).contiguous();
+  const OptT bias = flat(bias_in);
+  const at::Tensor dloss = plain(dloss_in).to(at::kFloat).contiguous();
+  need(dloss.numel() == (reduction == THERIA_REDUCE_NONE ? x.size(0) : 1) && dloss.device() == x.device(),
+       "the loss's gradient must have the shape of the loss");
+  const c10::hip::HIPGuard guard(x.get_device());
+  OptT dx, dw, db;
+  if (need_dx) dx = at::empty({x.size(0), width}, x.options());
+  if (need_dw) dw = at::empty({weight.size(0), width}, x.options());
+  if (need_db) db = at::empty({weight.size(0)}, x.options());
+  const auto p = ce_problem(x, weight, target, ignore, reduction);
+  const auto vx = rows_view(x), vw = rows_view(weight), vdx = rows_view(dx), vdw = rows_view(dw);
+  const auto ws = ce_workspace(p, vw, x, true, need_dx, need_dw, need_db);
+  check_rc(theria_linear_ce_bwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), fptr(stats), fptr(dloss), &vdx, &vdw, ptr(db), ws.data_ptr(),
+                                stream_of(x)),
+           "theria_linear_ce_bwd");
+  if (dx) dx = dx->view(x_in.sizes());
+  return py::make_tuple(given(dx), given(dw), given(db));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_theria_host, m) {
@@ -275,4 +454,11 @@ PYBIND11_MODULE(_theria_host, m) {
   m.def("bwd_bwd", &bwd_bwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("dout"),
         py::arg("lse"), py::arg("gq"), py::arg("gk"), py::arg("gv"), py::arg("scale"), py::arg("causal"),
         py::arg("noalloc"), py::arg("out"));
+  m.def("layer_norm_fwd", &layer_norm_fwd);
+  m.def("layer_norm_bwd", &layer_norm_bwd);
+  m.def("layer_norm_bwd_bwd", &layer_norm_bwd_bwd);
+  m.def("embedding_fwd", &embedding_fwd);
+  m.def("embedding_bwd", &embedding_bwd);
+  m.def("linear_ce_fwd", &linear_ce_fwd);
+  m.def("linear_ce_bwd", &linear_ce_bwd);
 }

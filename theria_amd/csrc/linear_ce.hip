@@ -1,0 +1,702 @@
+// Cross entropy of the logits z = x W^T + b of a linear head, and its gradient, without keeping the logits (gfx950).
+//
+//   forward    loss_n = log sum_v exp(z_nv) - z_{n, t_n}
+//   backward   dz = (softmax(z) - onehot(t)) g_n;   dx = dz W,   dW = dz^T x,   db = sum_n dz
+//
+// Rows whose target is ignored cost nothing: a first launch lists the kept rows, a second one gathers them, and every
+// product runs over those alone (what an ignored row holds is never read). Forward: tiles of z stay in the accumulators
+// of the product, whose epilogue takes the largest logit and the sum of exponentials of each row over the tile's classes;
+// a small launch joins the tiles. Backward: for a piece of the vocabulary at a time, z is formed again, dz leaves the
+// epilogue in 16 bits, and two products turn the piece's dz into its rows of dW and its share of dx, which is summed in
+// float32. 8 N V D operations, two of them the recomputed logits; the workspace is the piece's dz, whatever the vocabulary.
+//
+// dz enters the products in the inputs' 16-bit type, as an operand of a matrix product does everywhere here: one rounding
+// of 2^-9 (bfloat16) or 2^-12 (float16) relative to each entry, under the rounding of the gradients themselves once
+// summed. It is held without the loss's own factor (1 / kept rows, or the largest |g|), which multiplies the float32 sums, and
+// in float16 times 2^14, so that probabilities down to 2^-38 do not vanish. float32 operands and dz are three bfloat16
+// planes each (token_gemm.hpp).
+#include "token_common.hpp"
+#include "token_gemm.hpp"
+#include "token_params.hpp"
+
+namespace theria {
+namespace {
+
+constexpr int64_t kPieceBytes = int64_t(256) << 20;  // most of a piece's dz (and of a piece of W laid out anew)
+
+// ------------------------------------------------------------------------------------------ rows
+struct Meta {
+  int kept;
+  float most;    // largest finite |g| of the kept rows (kCeNone)
+  float factor;  // of the float32 sums that become gradients
+};
+
+constexpr int kScanPer = 4;
+
+// map: the kept rows in order, then from the end the dropped ones, ignored as n, invalid as -n - 1. target: of the kept.
+__global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward, int* map, int* target, Meta* meta) {
+  __shared__ int wave_kept[2][16];
+  __shared__ float wave_most[16];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  int64_t kept = 0;  // before this round's rows
+  float most = 0.f;
+  int turn = 0;
+  for (int64_t base = 0; base < p.n; base += 1024 * kScanPer, turn ^= 1) {
+    const int64_t n0 = base + threadIdx.x * kScanPer;
+    int64_t t[kScanPer];
+    bool keep[kScanPer], drop[kScanPer];
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < kScanPer; ++u) {
+      const int64_t n = n0 + u;
+      const bool in = n < p.n;
+      t[u] = !in ? 0 : p.target64 ? ((const int64_t*)p.target)[n] : (int64_t)((const int32_t*)p.target)[n];
+      const bool valid = t[u] != p.ignore && t[u] >= 0 && t[u] < p.classes;
+      keep[u] = in && valid;
+      drop[u] = in && !valid;
+      mine += keep[u];
+      if (backward && p.reduction == kCeNone && keep[u]) {
+        const float g = fabsf(p.gout[n]);
+        if (g < THERIA_INF) most = fmaxf(most, g);
+      }
+    }
+    int upto = mine;  // inclusive sum over the wave's lanes
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int add = __shfl_up(upto, o);
+      if (lane >= o) upto += add;
+    }
+    if (lane == 63) wave_kept[turn][wave] = upto;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      before += w < wave ? wave_kept[turn][w] : 0;
+      all += wave_kept[turn][w];
+    }
+    int64_t at = kept + before + upto - mine;
+#pragma unroll
+    for (int u = 0; u < kScanPer; ++u) {
+      const int64_t n = n0 + u;
+      if (keep[u]) {
+        map[at] = (int)n;
+        target[at] = (int)t[u];
+        ++at;
+      } else if (drop[u]) {
+        map[p.n - 1 - (n - at)] = t[u] == p.ignore ? (int)n : (int)(-n - 1);
+      }
+    }
+    kept += all;
+  }
+  most = fmaxf(most, __shfl_xor(most, 1));
+#pragma unroll
+  for (int o = 2; o < 64; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
+  if (lane == 0) wave_most[wave] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 16; ++w) most = fmaxf(most, wave_most[w]);
+    meta->kept = (int)kept;
+    meta->most = most;
+    if (backward) {
+      const float unit = p.dtype == 1 ? 0x1p-14f : 1.f;
+      // no kept row: zero, not the zero over zero of an empty mean
+      meta->factor = kept == 0 ? 0.f : unit * (p.reduction == kCeNone ? most : p.reduction == kCeMean ? p.gout[0] / (float)kept : p.gout[0]);
+    }
+  }
+}
+
+// Rows laid out for the products: `width` elements, zeros up to kp; float32 in three planes. With map: the kept rows of src.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int width, const int* map, const Meta* meta, char* out, int kp, int64_t plane) {
+  const int lane = threadIdx.x % 64;
+  const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (i >= (map ? (int64_t)meta->kept : rows)) return;
+  const T* row = (const T*)src.p + (map ? (int64_t)map[i] : i) * src.sr;
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vec = width % V == 0 && src.sr % V == 0 && (uintptr_t)src.p % 16 == 0;
+  for (int c = lane * 8; c < kp; c += 512) {
+    T v[8];
+    if (vec && c + 8 <= width) {
+#pragma unroll
+      for (int q = 0; q < 8 / V; ++q) *reinterpret_cast<u32x4_t*>(v + q * V) = *reinterpret_cast<const u32x4_t*>(row + c + q * V);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < width ? row[c + e] : (T)0.f;
+    }
+    char* to = out + i * kp * 2 + c * 2;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(v);
+    } else {
+      bf16x8_t h, m, l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 a, b, d;
+        split3(v[e], a, b, d);
+        h[e] = a, m[e] = b, l[e] = d;
+      }
+      *reinterpret_cast<bf16x8_t*>(to) = h;
+      *reinterpret_cast<bf16x8_t*>(to + plane) = m;
+      *reinterpret_cast<bf16x8_t*>(to + 2 * plane) = l;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ epilogues
+__device__ __forceinline__ float bias_at(const void* bias, int dtype, int64_t v) {
+  return dtype == 0 ? ((const float*)bias)[v] : dtype == 1 ? (float)((const _Float16*)bias)[v] : (float)((const __bf16*)bias)[v];
+}
+
+// z + bias in place; classes past the piece's end become -inf.
+template <class S>
+__device__ __forceinline__ void finish_logits(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, const void* bias, int dtype, int64_t v0) {
+  const int g = (threadIdx.x >> 5) & 1;
+  if (bias || t.i0 + 32 * S::FI > t.I) {
+#pragma unroll
+    for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = t.i0 + 32 * fi + acc_row(r, g);
+        const bool in = i < t.I;
+        const float b = bias && in ? bias_at(bias, dtype, v0 + i) : 0.f;
+#pragma unroll
+        for (int fj = 0; fj < S::FJ; ++fj) z[fi][fj][r] = in ? z[fi][fj][r] + b : -THERIA_INF;
+      }
+  }
+}
+
+// Forward: of each row (column j of the tile) the largest logit over the tile's classes and the sum of
+// exp(logit - largest), and the target's logit where it lies in the tile.
+struct LogitStats {
+  const void* bias;
+  int dtype;
+  int64_t v0;         // the piece's first class
+  const int* target;
+  float* at_target;   // one of each kept row
+  float2* part;       // [tile][n]
+  int64_t n;
+  int tile0;          // the piece's first tile
+
+  template <class S>
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    __shared__ float2 red[S::WI][S::TJ];
+    const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+    finish_logits<S>(z, t, bias, dtype, v0);
+#pragma unroll
+    for (int fj = 0; fj < S::FJ; ++fj) {
+      const int j = t.j0 + 32 * fj + li;
+      if (j < t.J) {
+        const int64_t want = (int64_t)target[j] - v0 - t.i0;
+        if (want >= 0 && want < 32 * S::FI) {
+#pragma unroll
+          for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (want == 32 * fi + acc_row(r, g)) at_target[j] = z[fi][fj][r];
+        }
+      }
+      float top = -THERIA_INF;
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, z[fi][fj][r]);
+      top = pair_max(top);
+      const float off = top == -THERIA_INF ? 0.f : top;  // nothing but -inf: a sum of zeros
+      float sum = 0.f;
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += fast_exp2((z[fi][fj][r] - off) * kLog2e);
+      sum = pair_sum(sum);
+      if (g == 0) red[t.wave_i][t.wave_j * (S::TJ / S::WJ) + 32 * fj + li] = float2{top, sum};
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < S::TJ; c += S::NW * 64) {
+      const int j = t.tile_j * S::TJ + c;
+      if (j >= t.J) continue;
+      float top = red[0][c].x;
+#pragma unroll
+      for (int w = 1; w < S::WI; ++w) top = fmaxf(top, red[w][c].x);
+      const float off = top == -THERIA_INF ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < S::WI; ++w) {
+        const float2 v = red[w][c];
+        sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));  // v.y is 0 there, or NaN
+      }
+      part[(int64_t)(tile0 + t.tile_i) * n + j] = float2{top, sum};
+    }
+  }
+};
+
+// Backward: dz of the tile, in 16 bits (three planes for float32 inputs), rows j of ld elements.
+template <int PLANES>
+struct LogitGrad {
+  const void* bias;
+  int dtype;
+  int64_t v0;
+  const int *target, *map;
+  const float* stats;  // [2][n]: largest logit, sum
+  int64_t n;
+  const float* gout;   // of each row (kCeNone), or null: 1
+  const Meta* meta;
+  char* dz;
+  int ld;              // the piece's classes rounded up to 64: the rest are zeros
+  int64_t plane;
+
+  template <class S>
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    using H = typename S::H;
+    const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+    finish_logits<S>(z, t, bias, dtype, v0);
+#pragma unroll
+    for (int fj = 0; fj < S::FJ; ++fj) {
+      const int j = t.j0 + 32 * fj + li;
+      if (j >= t.J) continue;
+      const float top = stats[j], inv = 1.0f / stats[n + j];
+      float unit = __is_same(H, _Float16) ? 0x1p14f : 1.f;
+      if (gout) {
+        const float go = gout[map[j]], most = meta->most;
+        // a gradient that is not finite keeps its own value: it is not in `most`
+        unit *= !(fabsf(go) < THERIA_INF) ? go : most > 0.f ? go / most : 0.f;
+      }
+      const int64_t want = (int64_t)target[j] - v0;
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
+          if (i >= ld) continue;
+          H out[PLANES][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = fast_exp2((z[fi][fj][4 * q + e] - top) * kLog2e) * inv;
+            if (want == i + e) v -= 1.f;
+            v = i + e < t.I ? v * unit : 0.f;
+            if constexpr (PLANES == 1)
+              out[0][e] = (H)v;
+            else
+              split3(v, out[0][e], out[1][e], out[2][e]);
+          }
+#pragma unroll
+          for (int k = 0; k < PLANES; ++k)
+            *reinterpret_cast<uint2*>(dz + k * plane + ((int64_t)j * ld + i) * 2) = *reinterpret_cast<const uint2*>(out[k]);
+        }
+    }
+  }
+};
+
+// float32 sums, one set for each part of k: [split][J][ld], added to what is there or written.
+struct SumTile {
+  float* sums;
+  int64_t rows;  // of a split
+  int ld;        // a multiple of 4
+  bool add;
+
+  template <class S>
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int fj = 0; fj < S::FJ; ++fj) {
+      const int j = t.j0 + 32 * fj + li;
+      if (j >= t.J) continue;
+      float* row = sums + (t.split * rows + j) * ld;
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
+          if (i >= ld) continue;
+          f32x4_t v = {z[fi][fj][4 * q], z[fi][fj][4 * q + 1], z[fi][fj][4 * q + 2], z[fi][fj][4 * q + 3]};
+          if (add) v += *reinterpret_cast<const f32x4_t*>(row + i);
+          *reinterpret_cast<f32x4_t*>(row + i) = v;
+        }
+    }
+  }
+};
+
+// The tile times the factor, in the output's type.
+template <typename T>
+struct OutTile {
+  T* out;
+  int64_t sr;
+  bool vec;  // four elements at a time
+  const Meta* meta;
+
+  template <class S>
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+    const float f = meta->factor;
+#pragma unroll
+    for (int fj = 0; fj < S::FJ; ++fj) {
+      const int j = t.j0 + 32 * fj + li;
+      if (j >= t.J) continue;
+      T* row = out + j * sr;
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
+          T v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (T)(z[fi][fj][4 * q + e] * f);
+          if (vec) {
+            if (i < t.I) {
+              if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<uint2*>(row + i) = *reinterpret_cast<const uint2*>(v);
+              else
+                *reinterpret_cast<u32x4_t*>(row + i) = *reinterpret_cast<const u32x4_t*>(v);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < t.I) row[i + e] = v[e];
+          }
+        }
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------ joins
+// Eight rows a workgroup, their tiles spread over 32 threads each. Dropped rows: zero, or NaN where the target is invalid.
+__global__ __launch_bounds__(256) void ce_join_kernel(CeParams p, int tiles, const float2* part, const float* at_target, const int* map,
+                                                      const Meta* meta, float* row_loss) {
+  __shared__ float2 red[32][9];
+  const int r = threadIdx.x % 8, s = threadIdx.x / 8;
+  const int64_t j = (int64_t)blockIdx.x * 8 + r;
+  const int kept = meta->kept;
+  float top = -THERIA_INF, sum = 0.f;
+  if (j < kept) {
+    for (int k = s; k < tiles; k += 32) top = fmaxf(top, part[(int64_t)k * p.n + j].x);
+    const float off = top == -THERIA_INF ? 0.f : top;
+    for (int k = s; k < tiles; k += 32) {
+      const float2 v = part[(int64_t)k * p.n + j];
+      sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));
+    }
+  }
+  red[s][r] = float2{top, sum};
+  __syncthreads();
+  if (s != 0 || j >= p.n) return;
+  if (j >= kept) {
+    if (row_loss) {
+      const int row = map[j];
+      row_loss[row < 0 ? -row - 1 : row] = row < 0 ? __builtin_nanf("") : 0.f;
+    }
+    return;
+  }
+  for (int k = 1; k < 32; ++k) top = fmaxf(top, red[k][r].x);
+  const float off = top == -THERIA_INF ? 0.f : top;
+  sum = 0.f;
+  for (int k = 0; k < 32; ++k) {
+    const float2 v = red[k][r];
+    sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));
+  }
+  p.stats[j] = top;
+  p.stats[p.n + j] = sum;
+  if (row_loss) row_loss[map[j]] = logf(sum) - (at_target[j] - top);
+}
+
+// The mean or sum of the rows' losses, by one workgroup in a fixed order.
+__global__ __launch_bounds__(1024) void ce_total_kernel(CeParams p, const float* row_loss, const Meta* meta) {
+  __shared__ float red[16];
+  float s[1] = {0.f};
+  for (int64_t n = threadIdx.x; n < p.n; n += 1024) s[0] += row_loss[n];
+  team_sum<1024, 1>(s, red);
+  if (threadIdx.x == 0) p.loss[0] = p.reduction == kCeMean ? s[0] / (float)meta->kept : s[0];
+}
+
+// out[row] = the sum over the splits of sums[split][i], times the factor. map: rows as in ce_rows_kernel, dropped ones
+// zero (NaN where the target is invalid); without: row i.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_join_rows_kernel(const float* sums, int splits, int64_t rows, int ld, int width, const int* map,
+                                                           const Meta* meta, T* out, int64_t sr, bool vec) {
+  const int lane = threadIdx.x % 64;
+  const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (i >= rows) return;
+  int64_t row = i;
+  bool have = true;
+  float fill = 0.f;
+  if (map) {
+    const int m = map[i];
+    have = i < meta->kept;
+    row = m < 0 ? -(int64_t)m - 1 : m;
+    fill = m < 0 ? __builtin_nanf("") : 0.f;
+  }
+  const float f = meta->factor;
+  for (int c = lane * 4; c < width; c += 256) {
+    f32x4_t v = {fill, fill, fill, fill};
+    if (have) {
+      v = *reinterpret_cast<const f32x4_t*>(sums + i * ld + c);
+      for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
+      v *= f;
+    }
+    T o[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    T* to = out + row * sr + c;
+    if (vec) {
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(o);
+      else
+        *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < width) to[e] = o[e];
+    }
+  }
+}
+
+// Column sums of a piece's dz: a thread adds eight columns over its share of the kept rows.
+template <typename H, int PLANES>
+__global__ __launch_bounds__(256) void ce_bias_kernel(const char* dz, int ld, int64_t plane, const Meta* meta, float* part) {
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 8, kept = meta->kept;
+  if (c >= ld) return;
+  const int per = (kept + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = min(kept, r0 + per);
+  float s[8] = {};
+#pragma unroll 4
+  for (int r = r0; r < r1; ++r) {
+#pragma unroll
+    for (int k = PLANES - 1; k >= 0; --k) {
+      RawVec<H, 8> v;
+      v.load((const H*)(dz + k * plane) + (int64_t)r * ld + c);
+      float f[8];
+      v.get(f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += f[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[(int64_t)blockIdx.y * ld + c + e] = s[e];
+}
+
+// ------------------------------------------------------------------------------------------ layout of a call
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// Product tiles: by how many tokens there are, and whether large tiles fill the GPU (a workgroup of 256 x 256 holds a CU by
+// itself and reads half the operand bytes of 128 x 128 for each product).
+enum class Tile { kFew, kMid, kLarge };
+Tile tile_for(int64_t I, int64_t J, bool few_columns) {
+  if (few_columns && J <= 64) return Tile::kFew;
+  return up(I, 256) / 256 * (up(J, 256) / 256) * 5 >= (int64_t)device_cu_count() * 4 ? Tile::kLarge : Tile::kMid;
+}
+int tile_i(Tile t) { return t == Tile::kLarge ? 256 : 128; }
+int tile_j(Tile t) { return t == Tile::kLarge ? 256 : t == Tile::kMid ? 128 : 64; }
+
+// Parts of k so that the tiles of I x J fill the GPU, each at least 8 steps long.
+int splits_for(int64_t I, int64_t J, int64_t K, Tile t) {
+  const int64_t tiles = up(I, tile_i(t)) / tile_i(t) * (up(J, tile_j(t)) / tile_j(t)), most = K / (8 * kGemmK);
+  const int64_t want = (2 * (int64_t)device_cu_count() + tiles - 1) / tiles;
+  return (int)(tiles >= device_cu_count() || most < 2 ? 1 : want < most ? (want < 32 ? want : 32) : (most < 32 ? most : 32));
+}
+
+// Where everything lies in the workspace.
+struct Layout {
+  bool planes;      // float32: operands in three bfloat16 planes
+  bool lay_w;       // W is laid out anew, a piece at a time
+  int kp;           // width rounded up to 64
+  int64_t piece;    // classes of a piece
+  int ldz;          // of a piece's dz
+  Tile tf, tx, tw;  // tiles of the logits, dx, dW
+  int sx, sw;       // splits of dx, dW
+  int ldx;          // of the float32 sums
+  int tiles;        // of classes, over all pieces
+  int bias_parts;
+  int64_t map, target, meta, xs, at_target, part, row_loss, ws_w, dz, sum_x, sum_w, bias_part, bytes;
+};
+
+Layout layout_of(const CeParams& p, bool backward) {
+  Layout l{};
+  l.planes = p.dtype == 0;
+  const int np = l.planes ? 3 : 1;
+  l.kp = (int)up(p.width, 64);
+  // the copies take 16-byte pieces and 32-bit offsets inside a tile
+  l.lay_w = l.planes || p.width % 8 || p.w.sr % 8 || (uintptr_t)p.w.p % 16 || p.w.sr > (1 << 21);
+  l.piece = up(p.classes, 64);
+  auto limit = [&](int64_t row_bytes) {  // bytes of one class
+    const int64_t most = kPieceBytes / row_bytes / 256 * 256;
+    if (l.piece > most) l.piece = most < 256 ? 256 : most;
+  };
+  if (l.lay_w) limit(2 * np * (int64_t)l.kp);
+  if (backward && p.n > 0) limit(2 * np * p.n);
+  l.ldz = (int)l.piece;
+  l.tf = tile_for(l.piece, p.n, true);
+  l.tx = tile_for(p.width, p.n, true);
+  l.tw = tile_for(p.width, l.piece, false);
+  l.sx = splits_for(p.width, p.n, l.piece, l.tx);
+  l.sw = splits_for(p.width, l.piece, p.n, l.tw);
+  l.ldx = (int)up(p.width, 4);
+  l.bias_parts = (int)(p.n < 64 ? 1 : p.n / 64 < 64 ? p.n / 64 : 64);
+  for (int64_t v = 0; v < p.classes; v += l.piece)
+    l.tiles += (int)(up(p.classes - v < l.piece ? p.classes - v : l.piece, tile_i(l.tf)) / tile_i(l.tf));
+  auto take = [&](int64_t bytes) {
+    const int64_t at = l.bytes;
+    l.bytes += up(bytes, 256);
+    return at;
+  };
+  l.meta = take(sizeof(Meta));
+  l.map = take(4 * p.n);
+  l.target = take(4 * p.n);
+  l.xs = take(2 * np * p.n * l.kp);
+  if (l.lay_w) l.ws_w = take(2 * np * l.piece * l.kp);
+  if (!backward) {
+    l.at_target = take(4 * p.n);
+    l.part = take(8 * l.tiles * p.n);
+    l.row_loss = take(4 * p.n);
+  } else {
+    l.dz = take(2 * np * p.n * l.ldz);
+    if (p.dx.p) l.sum_x = take(4 * l.sx * p.n * l.ldx);
+    if (p.dw.p && l.sw > 1) l.sum_w = take(4 * l.sw * l.piece * l.ldx);
+    if (p.db) l.bias_part = take(4 * (int64_t)l.bias_parts * l.ldz);
+  }
+  return l;
+}
+
+template <typename T>
+struct HalfOf {
+  using type = T;
+};
+template <>
+struct HalfOf<float> {
+  using type = __bf16;
+};
+
+template <typename H, bool A, bool B, class Epi>
+hipError_t gemm(Tile t, const GemmParams& g, const Epi& e, hipStream_t st) {
+  switch (t) {
+    case Tile::kLarge: return launch_gemm<GemmShape<H, 256, 256, 2, 4, A, B>>(g, e, st);
+    case Tile::kMid: return launch_gemm<GemmShape<H, 128, 128, 2, 2, A, B>>(g, e, st);
+    case Tile::kFew:
+      if constexpr (!B) return launch_gemm<GemmShape<H, 128, 64, 4, 1, A, B>>(g, e, st);
+  }
+  return hipErrorInvalidValue;
+}
+
+#define THERIA_TRY(call)                \
+  do {                                  \
+    const hipError_t e_ = (call);       \
+    if (e_ != hipSuccess) return e_;    \
+  } while (0)
+
+template <typename T>
+struct Call {
+  using H = typename HalfOf<T>::type;
+  const CeParams& p;
+  const Layout l;
+  hipStream_t st;
+  char* ws;
+  int* map;
+  int* target;
+  Meta* meta;
+
+  Call(const CeParams& p_, bool backward, hipStream_t st_)
+      : p(p_), l(layout_of(p_, backward)), st(st_), ws((char*)p_.ws), map((int*)(ws + l.map)), target((int*)(ws + l.target)), meta((Meta*)(ws + l.meta)) {}
+
+  int64_t plane_x() const { return 2 * p.n * l.kp; }
+  int64_t plane_w() const { return 2 * l.piece * l.kp; }
+  int64_t plane_z() const { return 2 * p.n * l.ldz; }
+  int segments() const { return l.planes ? 6 : 1; }
+  GemmOperand x_operand(bool across) const {
+    return {ws + l.xs, 2 * (int64_t)l.kp, plane_x(), across ? l.kp : (int)p.n};
+  }
+  GemmOperand z_operand(bool across) const { return {ws + l.dz, 2 * (int64_t)l.ldz, plane_z(), across ? l.ldz : (int)p.n}; }
+  // classes [v, v + have)
+  GemmOperand w_operand(bool across, int64_t v, int have) const {
+    if (l.lay_w) return {ws + l.ws_w, 2 * (int64_t)l.kp, plane_w(), across ? l.kp : have};
+    return {(const char*)p.w.p + v * p.w.sr * 2, 2 * p.w.sr, 0, across ? p.width : have};
+  }
+
+  hipError_t rows(bool backward) {
+    ce_rows_kernel<<<1, 1024, 0, st>>>(p, backward, map, target, meta);
+    THERIA_TRY(hipGetLastError());
+    if (p.n == 0) return hipSuccess;
+    ce_lay_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, ws + l.xs, l.kp, plane_x());
+    return hipGetLastError();
+  }
+  hipError_t lay_piece(int64_t v, int have) {
+    if (!l.lay_w) return hipSuccess;
+    const Rows src{(const T*)p.w.p + v * p.w.sr, p.w.sr};
+    ce_lay_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, ws + l.ws_w, l.kp, plane_w());
+    return hipGetLastError();
+  }
+
+  hipError_t forward() {
+    THERIA_TRY(rows(false));
+    int tile0 = 0;
+    for (int64_t v = 0; v < p.classes && p.n > 0; v += l.piece) {
+      const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
+      THERIA_TRY(lay_piece(v, have));
+      const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, segments(), &meta->kept, true, false};
+      const LogitStats e{p.bias, p.dtype, v, target, (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
+      THERIA_TRY((gemm<H, false, false>(l.tf, g, e, st)));
+      tile0 += (int)(up(have, tile_i(l.tf)) / tile_i(l.tf));
+    }
+    float* row_loss = p.reduction == kCeNone ? p.loss : (float*)(ws + l.row_loss);
+    if (p.n > 0) ce_join_kernel<<<dim3((unsigned)((p.n + 7) / 8)), 256, 0, st>>>(p, l.tiles, (const float2*)(ws + l.part), (const float*)(ws + l.at_target), map, meta, row_loss);
+    THERIA_TRY(hipGetLastError());
+    if (p.reduction != kCeNone) ce_total_kernel<<<1, 1024, 0, st>>>(p, row_loss, meta);
+    return hipGetLastError();
+  }
+
+  hipError_t backward() {
+    constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+    THERIA_TRY(rows(true));
+    const bool w4 = p.width % 4 == 0;
+    for (int64_t v = 0; v < p.classes; v += l.piece) {
+      const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
+      THERIA_TRY(lay_piece(v, have));
+      {
+        const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, segments(), &meta->kept, true, false};
+        const LogitGrad<PLANES> e{p.bias, p.dtype, v, target, map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, ws + l.dz, l.ldz, plane_z()};
+        THERIA_TRY((gemm<H, false, false>(l.tf, g, e, st)));
+      }
+      if (p.dx.p) {
+        const GemmParams g{w_operand(true, v, have), z_operand(false), p.width, (int)p.n, have, l.sx, segments(), &meta->kept, true, false};
+        const SumTile e{(float*)(ws + l.sum_x), p.n, l.ldx, v > 0};
+        THERIA_TRY((gemm<H, true, false>(l.tx, g, e, st)));
+      }
+      if (p.dw.p) {
+        T* out = (T*)p.dw.p + v * p.dw.sr;
+        const bool vec = w4 && p.dw.sr % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
+        const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.sw, segments(), &meta->kept, false, true};
+        if (l.sw == 1) {
+          THERIA_TRY((gemm<H, true, true>(l.tw, g, OutTile<T>{out, p.dw.sr, vec, meta}, st)));
+        } else {
+          float* sums = (float*)(ws + l.sum_w);
+          THERIA_TRY((gemm<H, true, true>(l.tw, g, SumTile{sums, l.piece, l.ldx, false}, st)));
+          ce_join_rows_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(sums, l.sw, l.piece, l.ldx, p.width, nullptr, meta, out, p.dw.sr, vec);
+          THERIA_TRY(hipGetLastError());
+        }
+      }
+      if (p.db) {
+        float* part = (float*)(ws + l.bias_part);
+        ce_bias_kernel<H, PLANES><<<dim3((unsigned)((l.ldz + 2047) / 2048), (unsigned)l.bias_parts), 256, 0, st>>>(ws + l.dz, l.ldz, plane_z(), meta, part);
+        THERIA_TRY(hipGetLastError());
+        column_sum_kernel<T><<<dim3((unsigned)((l.ldz + 63) / 64)), 1024, 0, st>>>(part, l.bias_parts, l.ldz, have, (T*)p.db + v, nullptr, &meta->factor);
+        THERIA_TRY(hipGetLastError());
+      }
+    }
+    if (p.dx.p && p.n > 0) {
+      const bool vec = w4 && p.dx.sr % 4 == 0 && (uintptr_t)p.dx.p % (4 * sizeof(T)) == 0;
+      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>((const float*)(ws + l.sum_x), l.sx, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, vec);
+      THERIA_TRY(hipGetLastError());
+    }
+    return hipSuccess;
+  }
+};
+
+template <typename T>
+hipError_t run(const CeParams& p, bool backward, hipStream_t st) {
+  Call<T> c(p, backward, st);
+  return backward ? c.backward() : c.forward();
+}
+
+hipError_t by_type(const CeParams& p, bool backward, hipStream_t st) {
+  if (p.dtype == 0) return run<float>(p, backward, st);
+  if (p.dtype == 1) return run<_Float16>(p, backward, st);
+  return run<__bf16>(p, backward, st);
+}
+
+}  // namespace
+
+int64_t ce_ws_bytes(const CeParams& p, bool backward) { return layout_of(p, backward).bytes; }
+hipError_t launch_ce_fwd(const CeParams& p, hipStream_t st) { return by_type(p, false, st); }
+hipError_t launch_ce_bwd(const CeParams& p, hipStream_t st) { return by_type(p, true, st); }
+
+}  // namespace theria

@@ -1,0 +1,212 @@
+// Matrix products of 16-bit operands for the linear cross entropy: C[i][j] = sum_k A[i][k] B[j][k] on MFMA (gfx950).
+//
+// Either operand lies in memory "along k" (rows i, k contiguous) or "across k" (rows k, i contiguous); the second kind is
+// transposed on its way from LDS to registers (ds_read_b64_tr_b16), so that no transposed copy is ever made. A workgroup
+// owns a tile of TI x TJ results, walks k in steps of 64 and keeps two stages of both operands in LDS, filled by LDS DMA:
+// the next step's copies run while this step's products do.
+//
+// float32 operands come as three bfloat16 planes each, x = h + m + l (split3); their product is six passes over k with the
+// planes (m m, l h, h l, m h, h m, h h), the smallest first: the dropped terms are at most 2^-24 of the product.
+//
+// The accumulators have i along registers and j along lanes: lane l holds column j = l % 32 of a 32 x 32 block and four
+// consecutive i in each group of four registers, so sums over i stay inside a lane and i is written in pieces of four.
+#pragma once
+
+#include "sdpa_lds.hpp"
+
+namespace theria {
+
+constexpr int kGemmK = 64;  // k per step
+
+struct GemmOperand {
+  const char* base;
+  int64_t ld;     // bytes from row to row, a multiple of 16
+  int64_t plane;  // bytes from plane to plane (float32 operands)
+  int extent;     // along k: its rows (i or j); across k: its columns, a multiple of 8
+};
+
+struct GemmParams {
+  GemmOperand a, b;
+  int I, J, K;
+  int splits;       // parts of k, each a workgroup of its own
+  int segments;     // 1, or 6 for operands in three planes
+  const int* kept;  // kept rows of the problem, read on the device
+  bool j_kept, k_kept;  // J (and b's extent), or K, is *kept instead
+};
+
+// x as three bfloat16 terms, each the nearest to what is left; infinities, NaN and values that would round past the
+// largest bfloat16 keep their whole value in the first two terms.
+__device__ __forceinline__ void split3(float x, __bf16& h, __bf16& m, __bf16& l) {
+  const uint32_t u = __float_as_uint(x), e = u & 0x7fffffffu;
+  h = e > 0x7f7f0000u ? __builtin_bit_cast(__bf16, (uint16_t)(e > 0x7f800000u ? 0x7fc0u : u >> 16)) : (__bf16)x;
+  const float r = e >= 0x7f800000u ? 0.f : x - (float)h;
+  m = (__bf16)r;
+  l = (__bf16)(r - (float)m);
+}
+
+// Copies of one operand's tile: EXT x 64 elements, EXT / 8 wave instructions over NW waves. Every address is inside the
+// operand: a lane whose row, column or k lies outside uses an offset past the buffer's end and gets zeros.
+template <bool ACROSS, int EXT, int NW>
+struct GemmLoader {
+  static constexpr int NQ = EXT / 8 / NW;
+  static constexpr uint32_t kOut = 0x80000000u, kRange = 0x7fffffffu;
+  static_assert(NQ * NW * 8 == EXT && (!ACROSS || EXT % 128 == 0));
+  uint32_t off[NQ];
+  int at[NQ];  // k of what the lane copies, from the step's first
+  int wave;
+
+  __device__ __forceinline__ void init(int w, int lane, int64_t ld, int valid) {
+    wave = w;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int piece = q * NW + w;
+      if constexpr (ACROSS) {
+        const int row = piece % 16 * 4 + lane / 16, col = piece / 16 * 128 + ((lane % 16) ^ swz<128>(row)) * 8;
+        off[q] = col < valid ? (uint32_t)(row * ld) + col * 2 : kOut;
+        at[q] = row;
+      } else {
+        const int row = piece * 8 + lane / 8, chunk = (lane % 8) ^ swz<64>(row);
+        off[q] = row < valid ? (uint32_t)(row * ld) + chunk * 16 : kOut;
+        at[q] = chunk * 8;
+      }
+    }
+  }
+  // base: the tile at this step's first k, of which `left` remain.
+  __device__ __forceinline__ void issue(const char* base, char* lds, int left) const {
+    const rsrc_t r = make_rsrc(base, kRange);
+    if (left >= kGemmK) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) dma16(r, lds + (q * NW + wave) * 1024, off[q], 0);
+    } else {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) dma16(r, lds + (q * NW + wave) * 1024, at[q] < left ? off[q] : kOut, 0);
+    }
+  }
+};
+
+// Fragment of rows (or columns) r0 .. r0 + 31, k chunk c of 16, in the KLIN order for both kinds.
+template <typename H, bool ACROSS>
+__device__ __forceinline__ typename Mfma<H>::frag_t gemm_frag(const char* tile, int r0, int c) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (!ACROSS) {
+    return swz_cols<H, 64>(tile, r0 + (lane & 31), c);
+  } else {
+    const int s = lane & 15, hh = (lane >> 4) & 1, g = lane >> 5;
+    const char* sub = tile + r0 / 128 * (kGemmK * 256);
+    const int col = r0 % 128 + 16 * hh + 4 * (s & 3), k0 = 16 * c + 8 * g + (s >> 2), k1 = k0 + 4;
+    const i16x4_t a = ds_read_tr16(sub + k0 * 256 + (((col >> 3) ^ swz<128>(k0)) << 4) + (col & 7) * 2);
+    const i16x4_t b = ds_read_tr16(sub + k1 * 256 + (((col >> 3) ^ swz<128>(k1)) << 4) + (col & 7) * 2);
+    const i16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(typename Mfma<H>::frag_t, v);
+  }
+}
+
+// What a tile's epilogue gets: its place and this wave's.
+struct GemmTile {
+  int i0, j0;      // the wave's first row and column
+  int tile_i, tile_j, split;
+  int I, J, K;     // valid extents
+  int wave_i, wave_j;
+};
+
+template <typename H_, int TI_, int TJ_, int WI_, int WJ_, bool A_, bool B_>
+struct GemmShape {
+  using H = H_;
+  static constexpr int TI = TI_, TJ = TJ_, WI = WI_, WJ = WJ_, NW = WI_ * WJ_;
+  static constexpr bool A = A_, B = B_;
+  static constexpr int FI = TI_ / WI_ / 32, FJ = TJ_ / WJ_ / 32;
+};
+
+template <class S, class Epi>
+__global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi) {
+  using H = typename S::H;
+  constexpr int TI = S::TI, TJ = S::TJ, FI = S::FI, FJ = S::FJ, NW = S::NW;
+  // two stages as arrays of their own, so that the reads of one are known not to wait for the copies into the other
+  __shared__ __align__(1024) char a0[TI * 128], b0[TJ * 128], a1[TI * 128], b1[TJ * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // Place. Workgroups go round the eight XCDs, each with an L2 of its own: an XCD takes a run of consecutive tiles, in
+  // which groups of eight columns of tiles are walked row by row, so that its workgroups share their operands' rows.
+  const int kept = (p.j_kept || p.k_kept) ? *p.kept : 0;
+  const int J = p.j_kept ? kept : p.J, K = p.k_kept ? kept : p.K;
+  const int ni = (p.I + TI - 1) / TI, nj = (J + TJ - 1) / TJ, total = ni * nj * p.splits;
+  const int per = (total + 7) / 8, place = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || place >= total) return;
+  GemmTile t;
+  t.split = place / (ni * nj);
+  const int tile = place % (ni * nj), group = tile / (8 * ni), wide = min(8, nj - 8 * group), in = tile % (8 * ni);
+  t.tile_i = in / wide;
+  t.tile_j = 8 * group + in % wide;
+  t.I = p.I, t.J = J, t.K = K;
+  t.wave_i = wave / S::WJ, t.wave_j = wave % S::WJ;
+  t.i0 = t.tile_i * TI + t.wave_i * (TI / S::WI);
+  t.j0 = t.tile_j * TJ + t.wave_j * (TJ / S::WJ);
+
+  // this part's k, in whole steps
+  const int steps_all = (K + kGemmK - 1) / kGemmK, steps_per = (steps_all + p.splits - 1) / p.splits;
+  const int first = min(t.split * steps_per, steps_all), ksteps = min(steps_per, steps_all - first), steps = ksteps * p.segments;
+
+  const int ti0 = t.tile_i * TI, tj0 = t.tile_j * TJ;
+  GemmLoader<S::A, TI, NW> la;
+  GemmLoader<S::B, TJ, NW> lb;
+  la.init(wave, lane, p.a.ld, p.a.extent - ti0);
+  lb.init(wave, lane, p.b.ld, (p.j_kept ? kept : p.b.extent) - tj0);
+  const int64_t astep = S::A ? kGemmK * p.a.ld : 2 * kGemmK, bstep = S::B ? kGemmK * p.b.ld : 2 * kGemmK;
+  const char* abase = p.a.base + (S::A ? (int64_t)ti0 * 2 : (int64_t)ti0 * p.a.ld) + first * astep;
+  const char* bbase = p.b.base + (S::B ? (int64_t)tj0 * 2 : (int64_t)tj0 * p.b.ld) + first * bstep;
+  // planes of the segments, two bits each, the first segment lowest: a = m l h m h h, b = m h l h m h
+  const uint32_t planes_a = p.segments == 1 ? 0u : 0x049u, planes_b = p.segments == 1 ? 0u : 0x121u;
+
+  f32x16_t acc[FI][FJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) acc[i][j] = zero16();
+
+  int seg = 0, ks = 0;  // of the next step to copy
+  auto copy = [&](char* a, char* b) {
+    const int left = K - (first + ks) * kGemmK;
+    la.issue(abase + (int64_t)(planes_a >> (2 * seg) & 3) * p.a.plane + ks * astep, a, left);
+    lb.issue(bbase + (int64_t)(planes_b >> (2 * seg) & 3) * p.b.plane + ks * bstep, b, left);
+    if (++ks == ksteps) ks = 0, ++seg;
+  };
+  auto products = [&](const char* a, const char* b) {
+#pragma unroll
+    for (int c = 0; c < kGemmK / 16; ++c) {
+      typename Mfma<H>::frag_t fa[FI], fb[FJ];
+#pragma unroll
+      for (int i = 0; i < FI; ++i) fa[i] = gemm_frag<H, S::A>(a, t.wave_i * (TI / S::WI) + 32 * i, c);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) fb[j] = gemm_frag<H, S::B>(b, t.wave_j * (TJ / S::WJ) + 32 * j, c);
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) acc[i][j] = Mfma<H>::mma(fa[i], fb[j], acc[i][j]);
+    }
+  };
+  if (steps > 0) copy(a0, b0);
+  for (int s = 0; s < steps; s += 2) {
+    wait_vm_all();
+    __syncthreads();  // this stage is there for every wave, and every wave is done with the other one
+    if (s + 1 < steps) copy(a1, b1);
+    products(a0, b0);
+    if (s + 1 >= steps) break;
+    wait_vm_all();
+    __syncthreads();
+    if (s + 2 < steps) copy(a0, b0);
+    products(a1, b1);
+  }
+  epi.template run<S>(acc, t);
+}
+
+template <class S, class Epi>
+hipError_t launch_gemm(const GemmParams& p, const Epi& epi, hipStream_t st) {
+  // p.J is the most that the kept rows can be: workgroups beyond the tiles that there are return at once
+  const int64_t tiles = (int64_t)((p.I + S::TI - 1) / S::TI) * ((p.J + S::TJ - 1) / S::TJ) * p.splits;
+  if (tiles == 0) return hipSuccess;
+  if (tiles > 0x7fffff00) return hipErrorInvalidValue;
+  gemm_kernel<S, Epi><<<dim3((unsigned)((tiles + 7) / 8 * 8)), S::NW * 64, 0, st>>>(p, epi);
+  return hipGetLastError();
+}
+
+}  // namespace theria
