@@ -1,0 +1,91 @@
+"""The token-side operators together, as a training step uses them: MHAClassifier with ops="hip" against ops="torch"."""
+
+import copy
+
+import pytest
+import torch
+
+from theria_amd.autograd import hip_embedding, hip_layer_norm, hip_linear_cross_entropy, hip_sdpa
+from theria_amd.maml import meta_loss_on_tasks
+from theria_amd.models import MHAClassifier, MHAConfig
+from theria_amd.tasks import sample_token_count_task
+
+pytestmark = pytest.mark.gpu
+
+
+def _flat(grads):
+    return torch.cat([g.reshape(-1) for g in grads]).double()
+
+
+def _pair(dev):
+    torch.manual_seed(0)
+    ref = MHAClassifier(MHAConfig(), backend="reference").to(dev)
+    hip = copy.deepcopy(ref)
+    hip.set_attention_backend("hip")
+    hip.set_ops("hip")
+    return ref, hip
+
+
+def test_training_step_matches_the_reference_model(hip_device):
+    """Loss and every parameter's gradient of a step. Both sides are float32 with some hundred roundings in a row between
+    an embedding and the loss: 2^-24 times a thousand, relative to the whole gradient."""
+    ref, hip = _pair(hip_device)
+    gen = torch.Generator().manual_seed(1)
+    tokens, y = torch.randint(0, 32, (40, 64), generator=gen).to(hip_device), torch.randint(0, 5, (40,), generator=gen).to(hip_device)
+    l0, l1 = ref(tokens, y), hip(tokens, y)
+    g0 = _flat(torch.autograd.grad(l0, list(ref.parameters())))
+    g1 = _flat(torch.autograd.grad(l1, list(hip.parameters())))
+    assert abs(float(l0) - float(l1)) <= 1000 * 2**-24 * abs(float(l0))
+    assert float((g0 - g1).norm() / g0.norm()) <= 1000 * 2**-24
+    assert abs(float(torch.nn.functional.cross_entropy(hip(tokens), y)) - float(l1)) <= 1000 * 2**-24 * abs(float(l1))
+
+
+def test_full_maml_metagradient_through_the_hip_operators(hip_device):
+    """Second order through embedding, norms and attention, at the bar the attention alone is held to (1e-5)."""
+    ref, hip = _pair(hip_device)
+    gen = torch.Generator().manual_seed(0)
+    tasks = [sample_token_count_task(generator=gen, device=hip_device)[0] for _ in range(2)]
+
+    def meta(model):
+        loss = meta_loss_on_tasks(model, tasks, inner_lr=0.4, inner_steps=5)
+        return _flat(torch.autograd.grad(loss, list(model.parameters())))
+
+    a, b = meta(ref), meta(hip)
+    assert float((a - b).norm() / a.norm()) < 1e-5
+
+
+def test_one_attention_layer_in_bfloat16_end_to_end(hip_device):
+    """Embedding, norm, attention, norm and loss in bfloat16, captured with its gradients and replayed."""
+    gen = torch.Generator().manual_seed(3)
+    V, D, H, B, T = 500, 128, 2, 3, 70
+    r = lambda *s: (torch.randn(*s, generator=gen) * 0.1).bfloat16().to(hip_device).requires_grad_(True)  # noqa: E731
+    table, qkv, head = r(V, D), r(3 * D, D), r(V, D)
+    w1, w2 = (torch.ones(D, device=hip_device, dtype=torch.bfloat16, requires_grad=True) for _ in range(2))
+    ids = torch.randint(0, V, (B, T), generator=gen).to(hip_device)
+    target = torch.randint(0, V, (B, T), generator=gen).to(hip_device)
+    target[:, -10:] = -100
+    params = (table, qkv, head, w1, w2)
+
+    def step():
+        x = hip_embedding(ids, table, scale=D**0.5)
+        q, k, v = (hip_layer_norm(x, w1) @ qkv.t()).view(B, T, 3, H, D // H).permute(2, 0, 3, 1, 4)
+        x = x + hip_sdpa(q, k, v, causal=True).transpose(1, 2).reshape(B, T, D)
+        loss = hip_linear_cross_entropy(hip_layer_norm(x, w2), head, target)
+        return [loss.detach(), *torch.autograd.grad(loss, params)]
+
+    eager = step()
+    assert all(torch.isfinite(t).all() for t in eager)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, eager):
+            assert torch.equal(a, b), f"replay {i}"
+        step()

@@ -482,6 +482,7 @@ int tile_j(Tile t) { return t == Tile::kLarge ? 256 : t == Tile::kMid ? 128 : 64
 // Parts of k so that the tiles of I x J fill the GPU, each at least 8 steps long.
 int splits_for(int64_t I, int64_t J, int64_t K, Tile t) {
   const int64_t tiles = up(I, tile_i(t)) / tile_i(t) * (up(J, tile_j(t)) / tile_j(t)), most = K / (8 * kGemmK);
+  if (tiles == 0) return 1;
   const int64_t want = (2 * (int64_t)device_cu_count() + tiles - 1) / tiles;
   return (int)(tiles >= device_cu_count() || most < 2 ? 1 : want < most ? (want < 32 ? want : 32) : (most < 32 ? most : 32));
 }

@@ -4,7 +4,8 @@ Not in the reference (nearest: examples/minimal_decoder_transformer.py:82-263 an
 Token embedding (no positions: the token-count task is order-free), `layers` pre-norm blocks of
 multi-head self-attention + GELU MLP with residuals, final LayerNorm, mean-pool over tokens, linear
 head. Attention goes through sdpa_custom(backend=...), so the same weights run on the pure-PyTorch
-"reference" backend or on the HIP operator, and full MAML differentiates through it twice.
+"reference" backend or on the HIP operator, and full MAML differentiates through it twice. With ops="hip" the embedding,
+the norms and, for forward(tokens, targets), the head with its loss run on the HIP kernels too.
 """
 
 from __future__ import annotations
@@ -16,6 +17,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..attention.custom import sdpa_custom
+from ..autograd.hip_embedding import hip_embedding
+from ..autograd.hip_layer_norm import hip_layer_norm
+from ..autograd.hip_linear_ce import hip_linear_cross_entropy
 
 
 @dataclass(frozen=True)
@@ -40,22 +44,35 @@ class _Block(nn.Module):
         self.fc1 = nn.Linear(d, cfg.mlp_ratio * d)
         self.fc2 = nn.Linear(cfg.mlp_ratio * d, d)
 
-    def forward(self, x: torch.Tensor, backend: str) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, backend: str, norm) -> torch.Tensor:
         B, T, d = x.shape
         H = self.heads
-        qkv = self.qkv(self.ln1(x)).view(B, T, 3, H, d // H).permute(2, 0, 3, 1, 4)
+        qkv = self.qkv(norm(self.ln1, x)).view(B, T, 3, H, d // H).permute(2, 0, 3, 1, 4)
         att = sdpa_custom(qkv[0], qkv[1], qkv[2], backend=backend)  # (B, H, T, d/H)
         x = x + self.proj(att.transpose(1, 2).reshape(B, T, d))
-        return x + self.fc2(F.gelu(self.fc1(self.ln2(x))))
+        return x + self.fc2(F.gelu(self.fc1(norm(self.ln2, x))))
+
+
+def _torch_norm(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
+    return ln(x)
+
+
+def _hip_norm(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
+    return hip_layer_norm(x, ln.weight, ln.bias, eps=ln.eps)
 
 
 class MHAClassifier(nn.Module):
-    """token ids (B, T) -> logits (B, num_classes)."""
+    """token ids (B, T) -> logits (B, num_classes), or with targets (B,) their mean cross entropy.
 
-    def __init__(self, cfg: MHAConfig | None = None, backend: str = "reference"):
+    ops: "torch" (embedding, norms and loss of PyTorch) or "hip" (this package's kernels). forward_batched, which holds
+    a parameter set for each task, is PyTorch's either way.
+    """
+
+    def __init__(self, cfg: MHAConfig | None = None, backend: str = "reference", ops: str = "torch"):
         super().__init__()
         self.cfg = cfg or MHAConfig()
         self.backend = backend
+        self.set_ops(ops)
         self.embed = nn.Embedding(self.cfg.vocab, self.cfg.d_model)
         self.blocks = nn.ModuleList(_Block(self.cfg) for _ in range(self.cfg.layers))
         self.ln_f = nn.LayerNorm(self.cfg.d_model)
@@ -64,11 +81,23 @@ class MHAClassifier(nn.Module):
     def set_attention_backend(self, backend: str) -> None:
         self.backend = backend
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
-        x = self.embed(tokens)
+    def set_ops(self, ops: str) -> None:
+        if ops not in ("torch", "hip"):
+            raise ValueError(f"ops must be 'torch' or 'hip', got {ops!r}")
+        self.ops = ops
+
+    def forward(self, tokens: torch.Tensor, targets: torch.Tensor | None = None) -> torch.Tensor:
+        hip = self.ops == "hip"
+        norm = _hip_norm if hip else _torch_norm
+        x = hip_embedding(tokens, self.embed.weight) if hip else self.embed(tokens)
         for blk in self.blocks:
-            x = blk(x, self.backend)
-        return self.head(self.ln_f(x).mean(dim=1))
+            x = blk(x, self.backend, norm)
+        x = norm(self.ln_f, x).mean(dim=1)
+        if targets is None:
+            return self.head(x)
+        if hip:
+            return hip_linear_cross_entropy(x, self.head.weight, targets, self.head.bias)
+        return F.cross_entropy(self.head(x), targets)
 
     def forward_batched(self, params: dict, tokens: torch.Tensor) -> torch.Tensor:
         """Many parameter sets at once: params[name] is (n, *shape), tokens (n, N, T) -> logits (n, N, C).
