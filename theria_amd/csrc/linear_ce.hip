@@ -258,19 +258,29 @@ struct LogitGrad {
         // a gradient that is not finite keeps its own value: it is not in `most`
         unit *= !(fabsf(go) < THERIA_INF) ? go : most > 0.f ? go / most : 0.f;
       }
-      const int64_t want = (int64_t)target[j] - v0;
+      // softmax times the unit; classes past the piece's end have z = -inf, so zeros
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[fi][fj][r] = fast_exp2((z[fi][fj][r] - top) * kLog2e) * inv;
+      const int64_t want = (int64_t)target[j] - v0 - t.i0;
+      if (want >= 0 && want < 32 * S::FI) {
+#pragma unroll
+        for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[fi][fj][r] -= want == 32 * fi + acc_row(r, g) ? 1.f : 0.f;
+      }
+      char* row = dz + ((int64_t)j * ld + t.i0 + 4 * g) * 2;
+      const int room = ld - t.i0 - 4 * g;
 #pragma unroll
       for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
-          if (i >= ld) continue;
+          if (32 * fi + 8 * q >= room) continue;
           H out[PLANES][4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float v = fast_exp2((z[fi][fj][4 * q + e] - top) * kLog2e) * inv;
-            if (want == i + e) v -= 1.f;
-            v = i + e < t.I ? v * unit : 0.f;
+            const float v = z[fi][fj][4 * q + e] * unit;
             if constexpr (PLANES == 1)
               out[0][e] = (H)v;
             else
@@ -278,7 +288,7 @@ struct LogitGrad {
           }
 #pragma unroll
           for (int k = 0; k < PLANES; ++k)
-            *reinterpret_cast<uint2*>(dz + k * plane + ((int64_t)j * ld + i) * 2) = *reinterpret_cast<const uint2*>(out[k]);
+            *reinterpret_cast<uint2*>(row + k * plane + (32 * fi + 8 * q) * 2) = *reinterpret_cast<const uint2*>(out[k]);
         }
     }
   }

@@ -84,22 +84,41 @@ struct GemmLoader {
   }
 };
 
-// Fragment of rows (or columns) r0 .. r0 + 31, k chunk c of 16, in the KLIN order for both kinds.
-template <typename H, bool ACROSS>
-__device__ __forceinline__ typename Mfma<H>::frag_t gemm_frag(const char* tile, int r0, int c) {
-  const int lane = threadIdx.x & 63;
-  if constexpr (!ACROSS) {
-    return swz_cols<H, 64>(tile, r0 + (lane & 31), c);
-  } else {
-    const int s = lane & 15, hh = (lane >> 4) & 1, g = lane >> 5;
-    const char* sub = tile + r0 / 128 * (kGemmK * 256);
-    const int col = r0 % 128 + 16 * hh + 4 * (s & 3), k0 = 16 * c + 8 * g + (s >> 2), k1 = k0 + 4;
-    const i16x4_t a = ds_read_tr16(sub + k0 * 256 + (((col >> 3) ^ swz<128>(k0)) << 4) + (col & 7) * 2);
-    const i16x4_t b = ds_read_tr16(sub + k1 * 256 + (((col >> 3) ^ swz<128>(k1)) << 4) + (col & 7) * 2);
-    const i16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    return __builtin_bit_cast(typename Mfma<H>::frag_t, v);
+// A lane's addresses in a tile for fragments of 32 rows from row r0 + 32 f, k chunk c of 16, in the KLIN order for both
+// kinds. The swizzles separate: along k it depends on c and the lane alone (32 f rows are a constant distance), across k
+// on f and the lane (a chunk of 16 rows is), so that a few offsets serve every fragment of a step.
+template <typename H, bool ACROSS, int NF>
+struct GemmFrags {
+  static constexpr int N = ACROSS ? 2 * NF : kGemmK / 16;
+  uint32_t off[N];
+
+  __device__ __forceinline__ void init(int r0) {
+    const int lane = threadIdx.x & 63, g = lane >> 5;
+    if constexpr (!ACROSS) {
+      const int row = r0 + (lane & 31);
+#pragma unroll
+      for (int c = 0; c < N; ++c) off[c] = row * 128 + (((2 * c + g) ^ swz<64>(row)) << 4);
+    } else {
+      const int s = lane & 15, hh = (lane >> 4) & 1;
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int r = r0 + 32 * f, col = r % 128 + 16 * hh + 4 * (s & 3), k = 8 * g + 4 * b + (s >> 2);
+          off[2 * f + b] = r / 128 * (kGemmK * 256) + k * 256 + (((col >> 3) ^ swz<128>(k)) << 4) + (col & 7) * 2;
+        }
+    }
   }
-}
+  __device__ __forceinline__ typename Mfma<H>::frag_t get(const char* tile, int f, int c) const {
+    if constexpr (!ACROSS) {
+      return __builtin_bit_cast(typename Mfma<H>::frag_t, *reinterpret_cast<const i16x8_t*>(tile + off[c] + f * 4096));
+    } else {
+      const i16x4_t a = ds_read_tr16(tile + off[2 * f] + c * 4096), b = ds_read_tr16(tile + off[2 * f + 1] + c * 4096);
+      const i16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      return __builtin_bit_cast(typename Mfma<H>::frag_t, v);
+    }
+  }
+};
 
 // What a tile's epilogue gets: its place and this wave's.
 struct GemmTile {
@@ -170,31 +189,48 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
     lb.issue(bbase + (int64_t)(planes_b >> (2 * seg) & 3) * p.b.plane + ks * bstep, b, left);
     if (++ks == ksteps) ks = 0, ++seg;
   };
-  auto products = [&](const char* a, const char* b) {
+  GemmFrags<H, S::A, FI> ra;
+  GemmFrags<H, S::B, FJ> rb;
+  ra.init(t.wave_i * (TI / S::WI));
+  rb.init(t.wave_j * (TJ / S::WJ));
+  // The fragments of chunk c + 1 are read while chunk c's products run, and no earlier (the barriers bound the registers).
+  auto products = [&](const char* a, const char* b) __attribute__((always_inline)) {
+    constexpr int NC = kGemmK / 16;
+    typename Mfma<H>::frag_t fa[2][FI], fb[2][FJ];
+    auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < kGemmK / 16; ++c) {
-      typename Mfma<H>::frag_t fa[FI], fb[FJ];
+      for (int i = 0; i < FI; ++i) fa[c & 1][i] = ra.get(a, i, c);
 #pragma unroll
-      for (int i = 0; i < FI; ++i) fa[i] = gemm_frag<H, S::A>(a, t.wave_i * (TI / S::WI) + 32 * i, c);
+      for (int j = 0; j < FJ; ++j) fb[c & 1][j] = rb.get(b, j, c);
+    };
+    read(0);
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) fb[j] = gemm_frag<H, S::B>(b, t.wave_j * (TJ / S::WJ) + 32 * j, c);
+    for (int c = 0; c < NC; ++c) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (c + 1 < NC) read(c + 1);
 #pragma unroll
       for (int i = 0; i < FI; ++i)
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = Mfma<H>::mma(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < FJ; ++j) acc[i][j] = Mfma<H>::mma(fa[c & 1][i], fb[c & 1][j], acc[i][j]);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
   if (steps > 0) copy(a0, b0);
-  for (int s = 0; s < steps; s += 2) {
+  int s = 0;
+  for (; s + 2 <= steps; s += 2) {
     wait_vm_all();
     __syncthreads();  // this stage is there for every wave, and every wave is done with the other one
-    if (s + 1 < steps) copy(a1, b1);
+    copy(a1, b1);
     products(a0, b0);
-    if (s + 1 >= steps) break;
     wait_vm_all();
     __syncthreads();
     if (s + 2 < steps) copy(a0, b0);
     products(a1, b1);
+  }
+  if (s < steps) {
+    wait_vm_all();
+    __syncthreads();
+    products(a0, b0);
   }
   epi.template run<S>(acc, t);
 }
