@@ -18,8 +18,6 @@ from . import _lib
 ALLOWED_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _DTYPE_CODE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 MAX_HEAD_DIM = 128
-MAX_NORM_WIDTH = 16384
-MAX_ROW_WIDTH = 1 << 20
 
 
 def default_scale(head_dim: int) -> float:
@@ -150,28 +148,6 @@ def check_inputs(q, k, v, what: str = "theria_amd SDPA", require_v: bool = True)
         raise AssertionError(f"{what} supports 1 <= D <= {MAX_HEAD_DIM}, got D={D}")
     if max(q.shape[2], k.shape[2]) >= 2**31 or B * H >= 2**31:
         raise AssertionError(f"{what}: sizes exceed the 32-bit row index range")
-
-
-def check_matrix(t, name: str, what: str) -> None:
-    """Device, dtype and size contract of the token-side operators' matrices."""
-    if not isinstance(t, torch.Tensor):
-        raise AssertionError(f"{what}: {name} must be a tensor")
-    if not t.is_cuda:
-        raise AssertionError(f"{what} requires GPU (HIP) tensors; {name} is on {t.device}")
-    if t.dtype not in ALLOWED_DTYPES:
-        raise AssertionError(f"Unsupported dtype for {name}: {t.dtype}")
-    if t.dim() and t.numel() // max(1, t.shape[-1]) > 2**31 - 64:
-        raise AssertionError(f"{what}: {name} has more rows than 32-bit indexes reach")
-
-
-def check_indexes(t, name: str, like: torch.Tensor, what: str) -> None:
-    """Ids or targets: whole numbers on the device of `like`."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
-        raise AssertionError(f"{what}: {name} must be an int32 or int64 tensor")
-    if t.device != like.device:
-        raise AssertionError(f"{what}: {name} must be on {like.device}, got {t.device}")
-    if t.numel() > 2**31 - 64:
-        raise AssertionError(f"{what}: {name} has more elements than 32-bit indexes reach")
 
 
 def _like_rows(t: torch.Tensor | None, ref: torch.Tensor, rows: int, name: str) -> torch.Tensor | None:

@@ -13,8 +13,12 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <optional>
+#include <stdexcept>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "theria_sdpa.h"
 
@@ -262,59 +266,137 @@ py::tuple bwd_bwd(at::Tensor q, at::Tensor k, at::Tensor v, OptT o, const at::Te
   return py::make_tuple(oq, ok, ov, odo);
 }
 
-// ---- token-side operators: matrices (rows, width), whose leading dimensions are flattened -------------------------
+// ---- token-side operators -------------------------------------------------------------------------------------------
+//
+// Matrices are (rows, width) with their leading dimensions flattened. The autograd Functions are C++ too: a training step
+// of a small model is bound by the host's time per operator, and a Python Function costs several times a kernel (argument
+// packing, and the interpreter lock taken again by the engine's thread): forward and backward of a (1600, 64) layer norm
+// took 85 us with Python Functions. An engine thread does not hold the interpreter lock, so nothing here touches
+// Python: contract violations are C++ exceptions, translated to AssertionError where the call came from Python.
+
+struct ContractError : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+void must(bool ok, const std::string& msg) {
+  if (!ok) throw ContractError(msg);
+}
+void token_rc(int rc, const char* what) {
+  if (rc == THERIA_OK) return;
+  const std::string msg = std::string(what) + ": " + theria_last_error();
+  if (rc == THERIA_ERR_CONTRACT) throw ContractError(msg);
+  throw std::runtime_error(msg);
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using at::Tensor;
+
+constexpr int64_t kMaxNormWidth = 16384, kMaxRowWidth = 1 << 20, kMaxRows = (int64_t(1) << 31) - 64;
+
+int32_t token_dtype(at::ScalarType st) { return st == at::kFloat ? THERIA_DTYPE_F32 : st == at::kHalf ? THERIA_DTYPE_F16 : THERIA_DTYPE_BF16; }
+
+std::string shape_text(const Tensor& t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + (t.dim() == 1 ? ",)" : ")");
+}
+
+// Device, dtype and size contract of the operators' matrices.
+void check_matrix(const Tensor& t, const char* name, const char* what) {
+  must(t.defined(), std::string(what) + ": " + name + " must be a tensor");
+  must(t.is_cuda(), std::string(what) + " requires GPU (HIP) tensors; " + name + " is on " + t.device().str());
+  must(t.has_storage(), std::string(what) + " does not run under torch.func transforms");
+  const auto st = t.scalar_type();
+  must(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, std::string("Unsupported dtype for ") + name + ": " + c10::toString(st));
+  must(t.dim() == 0 || t.size(-1) == 0 || t.numel() / t.size(-1) <= kMaxRows, std::string(what) + ": " + name + " has more rows than 32-bit indexes reach");
+}
+// Ids or targets.
+void check_indexes(const Tensor& t, const char* name, const Tensor& like, const char* what) {
+  must(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, std::string(what) + ": " + name + " must be an int32 or int64 tensor");
+  must(t.device() == like.device(), std::string(what) + ": " + name + " must be on " + like.device().str() + ", got " + t.device().str());
+  must(t.has_storage(), std::string(what) + " does not run under torch.func transforms");
+  must(t.numel() <= kMaxRows, std::string(what) + ": " + name + " has more elements than 32-bit indexes reach");
+}
 
 // A tensor's rows of `width` as a matrix; a copy only where no view with a contiguous last dimension exists.
-at::Tensor rows_of(const at::Tensor& t_in, int64_t width) {
-  at::Tensor t = plain(t_in);
+Tensor rows_of(const Tensor& t_in, int64_t width) {
+  Tensor t = t_in;
   if (t.dim() != 2) t = t.reshape({t.numel() / width, width});
   if (width > 1 && t.stride(1) != 1) t = t.contiguous();
   return t;
 }
-at::Tensor rows_of(const at::Tensor& t, const at::Tensor& like, const char* msg) {
-  need(t.sizes() == like.sizes() && t.device() == like.device(), msg);
+// A gradient or cotangent in the shape and type of `like`; undefined stays undefined.
+Tensor rows_like(const Tensor& t, const Tensor& like, const char* what) {
+  if (!t.defined()) return t;
+  must(t.sizes() == like.sizes() && t.device() == like.device(), std::string(what) + ": a gradient must have the shape of its input");
   return rows_of(t.scalar_type() == like.scalar_type() ? t : t.to(like.scalar_type()), like.size(-1));
 }
-OptT rows_of(const OptT& t, const at::Tensor& like, const char* msg) {
-  if (!t) return std::nullopt;
-  return rows_of(*t, like, msg);
-}
-theria_rows_t rows_view(const at::Tensor& t) { return {t.data_ptr(), t.stride(0)}; }
-theria_rows_t rows_view(const OptT& t) { return t ? rows_view(*t) : theria_rows_t{nullptr, 0}; }
-void* ptr(const OptT& t) { return t ? plain(*t).data_ptr() : nullptr; }
-OptT flat(const OptT& t) {
-  if (!t) return std::nullopt;
-  return plain(*t).contiguous();
-}
-py::object given(const OptT& t) { return t ? py::cast(*t) : py::none(); }
+Tensor flat(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+theria_rows_t rows_view(const Tensor& t) { return t.defined() ? theria_rows_t{t.data_ptr(), t.stride(0)} : theria_rows_t{nullptr, 0}; }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-theria_layer_norm_problem_t norm_problem(const at::Tensor& x, at::ScalarType param, double eps) {
-  return {dtype_code(x.scalar_type()), dtype_code(param), (int32_t)x.size(1), (float)eps, x.size(0)};
+// The gradients of `outs` (with cotangents `cots`) with respect to aliases of `prim` that require them, by autograd through
+// `map`: the derivatives that no kernel covers. Aliases, so that each result is a partial derivative. keep: with a graph of
+// their own (through the originals); else the inputs are cut off first.
+template <class Map>
+variable_list through_map(const variable_list& prim, const std::vector<bool>& want, const variable_list& cots, bool keep, const Map& map) {
+  const at::AutoGradMode grad(true);
+  variable_list alias, wrt, outs, gs;
+  for (size_t i = 0; i < prim.size(); ++i) {
+    alias.push_back(!want[i] || !prim[i].defined() ? prim[i] : keep ? prim[i].view_as(prim[i]) : prim[i].detach().requires_grad_(true));
+    if (want[i] && prim[i].defined()) wrt.push_back(alias.back());
+  }
+  const variable_list all = map(alias);
+  for (size_t i = 0; i < all.size(); ++i)
+    if (cots[i].defined() && all[i].requires_grad()) outs.push_back(all[i]), gs.push_back(cots[i].to(all[i].scalar_type()));
+  variable_list result(prim.size());
+  if (outs.empty() || wrt.empty()) return result;
+  const variable_list got = torch::autograd::grad(outs, wrt, gs, /*retain_graph=*/keep, /*create_graph=*/keep, /*allow_unused=*/true);
+  size_t k = 0;
+  for (size_t i = 0; i < prim.size(); ++i)
+    if (want[i] && prim[i].defined()) result[i] = got[k++];
+  return result;
 }
 
-py::tuple layer_norm_fwd(const at::Tensor& x_in, const OptT& weight_in, const OptT& bias_in, double eps) {
+// A Function's outputs are the gradients that are wanted, without the others: packed from, and its cotangents unpacked to,
+// a list with a place for each.
+variable_list packed(const variable_list& all) {
+  variable_list some;
+  for (const Tensor& t : all)
+    if (t.defined()) some.push_back(t);
+  return some;
+}
+variable_list unpacked(const variable_list& some, const std::vector<bool>& want) {
+  variable_list all(want.size());
+  size_t k = 0;
+  for (size_t i = 0; i < want.size(); ++i)
+    if (want[i]) all[i] = some[k++];
+  return all;
+}
+
+// A Function's inputs are all defined: an absent parameter goes in as an empty tensor and comes out undefined again.
+Tensor or_empty(const Tensor& t, const Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
+Tensor or_absent(const Tensor& t) { return t.numel() ? t : Tensor(); }
+
+std::vector<bool> needed(AutogradContext* ctx) {
+  const auto list = ctx->saved_data["need"].toBoolList();
+  return std::vector<bool>(list.begin(), list.end());
+}
+
+// ---- layer norm
+theria_layer_norm_problem_t norm_problem(const Tensor& x, at::ScalarType param, double eps) {
+  return {token_dtype(x.scalar_type()), token_dtype(param), (int32_t)x.size(1), (float)eps, x.size(0)};
+}
+
+variable_list norm_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& dy_in, const Tensor& mean, const Tensor& rstd, double eps,
+                       at::ScalarType param, bool need_dx, bool need_dw, bool need_db) {
   const int64_t width = x_in.size(-1);
-  const at::Tensor x = rows_of(x_in, width);
-  const OptT weight = flat(weight_in), bias = flat(bias_in);
+  const Tensor dy = rows_like(dy_in, x_in, "hip_layer_norm"), x = rows_of(x_in, width), weight = flat(weight_in);
   const c10::hip::HIPGuard guard(x.get_device());
-  const auto y = at::empty({x.size(0), width}, x.options());
-  const auto mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
-  const auto p = norm_problem(x, weight ? weight->scalar_type() : bias ? bias->scalar_type() : x.scalar_type(), eps);
-  const auto vx = rows_view(x), vy = rows_view(y);
-  check_rc(theria_layer_norm_fwd(&p, &vx, ptr(weight), ptr(bias), &vy, fptr(mean), fptr(rstd), stream_of(x)),
-           "theria_layer_norm_fwd");
-  return py::make_tuple(y.view(x_in.sizes()), mean, rstd);
-}
-
-py::tuple layer_norm_bwd(const at::Tensor& x_in, const OptT& weight_in, const at::Tensor& dout_in, const at::Tensor& mean,
-                         const at::Tensor& rstd, double eps, bool need_dx, bool need_dw, bool need_db, at::ScalarType param) {
-  const int64_t width = x_in.size(-1);
-  const at::Tensor dout = rows_of(dout_in, x_in, "the gradient must have the shape of the input");
-  const at::Tensor x = rows_of(x_in, width);
-  const OptT weight = flat(weight_in);
-  const c10::hip::HIPGuard guard(x.get_device());
-  OptT dx, dw, db, ws;
-  if (need_dx) dx = at::empty({x.size(0), width}, x.options());
+  Tensor dx, dw, db, ws;
+  if (need_dx) dx = at::empty(x_in.sizes(), x.options());
   const auto po = x.options().dtype(param);
   const bool none = x.size(0) == 0;
   if (need_dw) dw = none ? at::zeros({width}, po) : at::empty({width}, po);
@@ -322,122 +404,360 @@ py::tuple layer_norm_bwd(const at::Tensor& x_in, const OptT& weight_in, const at
   if (!none) {
     const auto p = norm_problem(x, param, eps);
     if (need_dw || need_db) ws = at::empty({theria_layer_norm_ws_floats(&p)}, x.options().dtype(at::kFloat));
-    const auto vx = rows_view(x), vg = rows_view(dout), vdx = rows_view(dx);
-    check_rc(theria_layer_norm_bwd(&p, &vx, ptr(weight), &vg, fptr(mean), fptr(rstd), &vdx, ptr(dw), ptr(db), fptr(ws), stream_of(x)),
+    const auto vx = rows_view(x), vg = rows_view(dy);
+    const theria_rows_t vdx{ptr(dx), width};
+    token_rc(theria_layer_norm_bwd(&p, &vx, ptr(weight), &vg, floats(mean), floats(rstd), &vdx, ptr(dw), ptr(db), floats(ws), stream_of(x)),
              "theria_layer_norm_bwd");
   }
-  if (dx) dx = dx->view(x_in.sizes());
-  return py::make_tuple(given(dx), given(dw), given(db));
+  return {dx, dw, db};
 }
 
-py::tuple layer_norm_bwd_bwd(const at::Tensor& x_in, const OptT& weight_in, const at::Tensor& dout_in, const at::Tensor& mean,
-                             const at::Tensor& rstd, double eps, const OptT& gdx_in, const OptT& gdw_in, const OptT& gdb_in,
-                             bool need_gx, bool need_gw, bool need_gdout, at::ScalarType param) {
+variable_list norm_bwd_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& dy_in, const Tensor& mean, const Tensor& rstd, double eps,
+                           at::ScalarType param, const Tensor& u_in, const Tensor& a_in, const Tensor& c_in, bool need_gx, bool need_gw,
+                           bool need_gdy) {
   const int64_t width = x_in.size(-1);
-  const at::Tensor dout = rows_of(dout_in, x_in, "the gradient must have the shape of the input");
-  const OptT gdx = rows_of(gdx_in, x_in, "a cotangent must have the shape of the input");
-  const at::Tensor x = rows_of(x_in, width);
-  auto param_like = [&](const OptT& t) -> OptT {
-    if (!t) return std::nullopt;
-    need(t->numel() == width && t->device() == x.device(), "a cotangent must have the shape of its parameter");
-    return flat(t->scalar_type() == param ? *t : t->to(param));
+  const Tensor dy = rows_like(dy_in, x_in, "hip_layer_norm"), u = rows_like(u_in, x_in, "hip_layer_norm"), x = rows_of(x_in, width),
+               weight = flat(weight_in);
+  auto param_like = [&](const Tensor& t) {
+    if (!t.defined()) return t;
+    must(t.numel() == width && t.device() == x.device(), "hip_layer_norm: a cotangent must have the shape of its parameter");
+    return flat(t.scalar_type() == param ? t : t.to(param));
   };
-  const OptT weight = flat(weight_in), gdw = param_like(gdw_in), gdb = param_like(gdb_in);
+  const Tensor a = param_like(a_in), c = param_like(c_in);
   const c10::hip::HIPGuard guard(x.get_device());
-  OptT gx, gw, gg, ws;
+  Tensor gx, gw, gdy, ws;
   const bool none = x.size(0) == 0;
-  if (need_gx) gx = at::empty({x.size(0), width}, x.options());
-  if (need_gdout) gg = at::empty({x.size(0), width}, x.options());
-  if (need_gw) gw = none ? at::zeros({width}, x.options().dtype(param)) : at::empty({width}, x.options().dtype(param));
+  const auto po = x.options().dtype(param);
+  if (need_gx) gx = at::empty(x_in.sizes(), x.options());
+  if (need_gdy) gdy = at::empty(x_in.sizes(), x.options());
+  if (need_gw) gw = none ? at::zeros({width}, po) : at::empty({width}, po);
   if (!none) {
     const auto p = norm_problem(x, param, eps);
     if (need_gw) ws = at::empty({theria_layer_norm_ws_floats(&p)}, x.options().dtype(at::kFloat));
-    const auto vx = rows_view(x), vg = rows_view(dout), vu = rows_view(gdx), vgx = rows_view(gx), vgg = rows_view(gg);
-    check_rc(theria_layer_norm_bwd_bwd(&p, &vx, ptr(weight), &vg, fptr(mean), fptr(rstd), &vu, ptr(gdw), ptr(gdb), &vgx, ptr(gw),
-                                       &vgg, fptr(ws), stream_of(x)),
+    const auto vx = rows_view(x), vg = rows_view(dy), vu = rows_view(u);
+    const theria_rows_t vgx{ptr(gx), width}, vgdy{ptr(gdy), width};
+    token_rc(theria_layer_norm_bwd_bwd(&p, &vx, ptr(weight), &vg, floats(mean), floats(rstd), &vu, ptr(a), ptr(c), &vgx, ptr(gw), &vgdy,
+                                       floats(ws), stream_of(x)),
              "theria_layer_norm_bwd_bwd");
   }
-  if (gx) gx = gx->view(x_in.sizes());
-  if (gg) gg = gg->view(x_in.sizes());
-  return py::make_tuple(given(gx), given(gw), given(gg));
+  if (gdy.defined() && dy_in.scalar_type() != gdy.scalar_type()) gdy = gdy.to(dy_in.scalar_type());
+  return {gx, gw, gdy};
 }
 
-at::Tensor embedding_fwd(const at::Tensor& ids_in, const at::Tensor& table_in, double scale, int64_t padding, bool zero_padding) {
-  const int64_t width = table_in.size(1);
-  const at::Tensor table = rows_of(table_in, width), ids = plain(ids_in).contiguous();
-  const c10::hip::HIPGuard guard(table.get_device());
-  const auto out = at::empty({ids.numel(), width}, table.options());
-  const theria_embedding_problem_t p{dtype_code(table.scalar_type()), ids.scalar_type() == at::kLong, (int32_t)width,
-                                     (float)scale, ids.numel(), table.size(0), padding};
-  const auto vt = rows_view(table), vo = rows_view(out);
-  check_rc(theria_embedding_fwd(&p, ids.data_ptr(), &vt, zero_padding, &vo, stream_of(table)), "theria_embedding_fwd");
-  auto sizes = ids_in.sizes().vec();
-  sizes.push_back(width);
-  return out.view(sizes);
+// (dx, dweight, dbias) as differentiable torch operations, in float32 or wider: orders three and higher only.
+variable_list norm_map(const variable_list& in, double eps) {
+  const Tensor &x_in = in[0], &weight = in[1], &dy_in = in[2];
+  const int64_t width = x_in.size(-1);
+  const auto ct = at::promote_types(x_in.scalar_type(), at::kFloat);
+  const Tensor x = x_in.to(ct).reshape({-1, width}), dy = dy_in.to(ct).reshape({-1, width});
+  const Tensor xc = x - x.mean(1, true);
+  const Tensor rstd = ((xc * xc).mean(1, true) + eps).rsqrt(), xh = xc * rstd;
+  const Tensor gw = weight.defined() ? dy * weight.to(ct) : dy;
+  const Tensor dx = rstd * (gw - gw.mean(1, true) - xh * (gw * xh).mean(1, true));
+  return {dx.reshape(x_in.sizes()).to(x_in.scalar_type()), (dy * xh).sum(0), dy.sum(0)};
 }
 
-at::Tensor embedding_bwd(const at::Tensor& ids_in, const at::Tensor& dout_in, int64_t classes, double scale, int64_t padding) {
+// (x, weight, dy, mean, rstd) -> (dx, dweight, dbias). mean and rstd are functions of x, whose part in the derivative the
+// double backward's kernel includes.
+struct NormBackwardFn : torch::autograd::Function<NormBackwardFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight_in, const Tensor& dy, const Tensor& mean,
+                               const Tensor& rstd, double eps, int64_t param, bool need_dx, bool need_dw, bool need_db) {
+    const Tensor weight = or_absent(weight_in);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, weight_in, dy, mean, rstd});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["param"] = param;
+    ctx->saved_data["need"] = std::vector<bool>{need_dx, need_dw, need_db};
+    return packed(norm_bwd(x, weight, dy, mean, rstd, eps, (at::ScalarType)param, need_dx, need_dw, need_db));
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& some) {
+    variable_list out(10);
+    const variable_list g = unpacked(some, needed(ctx));
+    if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], weight = or_absent(saved[1]), &dy = saved[2];
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), ny = ctx->needs_input_grad(2);
+    const bool keep = at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(dy) || wants(g[0]) || wants(g[1]) || wants(g[2]));
+    const variable_list r = keep ? through_map({x, weight, dy}, {nx, nw, ny}, {g[0], g[1], g[2]}, true, [&](const variable_list& in) { return norm_map(in, eps); })
+                                 : norm_bwd_bwd(x, weight, dy, saved[3], saved[4], eps, (at::ScalarType)ctx->saved_data["param"].toInt(), g[0], g[1], g[2], nx, nw, ny);
+    out[0] = r[0], out[1] = r[1], out[2] = r[2];
+    return out;
+  }
+};
+
+struct NormFn : torch::autograd::Function<NormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, double eps, int64_t param) {
+    const int64_t width = x_in.size(-1);
+    const Tensor x = rows_of(x_in, width), weight = flat(or_absent(weight_in)), bias = flat(or_absent(bias_in));
+    const c10::hip::HIPGuard guard(x.get_device());
+    const Tensor y = at::empty(x_in.sizes(), x.options());
+    const Tensor mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    const auto p = norm_problem(x, (at::ScalarType)param, eps);
+    const auto vx = rows_view(x);
+    const theria_rows_t vy{ptr(y), width};
+    token_rc(theria_layer_norm_fwd(&p, &vx, ptr(weight), ptr(bias), &vy, floats(mean), floats(rstd), stream_of(x)), "theria_layer_norm_fwd");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x_in, weight_in, mean, rstd});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["param"] = param;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(5);
+    if (!g[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], weight = or_absent(saved[1]);
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const int64_t param = ctx->saved_data["param"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2);
+    const variable_list r = at::GradMode::is_enabled()
+                                ? unpacked(NormBackwardFn::apply(x, saved[1], g[0], saved[2], saved[3], eps, param, nx, nw, nb), {nx, nw, nb})
+                                : norm_bwd(x, weight, g[0], saved[2], saved[3], eps, (at::ScalarType)param, nx, nw, nb);
+    out[0] = r[0], out[1] = r[1], out[2] = r[2];
+    return out;
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const OptT& weight_in, const OptT& bias_in, double eps) {
+  const char* what = "hip_layer_norm";
+  const Tensor weight = weight_in.value_or(Tensor()), bias = bias_in.value_or(Tensor());
+  check_matrix(x, "x", what);
+  must(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxNormWidth,
+       std::string(what) + " supports rows of 1 to " + std::to_string(kMaxNormWidth) + " elements, got shape " + shape_text(x));
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor&>("weight", weight), std::pair<const char*, const Tensor&>("bias", bias)}) {
+    if (!t.defined()) continue;
+    must(t.dim() == 1 && t.size(0) == x.size(-1), std::string(name) + " must have shape (" + std::to_string(x.size(-1)) + ",), got " + shape_text(t));
+    must((t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat) && t.device() == x.device() && t.has_storage(),
+         std::string(what) + ": " + name + " must be on " + x.device().str() + " in " + c10::toString(x.scalar_type()) + " or float32, got " +
+             c10::toString(t.scalar_type()) + " on " + t.device().str());
+  }
+  must(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), std::string(what) + ": weight and bias must have one dtype");
+  must(eps >= 0 && std::isfinite(eps), std::string(what) + ": eps must be finite and not negative, got " + std::to_string(eps));
+  const auto param = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type();
+  return NormFn::apply(x, or_empty(weight, x), or_empty(bias, x), eps, (int64_t)param);
+}
+
+// ---- embedding: linear in the table, so that the gradient's derivative is a lookup again
+theria_embedding_problem_t embed_problem(const Tensor& ids, const Tensor& rows, int64_t classes, double scale, int64_t padding) {
+  return {token_dtype(rows.scalar_type()), ids.scalar_type() == at::kLong, (int32_t)rows.size(1), (float)scale, ids.numel(), classes, padding};
+}
+
+Tensor embed_bwd(const Tensor& ids_in, const Tensor& dout_in, int64_t classes, double scale, int64_t padding) {
   const int64_t width = dout_in.size(-1);
-  const at::Tensor ids = plain(ids_in).contiguous(), dout = rows_of(dout_in, width);
-  need(dout.size(0) == ids.numel() && dout.device() == ids.device(), "the gradient must have one row for each id");
+  const Tensor ids = ids_in.contiguous(), dout = rows_of(dout_in, width);
+  must(dout.size(0) == ids.numel() && dout.device() == ids.device(), "hip_embedding: the gradient must have one row for each id");
   const c10::hip::HIPGuard guard(dout.get_device());
-  const auto out = at::empty({classes, width}, dout.options());
-  const theria_embedding_problem_t p{dtype_code(dout.scalar_type()), ids.scalar_type() == at::kLong, (int32_t)width,
-                                     (float)scale, ids.numel(), classes, padding};
-  const auto ws = at::empty({theria_embedding_ws_bytes(&p)}, dout.options().dtype(at::kByte));
+  const Tensor out = at::empty({classes, width}, dout.options());
+  const auto p = embed_problem(ids, dout, classes, scale, padding);
+  const Tensor ws = at::empty({theria_embedding_ws_bytes(&p)}, dout.options().dtype(at::kByte));
   const auto vg = rows_view(dout), vo = rows_view(out);
-  check_rc(theria_embedding_bwd(&p, ids.data_ptr(), &vg, &vo, ws.data_ptr(), stream_of(dout)), "theria_embedding_bwd");
+  token_rc(theria_embedding_bwd(&p, ids.data_ptr(), &vg, &vo, ws.data_ptr(), stream_of(dout)), "theria_embedding_bwd");
   return out;
 }
 
-theria_linear_ce_problem_t ce_problem(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, int64_t ignore, int reduction) {
-  return {dtype_code(x.scalar_type()), target.scalar_type() == at::kLong, reduction, (int32_t)x.size(1), x.size(0), weight.size(0), ignore};
+struct EmbedBackwardFn : torch::autograd::Function<EmbedBackwardFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& dout, const Tensor& ids, int64_t classes, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embed_bwd(ids, dout, classes, scale, padding);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g);
+};
+
+struct EmbedFn : torch::autograd::Function<EmbedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table_in, const Tensor& ids_in, double scale, int64_t padding, bool zero_padding) {
+    const int64_t width = table_in.size(1);
+    const Tensor table = rows_of(table_in, width), ids = ids_in.contiguous();
+    const c10::hip::HIPGuard guard(table.get_device());
+    auto sizes = ids_in.sizes().vec();
+    sizes.push_back(width);
+    const Tensor out = at::empty(sizes, table.options());
+    const auto p = embed_problem(ids, table, table.size(0), scale, padding);
+    const auto vt = rows_view(table);
+    const theria_rows_t vo{ptr(out), width};
+    token_rc(theria_embedding_fwd(&p, ids.data_ptr(), &vt, zero_padding, &vo, stream_of(table)), "theria_embedding_fwd");
+    ctx->save_for_backward({ids_in});
+    ctx->saved_data["classes"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const int64_t classes = ctx->saved_data["classes"].toInt(), padding = ctx->saved_data["padding"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    variable_list out(5);
+    out[0] = at::GradMode::is_enabled() ? EmbedBackwardFn::apply(g[0], ids, classes, scale, padding) : embed_bwd(ids, g[0], classes, scale, padding);
+    return out;
+  }
+};
+
+variable_list EmbedBackwardFn::backward(AutogradContext* ctx, const variable_list& g) {
+  variable_list out(5);
+  out[0] = EmbedFn::apply(g[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), true);
+  return out;
+}
+
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
+  const char* what = "hip_embedding";
+  check_matrix(weight, "weight", what);
+  must(weight.dim() == 2 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
+       std::string(what) + ": weight must be (V, D) with 1 <= D <= " + std::to_string(kMaxRowWidth) + ", got shape " + shape_text(weight));
+  check_indexes(ids, "ids", weight, what);
+  int64_t padding = -1;
+  if (padding_idx) {
+    padding = *padding_idx < 0 ? *padding_idx + weight.size(0) : *padding_idx;
+    must(padding >= 0 && padding < weight.size(0), std::string(what) + ": padding_idx " + std::to_string(*padding_idx) + " is outside the table of " +
+                                                       std::to_string(weight.size(0)) + " rows");
+  }
+  must(std::isfinite(scale) && std::isfinite((float)scale), std::string(what) + ": scale must be finite, got " + std::to_string(scale));
+  return EmbedFn::apply(weight, ids, scale, padding, false);
+}
+
+// ---- linear cross entropy
+theria_linear_ce_problem_t ce_problem(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore, int64_t reduction) {
+  return {token_dtype(x.scalar_type()), target.scalar_type() == at::kLong, (int32_t)reduction, (int32_t)x.size(1), x.size(0), weight.size(0), ignore};
 }
 
 // A 256-byte-aligned workspace: torch's allocations are.
-at::Tensor ce_workspace(const theria_linear_ce_problem_t& p, const theria_rows_t& w, const at::Tensor& x, bool backward, bool dx, bool dw, bool db) {
+Tensor ce_workspace(const theria_linear_ce_problem_t& p, const theria_rows_t& w, const Tensor& x, bool backward, bool dx, bool dw, bool db) {
   return at::empty({theria_linear_ce_ws_bytes(&p, &w, backward, dx, dw, db)}, x.options().dtype(at::kByte));
 }
 
-py::tuple linear_ce_fwd(const at::Tensor& x_in, const at::Tensor& weight_in, const OptT& bias_in, const at::Tensor& target_in,
-                        int64_t ignore, int reduction) {
+variable_list ce_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, const Tensor& target_in, const Tensor& stats,
+                     const Tensor& dloss_in, int64_t ignore, int64_t reduction, bool need_dx, bool need_dw, bool need_db) {
   const int64_t width = x_in.size(-1);
-  const at::Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = plain(target_in).contiguous();
-  const OptT bias = flat(bias_in);
+  const Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = target_in.contiguous(), bias = flat(bias_in);
+  const Tensor dloss = dloss_in.to(at::kFloat).contiguous();
+  must(dloss.numel() == (reduction == THERIA_REDUCE_NONE ? x.size(0) : 1) && dloss.device() == x.device(),
+       "hip_linear_cross_entropy: the loss's gradient must have the shape of the loss");
   const c10::hip::HIPGuard guard(x.get_device());
-  const auto f = x.options().dtype(at::kFloat);
-  const auto loss = reduction == THERIA_REDUCE_NONE ? at::empty({x.size(0)}, f) : at::empty({}, f);
-  const auto stats = at::empty({2, x.size(0)}, f);
-  const auto p = ce_problem(x, weight, target, ignore, reduction);
-  const auto vx = rows_view(x), vw = rows_view(weight);
-  const auto ws = ce_workspace(p, vw, x, false, false, false, false);
-  check_rc(theria_linear_ce_fwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), fptr(loss), fptr(stats), ws.data_ptr(), stream_of(x)),
-           "theria_linear_ce_fwd");
-  return py::make_tuple(reduction == THERIA_REDUCE_NONE ? loss.view(target_in.sizes()) : loss, stats);
-}
-
-py::tuple linear_ce_bwd(const at::Tensor& x_in, const at::Tensor& weight_in, const OptT& bias_in, const at::Tensor& target_in,
-                        const at::Tensor& stats, const at::Tensor& dloss_in, int64_t ignore, int reduction, bool need_dx, bool need_dw,
-                        bool need_db) {
-  const int64_t width = x_in.size(-1);
-  const at::Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = plain(target_in).contiguous();
-  const OptT bias = flat(bias_in);
-  const at::Tensor dloss = plain(dloss_in).to(at::kFloat).contiguous();
-  need(dloss.numel() == (reduction == THERIA_REDUCE_NONE ? x.size(0) : 1) && dloss.device() == x.device(),
-       "the loss's gradient must have the shape of the loss");
-  const c10::hip::HIPGuard guard(x.get_device());
-  OptT dx, dw, db;
-  if (need_dx) dx = at::empty({x.size(0), width}, x.options());
+  Tensor dx, dw, db;
+  if (need_dx) dx = at::empty(x_in.sizes(), x.options());
   if (need_dw) dw = at::empty({weight.size(0), width}, x.options());
   if (need_db) db = at::empty({weight.size(0)}, x.options());
   const auto p = ce_problem(x, weight, target, ignore, reduction);
-  const auto vx = rows_view(x), vw = rows_view(weight), vdx = rows_view(dx), vdw = rows_view(dw);
-  const auto ws = ce_workspace(p, vw, x, true, need_dx, need_dw, need_db);
-  check_rc(theria_linear_ce_bwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), fptr(stats), fptr(dloss), &vdx, &vdw, ptr(db), ws.data_ptr(),
+  const auto vx = rows_view(x), vw = rows_view(weight), vdw = rows_view(dw);
+  const theria_rows_t vdx{ptr(dx), width};
+  const Tensor ws = ce_workspace(p, vw, x, true, need_dx, need_dw, need_db);
+  token_rc(theria_linear_ce_bwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), floats(stats), floats(dloss), &vdx, &vdw, ptr(db), ws.data_ptr(),
                                 stream_of(x)),
            "theria_linear_ce_bwd");
-  if (dx) dx = dx->view(x_in.sizes());
-  return py::make_tuple(given(dx), given(dw), given(db));
+  return {dx, dw, db};
+}
+
+// (dx, dweight, dbias) as differentiable torch operations, in float32 or wider, with the logits materialised. in: x, weight,
+// bias, the loss's gradient.
+variable_list ce_map(const variable_list& in, const Tensor& target, int64_t ignore, int64_t reduction) {
+  const Tensor &x = in[0], &weight = in[1], &bias = in[2];
+  const auto ct = at::promote_types(x.scalar_type(), at::kFloat);
+  const int64_t V = weight.size(0), D = weight.size(1);
+  const Tensor t = target.reshape({-1}).to(at::kLong);
+  const Tensor kept = t.ne(ignore).logical_and(t.ge(0)).logical_and(t.lt(V));
+  const Tensor zero = at::zeros({}, x.options().dtype(ct));
+  const Tensor xf = at::where(kept.unsqueeze(1), x.to(ct).reshape({-1, D}), zero), wf = weight.to(ct);
+  Tensor z = at::matmul(xf, wf.t());
+  if (bias.defined()) z = z + bias.to(ct);
+  const Tensor classes = at::arange(V, t.options());
+  const Tensor onehot = at::where(kept, t, at::full({}, -1, t.options())).unsqueeze(1).eq(classes).to(ct);
+  Tensor up = at::where(kept, in[3].to(ct).reshape({-1}).expand({t.size(0)}), zero);
+  if (reduction == THERIA_REDUCE_MEAN) up = up / kept.sum().clamp_min(1).to(ct);
+  const Tensor dz = (at::softmax(z, 1) - onehot) * up.unsqueeze(1);
+  return {at::matmul(dz, wf).reshape(x.sizes()).to(x.scalar_type()), at::matmul(dz.t(), xf).to(weight.scalar_type()), dz.sum(0)};
+}
+
+struct CeBackwardFn : torch::autograd::Function<CeBackwardFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& target,
+                               const Tensor& stats, const Tensor& dloss, int64_t ignore, int64_t reduction, bool need_dx, bool need_dw,
+                               bool need_db) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, weight, bias, target, dloss});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["need"] = std::vector<bool>{need_dx, need_dw, need_db};
+    return packed(ce_bwd(x, weight, or_absent(bias), target, stats, dloss, ignore, reduction, need_dx, need_dw, need_db));
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& some) {
+    variable_list out(11);
+    const variable_list g = unpacked(some, needed(ctx));
+    if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const int64_t ignore = ctx->saved_data["ignore"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
+    const std::vector<bool> want{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(5)};
+    const variable_list r = through_map({saved[0], saved[1], or_absent(saved[2]), saved[4]}, want, {g[0], g[1], g[2]}, at::GradMode::is_enabled(),
+                                        [&](const variable_list& in) { return ce_map(in, saved[3], ignore, reduction); });
+    out[0] = r[0], out[1] = r[1], out[2] = r[2], out[5] = r[3];
+    return out;
+  }
+};
+
+struct CeFn : torch::autograd::Function<CeFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, const Tensor& target_in,
+                        int64_t ignore, int64_t reduction) {
+    const int64_t width = x_in.size(-1);
+    const Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = target_in.contiguous(),
+                 bias = flat(or_absent(bias_in));
+    const c10::hip::HIPGuard guard(x.get_device());
+    const auto f = x.options().dtype(at::kFloat);
+    const Tensor loss = reduction == THERIA_REDUCE_NONE ? at::empty(target_in.sizes(), f) : at::empty({}, f);
+    const Tensor stats = at::empty({2, x.size(0)}, f);
+    const auto p = ce_problem(x, weight, target, ignore, reduction);
+    const auto vx = rows_view(x), vw = rows_view(weight);
+    const Tensor ws = ce_workspace(p, vw, x, false, false, false, false);
+    token_rc(theria_linear_ce_fwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), floats(loss), floats(stats), ws.data_ptr(), stream_of(x)),
+             "theria_linear_ce_fwd");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x_in, weight_in, bias_in, target_in, stats});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(6);
+    if (!g[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const int64_t ignore = ctx->saved_data["ignore"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2);
+    const variable_list r = at::GradMode::is_enabled()
+                                ? unpacked(CeBackwardFn::apply(saved[0], saved[1], saved[2], saved[3], saved[4], g[0], ignore, reduction, nx, nw, nb), {nx, nw, nb})
+                                : ce_bwd(saved[0], saved[1], or_absent(saved[2]), saved[3], saved[4], g[0], ignore, reduction, nx, nw, nb);
+    out[0] = r[0], out[1] = r[1], out[2] = r[2];
+    return out;
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target, const OptT& bias_in, int64_t ignore, const std::string& reduction) {
+  const char* what = "hip_linear_cross_entropy";
+  const std::string w = what;
+  const Tensor bias = bias_in.value_or(Tensor());
+  check_matrix(x, "x", what);
+  check_matrix(weight, "weight", what);
+  must(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
+       w + ": x must be (..., D) and weight (V, D), got " + shape_text(x) + " and " + shape_text(weight));
+  must(weight.size(0) >= 1 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
+       w + " supports V >= 1 and 1 <= D <= " + std::to_string(kMaxRowWidth) + ", got weight " + shape_text(weight));
+  must(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(), w + ": weight must match x in dtype and device");
+  must(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0) && bias.scalar_type() == x.scalar_type() &&
+                           bias.device() == x.device() && bias.has_storage()),
+       w + ": bias must be (" + std::to_string(weight.size(0)) + ",) and match x in dtype and device");
+  check_indexes(target, "target", x, what);
+  must(target.sizes() == x.sizes().slice(0, x.dim() - 1), w + ": target must have shape " + "x's without its last dimension, got " + shape_text(target) +
+                                                              " for x " + shape_text(x));
+  must(reduction == "none" || reduction == "mean" || reduction == "sum", w + ": reduction must be 'none', 'mean' or 'sum', got '" + reduction + "'");
+  const int64_t r = reduction == "none" ? THERIA_REDUCE_NONE : reduction == "mean" ? THERIA_REDUCE_MEAN : THERIA_REDUCE_SUM;
+  return CeFn::apply(x, weight, or_empty(bias, x), target, ignore, r);
+}
+
+// The differentiable restatements, for tests without a GPU.
+py::tuple norm_map_py(const Tensor& x, const OptT& w, const Tensor& dy, double eps) {
+  const auto r = norm_map({x, w.value_or(Tensor()), dy}, eps);
+  return py::make_tuple(r[0], r[1], r[2]);
+}
+py::tuple ce_map_py(const Tensor& x, const Tensor& w, const OptT& b, const Tensor& target, const Tensor& dloss, int64_t ignore, int64_t reduction) {
+  const auto r = ce_map({x, w, b.value_or(Tensor()), dloss}, target, ignore, reduction);
+  return py::make_tuple(r[0], r[1], r[2]);
 }
 
 }  // namespace
@@ -454,11 +774,17 @@ PYBIND11_MODULE(_theria_host, m) {
   m.def("bwd_bwd", &bwd_bwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("dout"),
         py::arg("lse"), py::arg("gq"), py::arg("gk"), py::arg("gv"), py::arg("scale"), py::arg("causal"),
         py::arg("noalloc"), py::arg("out"));
-  m.def("layer_norm_fwd", &layer_norm_fwd);
-  m.def("layer_norm_bwd", &layer_norm_bwd);
-  m.def("layer_norm_bwd_bwd", &layer_norm_bwd_bwd);
-  m.def("embedding_fwd", &embedding_fwd);
-  m.def("embedding_bwd", &embedding_bwd);
-  m.def("linear_ce_fwd", &linear_ce_fwd);
-  m.def("linear_ce_bwd", &linear_ce_bwd);
+  py::register_exception_translator([](std::exception_ptr e) {
+    try {
+      if (e) std::rethrow_exception(e);
+    } catch (const ContractError& x) {
+      PyErr_SetString(PyExc_AssertionError, x.what());
+    }
+  });
+  m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
+  m.def("embedding", &embedding, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("padding_idx"));
+  m.def("linear_cross_entropy", &linear_cross_entropy, py::arg("x"), py::arg("weight"), py::arg("target"), py::arg("bias"),
+        py::arg("ignore_index"), py::arg("reduction"));
+  m.def("layer_norm_backward_map", &norm_map_py);
+  m.def("linear_ce_backward_map", &ce_map_py);
 }
