@@ -290,7 +290,7 @@ typedef struct {
   int32_t width;
   float scale;
   int64_t n;       /* ids */
-  int64_t classes; /* rows of the table, below 2^31 */
+  int64_t classes; /* rows of the table, at most 2^27 */
   int64_t padding; /* id whose row gets no gradient, or -1 */
 } theria_embedding_problem_t;
 
@@ -312,8 +312,8 @@ typedef struct {
   int32_t target64;  /* targets are int64, else int32 */
   int32_t reduction; /* enum theria_reduction */
   int32_t width;
-  int64_t n;         /* rows of x, below 2^31 */
-  int64_t classes;   /* rows of weight, below 2^31 */
+  int64_t n;         /* rows of x, at most 2^26 */
+  int64_t classes;   /* rows of weight, at most 2^26 */
   int64_t ignore;    /* target of the rows that are left out */
 } theria_linear_ce_problem_t;
 

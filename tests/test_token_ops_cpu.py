@@ -77,7 +77,7 @@ def test_embedding_contract():
     _refused(fwd(P(5, 1, 64, 1.0, 4, 10, -1)), "dtype")
     _refused(fwd(P(2, 1, 0, 1.0, 4, 10, -1)), "width")
     _refused(fwd(P(2, 1, 64, float("nan"), 4, 10, -1)), "scale")
-    _refused(fwd(P(2, 1, 64, 1.0, 4, 2**31, -1)), "classes")
+    _refused(fwd(P(2, 1, 64, 1.0, 4, 2**27 + 1, -1)), "classes")
     _refused(fwd(P(2, 1, 64, 1.0, 4, 10, 10)), "padding")
     _refused(fwd(P(2, 1, 64, 1.0, 4, 10, -1), ids=None), "ids")
     assert fwd(P(2, 1, 64, 1.0, 0, 10, -1)) == _lib.OK
@@ -103,6 +103,7 @@ def test_linear_ce_contract():
     _refused(fwd(P(2, 1, 1, 0, 4, 10, -100)), "width")
     _refused(fwd(P(2, 1, 1, 64, 4, 0, -100)), "classes")
     _refused(fwd(P(2, 1, 1, 64, -4, 10, -100)), "n must")
+    _refused(fwd(P(2, 1, 1, 64, 4, 2**26 + 1, -100)), "classes")
     _refused(fwd(P(2, 1, 1, 64, 4, 10, -100), loss=None), "loss")
     _refused(fwd(P(2, 1, 1, 64, 4, 10, -100), ws=FAKE + 16), "256-byte-aligned")
     _refused(fwd(P(2, 1, 1, 64, 4, 10, -100), stats=None), "stats")

@@ -10,7 +10,9 @@
 namespace theria {
 namespace {
 
-constexpr int64_t kMost = (int64_t(1) << 31) - 64;  // rows and classes, whose 32-bit indexes are rounded up to tiles
+constexpr int64_t kMost = (int64_t(1) << 31) - 64;  // rows and tokens, whose 32-bit indexes are rounded up to pieces
+// Rows of a table or of logits: with the workgroups that they take, a launch has to hold fewer than 2^32 threads.
+constexpr int64_t kMostClasses = int64_t(1) << 27, kMostLogits = int64_t(1) << 26;
 
 const char* check_type(int dtype) { return dtype < 0 || dtype > 2 ? "dtype must be 0 (f32), 1 (f16) or 2 (bf16)" : nullptr; }
 
@@ -57,7 +59,7 @@ const char* embed_from(const theria_embedding_problem_t* p, EmbedParams& e) {
   if (!p) return "problem is required";
   if (const char* m = check_type(p->dtype)) return m;
   if (p->width < 1 || p->width > (1 << 20)) return "width must be in 1..2^20";
-  if (p->n < 0 || p->n > kMost || p->classes < 0 || p->classes > kMost) return "n and classes must be in 0..2^31 - 64";
+  if (p->n < 0 || p->n > kMost || p->classes < 0 || p->classes > kMostClasses) return "n must be in 0..2^31 - 64 and classes in 0..2^27";
   if (p->padding < -1 || p->padding >= p->classes) return "padding must be -1 or a row of the table";
   if (!std::isfinite(p->scale)) return "scale must be finite";
   e = EmbedParams{};
@@ -77,8 +79,8 @@ const char* ce_from(const theria_linear_ce_problem_t* p, CeParams& c) {
   if (const char* m = check_type(p->dtype)) return m;
   if (p->reduction < 0 || p->reduction > 2) return "reduction must be 0 (none), 1 (mean) or 2 (sum)";
   if (p->width < 1 || p->width > (1 << 20)) return "width must be in 1..2^20";
-  if (p->n < 0 || p->n > kMost) return "n must be in 0..2^31 - 64";
-  if (p->classes < 1 || p->classes > kMost) return "classes must be in 1..2^31 - 64";
+  if (p->n < 0 || p->n > kMostLogits) return "n must be in 0..2^26";
+  if (p->classes < 1 || p->classes > kMostLogits) return "classes must be in 1..2^26";
   c = CeParams{};
   c.dtype = p->dtype;
   c.target64 = p->target64 != 0;

@@ -11,8 +11,7 @@
 //           of LDS, spread over the GPU). More: a stable radix sort, digits of at most 10 bits, two launches a digit.
 //   pieces  frequent ids: every aligned run of 64 sorted tokens that holds one id alone is summed by a workgroup of its
 //           own into a float32 row of the workspace, so that an id with thousands of tokens is spread over the GPU.
-//   rows    every table row: its bounds by binary search, then the tokens before its first whole piece, the pieces,
-//           and the tokens after its last one.
+//   rows    every table row: the tokens before its first whole piece, the pieces, and the tokens after its last one.
 #include "token_common.hpp"
 #include "token_params.hpp"
 
@@ -21,8 +20,7 @@ namespace {
 
 constexpr int kPiece = 64;         // sorted tokens of a piece
 constexpr int kRankTokens = 8192;  // most tokens ordered by counting
-constexpr int kSortTile = 4096;    // tokens of a radix sort's workgroup
-constexpr int kSortMost = 1024;    // digits of a radix sort's pass
+constexpr int kSortMost = 1024;     // digits of a radix sort's pass
 
 __device__ __forceinline__ int64_t load_id(const void* ids, bool ids64, int64_t n) {
   return ids64 ? ((const int64_t*)ids)[n] : (int64_t)((const int32_t*)ids)[n];
@@ -65,11 +63,17 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
 }
 
 // ------------------------------------------------------------------------------------------ order
+// No tokens for any row yet: a share of the first launch.
+__device__ __forceinline__ void clear_bounds(int2* bounds, int64_t classes) {
+  for (int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; v < classes; v += (int64_t)gridDim.x * blockDim.x) bounds[v] = int2{0, 0};
+}
+
 // keys[r], order[r]: the token of rank r. A workgroup ranks 64 tokens, each of its 16 waves against a sixteenth of all.
-__global__ __launch_bounds__(1024) void rank_kernel(EmbedParams p, uint32_t* keys, uint32_t* order) {
+__global__ __launch_bounds__(1024) void rank_kernel(EmbedParams p, uint32_t* keys, uint32_t* order, int2* bounds) {
   __shared__ __align__(16) uint32_t all[kRankTokens + 64];
   __shared__ int part[16][64];
   const int n = (int)p.n, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  clear_bounds(bounds, p.classes);
   const int slice = (n + 63) / 64 * 4;  // tokens of a wave, a multiple of 4; 16 slices cover n
   for (int i = threadIdx.x; i < 16 * slice; i += 1024) all[i] = i < n ? key_of(p, i) : 0xffffffffu;
   __syncthreads();
@@ -107,6 +111,7 @@ struct SortPass {
   const uint32_t *from_key, *from_order;
   uint32_t *to_key, *to_order;
   uint32_t* hist;  // [tiles][digits]
+  int2* bounds;
   int shift, bits, tiles;
 };
 
@@ -114,14 +119,17 @@ __device__ __forceinline__ uint32_t sort_key(const EmbedParams& p, const SortPas
   return s.from_key ? s.from_key[n] : key_of(p, n);
 }
 
+// ROUNDS rounds of 64 tokens for each of a workgroup's four waves.
+template <int ROUNDS>
 __global__ __launch_bounds__(256) void sort_count_kernel(EmbedParams p, SortPass s) {
   __shared__ uint32_t count[kSortMost];
   const int digits = 1 << s.bits;
+  if (!s.from_key) clear_bounds(s.bounds, p.classes);
   for (int d = threadIdx.x; d < digits; d += 256) count[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile;
+  const int64_t base = (int64_t)blockIdx.x * 256 * ROUNDS;
 #pragma unroll 4
-  for (int r = 0; r < kSortTile / 256; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const int64_t n = base + r * 256 + threadIdx.x;
     if (n < p.n) atomicAdd(&count[sort_key(p, s, n) >> s.shift & (digits - 1)], 1u);  // whole numbers: any order
   }
@@ -130,22 +138,23 @@ __global__ __launch_bounds__(256) void sort_count_kernel(EmbedParams p, SortPass
 }
 
 // Places of a tile's tokens: the tokens of smaller digits, of the same digit in earlier tiles, in earlier waves of this
-// tile (a wave takes 1024 consecutive tokens), and before it in its wave (by ballots over the digit's bits).
+// tile (a wave takes consecutive tokens), and before it in its wave (by ballots over the digit's bits).
+template <int ROUNDS>
 __global__ __launch_bounds__(256) void sort_place_kernel(EmbedParams p, SortPass s) {
   __shared__ uint32_t count[4][kSortMost];  // a wave's tokens of each digit so far; then the place of its first
   __shared__ uint32_t sums[256];
   const int digits = 1 << s.bits, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   for (int d = threadIdx.x; d < 4 * kSortMost; d += 256) count[d / kSortMost][d % kSortMost] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile + wave * (kSortTile / 4);
-  uint32_t key[16], rank[16];
+  const int64_t base = ((int64_t)blockIdx.x * 4 + wave) * 64 * ROUNDS;
+  uint32_t key[ROUNDS], rank[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const int64_t n = base + r * 64 + lane;
     key[r] = n < p.n ? sort_key(p, s, n) : 0;
   }
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const bool in = base + r * 64 + lane < p.n;
     const uint32_t d = key[r] >> s.shift & (digits - 1);
     uint64_t same = __ballot(in);
@@ -165,6 +174,7 @@ __global__ __launch_bounds__(256) void sort_place_kernel(EmbedParams p, SortPass
   for (int q = 0; q < per; ++q) {
     const int d = threadIdx.x * per + q;
     if (d >= digits) break;
+#pragma unroll 8
     for (int b = 0; b < s.tiles; ++b) {
       const uint32_t h = s.hist[(int64_t)b * digits + d];
       total[q] += h;
@@ -194,7 +204,7 @@ __global__ __launch_bounds__(256) void sort_place_kernel(EmbedParams p, SortPass
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const int64_t n = base + r * 64 + lane;
     if (n < p.n) {
       const uint32_t at = count[wave][key[r] >> s.shift & (digits - 1)] + rank[r];
@@ -205,155 +215,132 @@ __global__ __launch_bounds__(256) void sort_place_kernel(EmbedParams p, SortPass
 }
 
 // ------------------------------------------------------------------------------------------ sums
-// Tokens [s, e) of the order, every `step`-th from s + first: the thread's vectors of their rows added to acc.
-template <typename T, int VEC, int NPT, int TPR>
-__device__ __forceinline__ void add_tokens(float (&acc)[NPT][VEC], const EmbedParams& p, const uint32_t* order, int64_t s, int64_t e,
-                                           int first, int step, int c0) {
-  constexpr int U = NPT > 1 ? 2 : 4;  // rows in flight
-  for (int64_t j = s + first; j < e; j += (int64_t)U * step) {
-    RawVec<T, VEC> raw[U][NPT];
+// Tokens [s, e) of the order, every `step`-th from s + first: the thread's vector of their rows added to acc, eight rows
+// in flight.
+template <typename T, int VEC>
+__device__ __forceinline__ void add_tokens(float (&acc)[VEC], const EmbedParams& p, const uint32_t* order, uint32_t s, uint32_t e, int first, int step,
+                                           int c) {
+  constexpr int U = 8;
+  for (uint32_t j = s + first; j < e; j += U * step) {
+    RawVec<T, VEC> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = j + (int64_t)u * step;
-      const T* row = (const T*)p.dout.p + (at < e ? (int64_t)order[at] : 0) * p.dout.sr;
-#pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        const int c = c0 + i * TPR * VEC;
-        if (at < e && c < p.width)
-          raw[u][i].load(row + c);
-        else
-          raw[u][i].zero();
-      }
+      const uint32_t at = j + u * step;
+      if (at < e && c < p.width)
+        raw[u].load((const T*)p.dout.p + (int64_t)order[at] * p.dout.sr + c);
+      else
+        raw[u].zero();
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      raw[u].get(f);
 #pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        float f[VEC];
-        raw[u][i].get(f);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[i][k] += f[k];
-      }
-  }
-}
-
-// acc summed over the TEAMS teams of a workgroup in team 0's threads, in the teams' order.
-template <int VEC, int NPT, int TPR>
-__device__ __forceinline__ void join_teams(float (&acc)[NPT][VEC], float* lds) {
-  constexpr int TEAMS = 256 / TPR, PER = VEC * NPT;
-  if constexpr (TEAMS > 1) {
-    const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NPT; ++i)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) lds[(team * TPR + t) * (PER + 1) + i * VEC + k] = acc[i][k];
-    __syncthreads();
-    if (team == 0) {
-      for (int q = 1; q < TEAMS; ++q)
-#pragma unroll
-        for (int i = 0; i < NPT; ++i)
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[i][k] += lds[(q * TPR + t) * (PER + 1) + i * VEC + k];
+      for (int k = 0; k < VEC; ++k) acc[k] += f[k];
     }
   }
 }
 
-template <typename T, int VEC, int NPT, int TPR>
-__global__ __launch_bounds__(256) void embed_piece_kernel(EmbedParams p, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order,
-                                                          float* __restrict__ pieces) {
+// acc summed over a workgroup's teams in team 0's threads, in the teams' order.
+template <int VEC, int TPR>
+__device__ __forceinline__ void join_teams(float (&acc)[VEC], float* lds) {
   constexpr int TEAMS = 256 / TPR;
-  __shared__ float lds[TEAMS > 1 ? 256 * (VEC * NPT + 1) : 1];
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) lds[(team * TPR + t) * (VEC + 1) + k] = acc[k];
+  __syncthreads();
+  if (team == 0) {
+#pragma unroll
+    for (int q = 1; q < TEAMS; ++q)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += lds[(q * TPR + t) * (VEC + 1) + k];
+  }
+}
+
+// Sums of the pieces that hold one id, and every row's bounds in the order: the tokens where the id changes write them.
+template <typename T, int VEC, int TPR>
+__global__ __launch_bounds__(256) void embed_piece_kernel(EmbedParams p, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order,
+                                                          int2* __restrict__ bounds, float* __restrict__ pieces) {
+  constexpr int TEAMS = 256 / TPR;
+  __shared__ float lds[256 * (VEC + 1)];
   const int64_t s = (int64_t)blockIdx.x * kPiece;
+  if (blockIdx.y == 0 && threadIdx.x < kPiece && s + threadIdx.x < p.n) {
+    const int64_t i = s + threadIdx.x;
+    const uint32_t key = keys[i];
+    if (key < p.classes) {
+      if (i == 0 || keys[i - 1] != key) bounds[key].x = (int)i;
+      if (i + 1 == p.n || keys[i + 1] != key) bounds[key].y = (int)i + 1;
+    }
+  }
+  if (s + kPiece > p.n) return;
   const uint32_t key = keys[s];
   if (key != keys[s + kPiece - 1] || key >= p.classes) return;
-  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c0 = (blockIdx.y * NPT * TPR + t) * VEC;
-  float acc[NPT][VEC] = {};
-  add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, s + kPiece, team, TEAMS, c0);
-  join_teams<VEC, NPT, TPR>(acc, lds);
-  if (team != 0) return;
-#pragma unroll
-  for (int i = 0; i < NPT; ++i) {
-    const int c = c0 + i * TPR * VEC;
-    if (c < p.width) {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) pieces[(int64_t)blockIdx.x * p.width + c + k] = acc[i][k];
-    }
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c = (blockIdx.y * TPR + t) * VEC;
+  float acc[VEC] = {};
+  add_tokens<T, VEC>(acc, p, order, (uint32_t)s, (uint32_t)s + kPiece, team, TEAMS, c);
+  join_teams<VEC, TPR>(acc, lds);
+  if (team == 0 && c < p.width) {
+    RawVec<float, VEC> out;
+    out.set(acc);
+    out.store(pieces + (int64_t)blockIdx.x * p.width + c);
   }
 }
 
-// First of n sorted keys that is not below v.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t v) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (keys[mid] < v)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  return lo;
-}
-
-constexpr int kRowsMost = 16;  // table rows of a workgroup
-constexpr int kTeamTokens = 8;  // most tokens that one of several teams sums alone
+constexpr int kRowsMost = 16;   // table rows of a workgroup
+constexpr int kTeamTokens = 8;  // most tokens that a team sums alone
 
 // `rows` table rows of a workgroup, one for each team in turn; rows with more tokens take all the teams.
-template <typename T, int VEC, int NPT, int TPR>
-__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order,
+template <typename T, int VEC, int TPR>
+__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const uint32_t* __restrict__ order, const int2* __restrict__ bounds,
                                                          const float* __restrict__ pieces, int rows) {
   constexpr int TEAMS = 256 / TPR;
-  __shared__ float lds[TEAMS > 1 ? 256 * (VEC * NPT + 1) : 1];
-  __shared__ int64_t bound[kRowsMost + 1];
+  __shared__ float lds[256 * (VEC + 1)];
+  __shared__ int2 bound[kRowsMost];
   const int64_t v0 = (int64_t)blockIdx.x * rows;
-  if ((int)threadIdx.x <= rows) bound[threadIdx.x] = lower_bound(keys, p.n, (uint32_t)min(v0 + threadIdx.x, p.classes));
-  __syncthreads();
-  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c0 = (blockIdx.y * NPT * TPR + t) * VEC;
-  auto write = [&](const float(&acc)[NPT][VEC], int64_t v) {
-#pragma unroll
-    for (int i = 0; i < NPT; ++i) {
-      const int c = c0 + i * TPR * VEC;
-      if (c >= p.width) continue;
-      float f[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = acc[i][k] * p.scale;
-      RawVec<T, VEC> out;
-      out.set(f);
-      out.store((T*)p.out.p + v * p.out.sr + c);
-    }
-  };
   const int have = (int)min((int64_t)rows, p.classes - v0);
-  if constexpr (TEAMS > 1) {
-    for (int r = team; r < have; r += TEAMS) {
-      const int64_t s = bound[r], e = bound[r + 1];
-      if (e - s > kTeamTokens) continue;
-      float acc[NPT][VEC] = {};
-      add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, e, 0, 1, c0);
-      write(acc, v0 + r);
-    }
+  if ((int)threadIdx.x < have) bound[threadIdx.x] = p.n ? bounds[v0 + threadIdx.x] : int2{0, 0};
+  __syncthreads();
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c = (blockIdx.y * TPR + t) * VEC;
+  auto write = [&](const float(&acc)[VEC], int64_t v) {
+    if (c >= p.width) return;
+    float f[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[k] = acc[k] * p.scale;
+    RawVec<T, VEC> out;
+    out.set(f);
+    out.store((T*)p.out.p + v * p.out.sr + c);
+  };
+  for (int r = team; r < have; r += TEAMS) {
+    const int2 at = bound[r];
+    if (at.y - at.x > kTeamTokens) continue;
+    float acc[VEC] = {};
+    add_tokens<T, VEC>(acc, p, order, at.x, at.y, 0, 1, c);
+    write(acc, v0 + r);
   }
   for (int r = 0; r < have; ++r) {
-    const int64_t s = bound[r], e = bound[r + 1];
-    if (TEAMS > 1 && e - s <= kTeamTokens) continue;
-    const int64_t a = (s + kPiece - 1) / kPiece, b = e / kPiece;  // whole pieces [a, b)
-    float acc[NPT][VEC] = {};
+    const int s = bound[r].x, e = bound[r].y;
+    if (e - s <= kTeamTokens) continue;
+    const int a = (s + kPiece - 1) / kPiece, b = e / kPiece;  // whole pieces [a, b)
+    float acc[VEC] = {};
     if (a < b) {
-      add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, a * kPiece, team, TEAMS, c0);
-      for (int64_t q = a + team; q < b; q += TEAMS) {
+      add_tokens<T, VEC>(acc, p, order, s, a * kPiece, team, TEAMS, c);
+      if (c < p.width) {
+#pragma unroll 4
+        for (int q = a + team; q < b; q += TEAMS) {
+          RawVec<float, VEC> raw;
+          raw.load(pieces + (int64_t)q * p.width + c);
+          float f[VEC];
+          raw.get(f);
 #pragma unroll
-        for (int i = 0; i < NPT; ++i) {
-          const int c = c0 + i * TPR * VEC;
-          if (c < p.width) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[i][k] += pieces[q * p.width + c + k];
-          }
+          for (int k = 0; k < VEC; ++k) acc[k] += f[k];
         }
       }
-      add_tokens<T, VEC, NPT, TPR>(acc, p, order, b * kPiece, e, team, TEAMS, c0);
+      add_tokens<T, VEC>(acc, p, order, b * kPiece, e, team, TEAMS, c);
     } else {
-      add_tokens<T, VEC, NPT, TPR>(acc, p, order, s, e, team, TEAMS, c0);
+      add_tokens<T, VEC>(acc, p, order, s, e, team, TEAMS, c);
     }
-    join_teams<VEC, NPT, TPR>(acc, lds);
+    join_teams<VEC, TPR>(acc, lds);
     if (team == 0) write(acc, v0 + r);
   }
 }
@@ -370,56 +357,85 @@ int key_bits(int64_t classes) {  // keys run from 0 to classes
 template <typename T, int VEC, int TPR>
 hipError_t fwd(const EmbedParams& p, hipStream_t st) {
   constexpr int TEAMS = 256 / TPR, COLS = 2 * TPR * VEC;
-  embed_fwd_kernel<T, VEC, TPR><<<dim3((unsigned)((p.n + TEAMS - 1) / TEAMS), (p.width + COLS - 1) / COLS), 256, 0, st>>>(p);
-  return hipGetLastError();
+  // a launch holds fewer than 2^32 threads in x
+  for (int64_t n = 0; n < p.n; n += int64_t(1) << 23) {
+    EmbedParams q = p;
+    q.n = p.n - n < int64_t(1) << 23 ? p.n - n : int64_t(1) << 23;
+    q.ids = (const char*)p.ids + n * (p.ids64 ? 8 : 4);
+    q.out.p = (T*)p.out.p + n * p.out.sr;
+    embed_fwd_kernel<T, VEC, TPR><<<dim3((unsigned)((q.n + TEAMS - 1) / TEAMS), (p.width + COLS - 1) / COLS), 256, 0, st>>>(q);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 struct Order {
   uint32_t *keys, *order;
+  int2* bounds;
+  float* pieces;
+};
+
+// A radix sort's workgroup takes 1024 tokens, or 4096 where so many workgroups would each read too many others' counts.
+constexpr int64_t kSmallSort = 131072;
+int sort_tiles(int64_t n) { return (int)((n + 1023) / 1024 <= kSmallSort / 1024 ? (n + 1023) / 1024 : (n + 4095) / 4096); }
+
+// The workspace: keys and order twice, the digits' counts, the rows' bounds, and a float32 row for each piece.
+struct Space {
+  int64_t each, hist, bounds, pieces, bytes;
+  explicit Space(const EmbedParams& p)
+      : each(align256(4 * p.n)),
+        hist(4 * each),
+        bounds(hist + align256(4 * kSortMost * (int64_t)sort_tiles(p.n))),
+        pieces(bounds + align256(8 * p.classes)),
+        bytes(pieces + 4 * (p.n / kPiece) * p.width) {}
 };
 
 hipError_t sort_tokens(const EmbedParams& p, Order& o, hipStream_t st) {
   char* ws = (char*)p.ws;
-  const int64_t each = align256(4 * p.n);
-  uint32_t *key[2] = {(uint32_t*)ws, (uint32_t*)(ws + each)}, *ord[2] = {(uint32_t*)(ws + 2 * each), (uint32_t*)(ws + 3 * each)};
+  const Space at(p);
+  uint32_t *key[2] = {(uint32_t*)ws, (uint32_t*)(ws + at.each)}, *ord[2] = {(uint32_t*)(ws + 2 * at.each), (uint32_t*)(ws + 3 * at.each)};
+  o = {key[0], ord[0], (int2*)(ws + at.bounds), (float*)(ws + at.pieces)};
+  if (p.n == 0) return hipSuccess;
   if (p.n <= kRankTokens) {
-    rank_kernel<<<dim3((unsigned)((p.n + 63) / 64)), 1024, 0, st>>>(p, key[0], ord[0]);
-    o = {key[0], ord[0]};
+    rank_kernel<<<dim3((unsigned)((p.n + 63) / 64)), 1024, 0, st>>>(p, o.keys, o.order, o.bounds);
     return hipGetLastError();
   }
   const int bits = key_bits(p.classes), passes = (bits + 9) / 10, each_bits = (bits + passes - 1) / passes;
-  const int tiles = (int)((p.n + kSortTile - 1) / kSortTile);
-  SortPass s{nullptr, nullptr, key[0], ord[0], (uint32_t*)(ws + 4 * each), 0, each_bits, tiles};
+  const int tiles = sort_tiles(p.n);
+  SortPass s{nullptr, nullptr, key[0], ord[0], (uint32_t*)(ws + at.hist), o.bounds, 0, each_bits, tiles};
   for (int q = 0; q < passes; ++q) {
     s.to_key = key[q & 1], s.to_order = ord[q & 1];
-    sort_count_kernel<<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
-    sort_place_kernel<<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+    if (p.n <= kSmallSort) {
+      sort_count_kernel<4><<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+      sort_place_kernel<4><<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+    } else {
+      sort_count_kernel<16><<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+      sort_place_kernel<16><<<dim3((unsigned)tiles), 256, 0, st>>>(p, s);
+    }
     s.from_key = s.to_key, s.from_order = s.to_order;
     s.shift += each_bits;
   }
-  o = {s.to_key, s.to_order};
+  o.keys = s.to_key, o.order = s.to_order;
   return hipGetLastError();
 }
 
-template <typename T, int VEC, int NPT, int TPR>
+template <typename T, int VEC, int TPR>
 hipError_t bwd(const EmbedParams& p, hipStream_t st) {
-  constexpr int COLS = NPT * TPR * VEC;
+  constexpr int COLS = TPR * VEC;
   const unsigned cols = (unsigned)((p.width + COLS - 1) / COLS);
-  Order o{nullptr, nullptr};
-  float* pieces = (float*)((char*)p.ws + embed_ws_bytes(p)) - p.n / kPiece * p.width;
+  Order o;
+  hipError_t e = sort_tokens(p, o, st);
+  if (e != hipSuccess) return e;
   if (p.n > 0) {
-    hipError_t e = sort_tokens(p, o, st);
+    embed_piece_kernel<T, VEC, TPR><<<dim3((unsigned)((p.n + kPiece - 1) / kPiece), cols), 256, 0, st>>>(p, o.keys, o.order, o.bounds, o.pieces);
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (p.n >= kPiece) {
-      embed_piece_kernel<T, VEC, NPT, TPR><<<dim3((unsigned)(p.n / kPiece), cols), 256, 0, st>>>(p, o.keys, o.order, pieces);
-      e = hipGetLastError();
-      if (e != hipSuccess) return e;
-    }
   }
-  // several rows for a workgroup (one binary search for all) once they fill the GPU
-  const int64_t per = p.classes * cols / (8 * (int64_t)device_cu_count());
+  // several rows for a workgroup once they fill the GPU
+  const int64_t per = p.classes * cols / (16 * (int64_t)device_cu_count());
   const int rows = (int)(per < 1 ? 1 : per < kRowsMost ? per : kRowsMost);
-  embed_rows_kernel<T, VEC, NPT, TPR><<<dim3((unsigned)((p.classes + rows - 1) / rows), cols), 256, 0, st>>>(p, o.keys, o.order, pieces, rows);
+  embed_rows_kernel<T, VEC, TPR><<<dim3((unsigned)((p.classes + rows - 1) / rows), cols), 256, 0, st>>>(p, o.order, o.bounds, o.pieces, rows);
   return hipGetLastError();
 }
 
@@ -427,10 +443,10 @@ template <typename T, bool GRAD>
 hipError_t by_width(const EmbedParams& p, hipStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const int n = p.vec ? p.width / V : p.width;
-#define THERIA_EMBED_CASE(VEC, TPR)               \
-  if constexpr (GRAD)                             \
-    return bwd<T, VEC, TPR == 256 ? 2 : 1, TPR>(p, st); \
-  else                                            \
+#define THERIA_EMBED_CASE(VEC, TPR)                       \
+  if constexpr (GRAD)                                     \
+    return bwd<T, VEC, TPR == 16 ? 16 : 64>(p, st);       \
+  else                                                    \
     return fwd<T, VEC, TPR>(p, st);
   if (p.vec) {
     if (n <= 16) { THERIA_EMBED_CASE(V, 16) }
@@ -452,11 +468,7 @@ hipError_t by_type(const EmbedParams& p, hipStream_t st) {
 
 }  // namespace
 
-// Keys and order twice, the digits' counts, and a float32 row for each piece.
-int64_t embed_ws_bytes(const EmbedParams& p) {
-  const int64_t tiles = (p.n + kSortTile - 1) / kSortTile;
-  return 4 * align256(4 * p.n) + align256(4 * kSortMost * tiles) + 4 * (p.n / kPiece) * p.width;
-}
+int64_t embed_ws_bytes(const EmbedParams& p) { return Space(p).bytes; }
 hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st) { return by_type<false>(p, st); }
 hipError_t launch_embed_bwd(const EmbedParams& p, hipStream_t st) { return by_type<true>(p, st); }
 

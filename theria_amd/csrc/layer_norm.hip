@@ -335,8 +335,18 @@ struct Fwd {
   template <typename T, typename WT, int VEC, int NPT, int TPR>
   static hipError_t run(const NormParams& p, hipStream_t st) {
     constexpr int TEAMS = kBlock<TPR> / TPR;
-    norm_fwd_kernel<T, WT, VEC, NPT, TPR><<<dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), kBlock<TPR>, 0, st>>>(p);
-    return hipGetLastError();
+    constexpr int64_t most = int64_t(1) << 21;  // rows: a launch holds fewer than 2^32 threads
+    for (int64_t r = 0; r < p.rows; r += most) {
+      NormParams q = p;
+      q.rows = p.rows - r < most ? p.rows - r : most;
+      q.x.p = (const T*)p.x.p + r * p.x.sr;
+      q.y.p = (T*)p.y.p + r * p.y.sr;
+      q.mean = p.mean + r, q.rstd = p.rstd + r;
+      norm_fwd_kernel<T, WT, VEC, NPT, TPR><<<dim3((unsigned)((q.rows + TEAMS - 1) / TEAMS)), kBlock<TPR>, 0, st>>>(q);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
   }
 };
 

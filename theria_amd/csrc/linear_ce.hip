@@ -366,24 +366,39 @@ struct OutTile {
 };
 
 // ------------------------------------------------------------------------------------------ joins
-// Eight rows a workgroup, their tiles spread over 32 threads each. Dropped rows: zero, or NaN where the target is invalid.
+// R rows a workgroup, each one's tiles spread over 256 / R threads. Dropped rows: zero, or NaN where the target is invalid.
+template <int R>
 __global__ __launch_bounds__(256) void ce_join_kernel(CeParams p, int tiles, const float2* part, const float* at_target, const int* map,
                                                       const Meta* meta, float* row_loss) {
-  __shared__ float2 red[32][9];
-  const int r = threadIdx.x % 8, s = threadIdx.x / 8;
-  const int64_t j = (int64_t)blockIdx.x * 8 + r;
+  constexpr int S = 256 / R;
+  __shared__ float2 red[S][R + 1];
+  const int r = threadIdx.x % R, s = threadIdx.x / R;
+  const int64_t j = (int64_t)blockIdx.x * R + r;
   const int kept = meta->kept;
   float top = -THERIA_INF, sum = 0.f;
   if (j < kept) {
-    for (int k = s; k < tiles; k += 32) top = fmaxf(top, part[(int64_t)k * p.n + j].x);
+#pragma unroll 4
+    for (int k = s; k < tiles; k += S) top = fmaxf(top, part[(int64_t)k * p.n + j].x);
     const float off = top == -THERIA_INF ? 0.f : top;
-    for (int k = s; k < tiles; k += 32) {
+#pragma unroll 4
+    for (int k = s; k < tiles; k += S) {
       const float2 v = part[(int64_t)k * p.n + j];
       sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));
     }
   }
   red[s][r] = float2{top, sum};
-  __syncthreads();
+  // halves of the slices joined in turn, in an order that does not depend on the run
+#pragma unroll
+  for (int o = S / 2; o > 0; o /= 2) {
+    __syncthreads();
+    if (s < o) {
+      const float2 a = red[s][r], b = red[s + o][r];
+      top = fmaxf(a.x, b.x);
+      const float off = top == -THERIA_INF ? 0.f : top;
+      sum = a.y * (a.x == -THERIA_INF ? 1.f : fast_exp2((a.x - off) * kLog2e)) + b.y * (b.x == -THERIA_INF ? 1.f : fast_exp2((b.x - off) * kLog2e));
+      red[s][r] = float2{top, sum};
+    }
+  }
   if (s != 0 || j >= p.n) return;
   if (j >= kept) {
     if (row_loss) {
@@ -391,13 +406,6 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeParams p, int tiles, con
       row_loss[row < 0 ? -row - 1 : row] = row < 0 ? __builtin_nanf("") : 0.f;
     }
     return;
-  }
-  for (int k = 1; k < 32; ++k) top = fmaxf(top, red[k][r].x);
-  const float off = top == -THERIA_INF ? 0.f : top;
-  sum = 0.f;
-  for (int k = 0; k < 32; ++k) {
-    const float2 v = red[k][r];
-    sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));
   }
   p.stats[j] = top;
   p.stats[p.n + j] = sum;
@@ -639,7 +647,15 @@ struct Call {
       tile0 += (int)(up(have, tile_i(l.tf)) / tile_i(l.tf));
     }
     float* row_loss = p.reduction == kCeNone ? p.loss : (float*)(ws + l.row_loss);
-    if (p.n > 0) ce_join_kernel<<<dim3((unsigned)((p.n + 7) / 8)), 256, 0, st>>>(p, l.tiles, (const float2*)(ws + l.part), (const float*)(ws + l.at_target), map, meta, row_loss);
+    // few rows: a workgroup for each, so that the tiles' partial sums are read by more threads
+    if (p.n > 0) {
+      const float2* part = (const float2*)(ws + l.part);
+      const float* at = (const float*)(ws + l.at_target);
+      if (p.n <= 1024)
+        ce_join_kernel<1><<<dim3((unsigned)p.n), 256, 0, st>>>(p, l.tiles, part, at, map, meta, row_loss);
+      else
+        ce_join_kernel<8><<<dim3((unsigned)((p.n + 7) / 8)), 256, 0, st>>>(p, l.tiles, part, at, map, meta, row_loss);
+    }
     THERIA_TRY(hipGetLastError());
     if (p.reduction != kCeNone) ce_total_kernel<<<1, 1024, 0, st>>>(p, row_loss, meta);
     return hipGetLastError();

@@ -240,7 +240,7 @@ hipError_t launch_gemm(const GemmParams& p, const Epi& epi, hipStream_t st) {
   // p.J is the most that the kept rows can be: workgroups beyond the tiles that there are return at once
   const int64_t tiles = (int64_t)((p.I + S::TI - 1) / S::TI) * ((p.J + S::TJ - 1) / S::TJ) * p.splits;
   if (tiles == 0) return hipSuccess;
-  if (tiles > 0x7fffff00) return hipErrorInvalidValue;
+  if (tiles * S::NW * 64 >= (int64_t(1) << 32)) return hipErrorInvalidValue;  // more threads than a launch holds
   gemm_kernel<S, Epi><<<dim3((unsigned)((tiles + 7) / 8 * 8)), S::NW * 64, 0, st>>>(p, epi);
   return hipGetLastError();
 }
