@@ -293,15 +293,15 @@ constexpr int kTeamTokens = 8;  // most tokens that a team sums alone
 // `rows` table rows of a workgroup, one for each team in turn; rows with more tokens take all the teams.
 template <typename T, int VEC, int TPR>
 __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const uint32_t* __restrict__ order, const int2* __restrict__ bounds,
-                                                         const float* __restrict__ pieces, int rows) {
+                                                         const float* __restrict__ pieces, int rows, int cols) {
   constexpr int TEAMS = 256 / TPR;
   __shared__ float lds[256 * (VEC + 1)];
   __shared__ int2 bound[kRowsMost];
-  const int64_t v0 = (int64_t)blockIdx.x * rows;
+  const int64_t v0 = (int64_t)(blockIdx.x / cols) * rows;
   const int have = (int)min((int64_t)rows, p.classes - v0);
   if ((int)threadIdx.x < have) bound[threadIdx.x] = p.n ? bounds[v0 + threadIdx.x] : int2{0, 0};
   __syncthreads();
-  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c = (blockIdx.y * TPR + t) * VEC;
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c = ((int)(blockIdx.x % cols) * TPR + t) * VEC;
   auto write = [&](const float(&acc)[VEC], int64_t v) {
     if (c >= p.width) return;
     float f[VEC];
@@ -435,8 +435,16 @@ hipError_t bwd(const EmbedParams& p, hipStream_t st) {
   // several rows for a workgroup once they fill the GPU
   const int64_t per = p.classes * cols / (16 * (int64_t)device_cu_count());
   const int rows = (int)(per < 1 ? 1 : per < kRowsMost ? per : kRowsMost);
-  embed_rows_kernel<T, VEC, TPR><<<dim3((unsigned)((p.classes + rows - 1) / rows), cols), 256, 0, st>>>(p, o.order, o.bounds, o.pieces, rows);
-  return hipGetLastError();
+  const int64_t most = (int64_t(1) << 23) / cols * rows;  // table rows: a launch holds fewer than 2^32 threads
+  for (int64_t v = 0; v < p.classes; v += most) {
+    EmbedParams q = p;
+    q.classes = p.classes - v < most ? p.classes - v : most;
+    q.out.p = (T*)p.out.p + v * p.out.sr;
+    embed_rows_kernel<T, VEC, TPR><<<dim3((unsigned)((q.classes + rows - 1) / rows * cols)), 256, 0, st>>>(q, o.order, o.bounds + v, o.pieces, rows, (int)cols);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T, bool GRAD>

@@ -176,7 +176,7 @@ struct LogitStats {
   int tile0;          // the piece's first tile
 
   template <class S>
-  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char*) const {
     __shared__ float2 red[S::WI][S::TJ];
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
     finish_logits<S>(z, t, bias, dtype, v0);
@@ -243,17 +243,17 @@ struct LogitGrad {
   int64_t plane;
 
   template <class S>
-  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     using H = typename S::H;
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
     finish_logits<S>(z, t, bias, dtype, v0);
 #pragma unroll
     for (int fj = 0; fj < S::FJ; ++fj) {
       const int j = t.j0 + 32 * fj + li;
-      if (j >= t.J) continue;
-      const float top = stats[j], inv = 1.0f / stats[n + j];
+      const bool in = j < t.J;
+      const float top = in ? stats[j] : 0.f, inv = in ? 1.0f / stats[n + j] : 0.f;
       float unit = __is_same(H, _Float16) ? 0x1p14f : 1.f;
-      if (gout) {
+      if (in && gout) {
         const float go = gout[map[j]], most = meta->most;
         // a gradient that is not finite keeps its own value: it is not in `most`
         unit *= !(fabsf(go) < THERIA_INF) ? go : most > 0.f ? go / most : 0.f;
@@ -263,33 +263,39 @@ struct LogitGrad {
       for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[fi][fj][r] = fast_exp2((z[fi][fj][r] - top) * kLog2e) * inv;
-      const int64_t want = (int64_t)target[j] - v0 - t.i0;
+      const int64_t want = in ? (int64_t)target[j] - v0 - t.i0 : -1;
       if (want >= 0 && want < 32 * S::FI) {
 #pragma unroll
         for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
           for (int r = 0; r < 16; ++r) z[fi][fj][r] -= want == 32 * fi + acc_row(r, g) ? 1.f : 0.f;
       }
-      char* row = dz + ((int64_t)j * ld + t.i0 + 4 * g) * 2;
-      const int room = ld - t.i0 - 4 * g;
 #pragma unroll
-      for (int fi = 0; fi < S::FI; ++fi)
+      for (int fi = 0; fi < S::FI; ++fi) z[fi][fj] *= unit;
+    }
+    using Stage = GemmStage<S, 2>;
+    // each plane in turn: what the last ones held is taken off first
+#pragma unroll 1
+    for (int k = 0; k < PLANES; ++k) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (32 * fi + 8 * q >= room) continue;
-          H out[PLANES][4];
+      for (int fj = 0; fj < S::FJ; ++fj)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = z[fi][fj][4 * q + e] * unit;
-            if constexpr (PLANES == 1)
-              out[0][e] = (H)v;
-            else
-              split3(v, out[0][e], out[1][e], out[2][e]);
+        for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            H out[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = z[fi][fj][4 * q + e];
+              out[e] = (H)v;
+              // an infinity or NaN is whole in its first plane
+              if constexpr (PLANES > 1) z[fi][fj][4 * q + e] = fabsf(v) < THERIA_INF ? v - (float)out[e] : 0.f;
+            }
+            Stage::put(lds, 32 * fj + li, fi, q, g, out);
           }
-#pragma unroll
-          for (int k = 0; k < PLANES; ++k)
-            *reinterpret_cast<uint2*>(row + k * plane + (32 * fi + 8 * q) * 2) = *reinterpret_cast<const uint2*>(out[k]);
-        }
+      Stage::each(lds, 32 * S::FJ, [&](int r, int i, const i32x4_t& v) {
+        if (t.j0 + r < t.J && t.i0 + i < ld) *reinterpret_cast<i32x4_t*>(dz + k * plane + ((int64_t)(t.j0 + r) * ld + t.i0 + i) * 2) = v;
+      });
     }
   }
 };
@@ -302,23 +308,26 @@ struct SumTile {
   bool add;
 
   template <class S>
-  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+    using Stage = GemmStage<S, 4>;
 #pragma unroll
     for (int fj = 0; fj < S::FJ; ++fj) {
-      const int j = t.j0 + 32 * fj + li;
-      if (j >= t.J) continue;
-      float* row = sums + (t.split * rows + j) * ld;
 #pragma unroll
       for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
-          if (i >= ld) continue;
-          f32x4_t v = {z[fi][fj][4 * q], z[fi][fj][4 * q + 1], z[fi][fj][4 * q + 2], z[fi][fj][4 * q + 3]};
-          if (add) v += *reinterpret_cast<const f32x4_t*>(row + i);
-          *reinterpret_cast<f32x4_t*>(row + i) = v;
+          const f32x4_t v = {z[fi][fj][4 * q], z[fi][fj][4 * q + 1], z[fi][fj][4 * q + 2], z[fi][fj][4 * q + 3]};
+          Stage::put(lds, li, fi, q, g, &v);
         }
+      const int j0 = t.j0 + 32 * fj;
+      Stage::each(lds, 32, [&](int r, int i, const i32x4_t& c) {
+        if (j0 + r >= t.J || t.i0 + i >= ld) return;
+        f32x4_t* to = reinterpret_cast<f32x4_t*>(sums + (t.split * rows + j0 + r) * ld + t.i0 + i);
+        f32x4_t v = __builtin_bit_cast(f32x4_t, c);
+        if (add) v += *to;
+        *to = v;
+      });
     }
   }
 };
@@ -328,39 +337,42 @@ template <typename T>
 struct OutTile {
   T* out;
   int64_t sr;
-  bool vec;  // four elements at a time
+  bool vec;  // 16 bytes at a time
   const Meta* meta;
 
   template <class S>
-  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+  __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
     const float f = meta->factor;
+    using Stage = GemmStage<S, (int)sizeof(T)>;
+    // the share holds every row of 16-bit results, or one block's rows of float32 ones
+    constexpr int kBlocks = sizeof(T) == 2 ? S::FJ : 1, kPer = 16 / (int)sizeof(T);
 #pragma unroll
-    for (int fj = 0; fj < S::FJ; ++fj) {
-      const int j = t.j0 + 32 * fj + li;
-      if (j >= t.J) continue;
-      T* row = out + j * sr;
+    for (int f0 = 0; f0 < S::FJ; f0 += kBlocks) {
 #pragma unroll
-      for (int fi = 0; fi < S::FI; ++fi)
+      for (int fj = f0; fj < f0 + kBlocks; ++fj)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
-          T v[4];
+        for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (T)(z[fi][fj][4 * q + e] * f);
-          if (vec) {
-            if (i < t.I) {
-              if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<uint2*>(row + i) = *reinterpret_cast<const uint2*>(v);
-              else
-                *reinterpret_cast<u32x4_t*>(row + i) = *reinterpret_cast<const u32x4_t*>(v);
-            }
-          } else {
+          for (int q = 0; q < 4; ++q) {
+            T v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e < t.I) row[i + e] = v[e];
+            for (int e = 0; e < 4; ++e) v[e] = (T)(z[fi][fj][4 * q + e] * f);
+            Stage::put(lds, 32 * (fj - f0) + li, fi, q, g, v);
           }
+      const int j0 = t.j0 + 32 * f0;
+      Stage::each(lds, 32 * kBlocks, [&](int r, int i, const i32x4_t& c) {
+        if (j0 + r >= t.J || t.i0 + i >= t.I) return;
+        T* to = out + (j0 + r) * sr + t.i0 + i;
+        if (vec) {
+          *reinterpret_cast<i32x4_t*>(to) = c;
+        } else {
+          const T* v = reinterpret_cast<const T*>(&c);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (t.i0 + i + e < t.I) to[e] = v[e];
         }
+      });
     }
   }
 };
@@ -683,7 +695,9 @@ struct Call {
         const bool vec = w4 && p.dw.sr % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
         const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.sw, segments(), &meta->kept, false, true};
         if (l.sw == 1) {
-          THERIA_TRY((gemm<H, true, true>(l.tw, g, OutTile<T>{out, p.dw.sr, vec, meta}, st)));
+          constexpr int V = 16 / (int)sizeof(T);
+          const bool whole = p.width % V == 0 && p.dw.sr % V == 0 && (uintptr_t)out % 16 == 0;
+          THERIA_TRY((gemm<H, true, true>(l.tw, g, OutTile<T>{out, p.dw.sr, whole, meta}, st)));
         } else {
           float* sums = (float*)(ws + l.sum_w);
           THERIA_TRY((gemm<H, true, true>(l.tw, g, SumTile{sums, l.piece, l.ldx, false}, st)));

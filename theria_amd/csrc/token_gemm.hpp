@@ -16,6 +16,8 @@
 
 namespace theria {
 
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
 constexpr int kGemmK = 64;  // k per step
 
 struct GemmOperand {
@@ -136,6 +138,38 @@ struct GemmShape {
   static constexpr int FI = TI_ / WI_ / 32, FJ = TJ_ / WJ_ / 32;
 };
 
+// A wave's results on their way to memory through its share of the LDS: a lane has four consecutive i of one j, memory
+// wants whole rows of i. Rows j of 32 FI elements, in 16-byte chunks swizzled by the row. Element: 2 or 4 bytes; a
+// 2-byte piece is half a chunk. (Stores of 8 bytes from the accumulators' layout touch 32 rows each.)
+template <class S, int ELEM>
+struct GemmStage {
+  static constexpr int kChunks = 32 * S::FI * ELEM / 16, kRow = 16 * kChunks;
+  __device__ __forceinline__ static int at(int row, int chunk) { return row * kRow + ((chunk ^ row) % kChunks << 4); }
+  // four values of row `row` from i = 32 fi + 8 q + 4 g
+  __device__ __forceinline__ static void put(char* lds, int row, int fi, int q, int g, const void* v) {
+    if constexpr (ELEM == 2)
+      *reinterpret_cast<uint2*>(lds + at(row, 4 * fi + q) + 8 * g) = *static_cast<const uint2*>(v);
+    else
+      *reinterpret_cast<i32x4_t*>(lds + at(row, 8 * fi + 2 * q + g)) = *static_cast<const i32x4_t*>(v);
+  }
+  // f(row, i, chunk) for every chunk of `rows` rows, a wave instruction over whole rows
+  template <class F>
+  __device__ __forceinline__ static void each(const char* lds, int rows, const F& f) {
+    constexpr int kRows = 64 / kChunks;  // rows of an instruction
+    const int lane = threadIdx.x & 63;
+    wave_order();
+#pragma unroll 4
+    for (int r = lane / kChunks; r < rows; r += kRows)
+      f(r, lane % kChunks * (16 / ELEM), *reinterpret_cast<const i32x4_t*>(lds + at(r, lane % kChunks)));
+    wave_order();
+  }
+  // The lanes of a wave read what others of its lanes wrote: LDS keeps a wave's order, and so must the compiler.
+  __device__ __forceinline__ static void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
 template <class S, class Epi>
 __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi) {
   using H = typename S::H;
@@ -232,7 +266,12 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
     __syncthreads();
     products(a0, b0);
   }
-  epi.template run<S>(acc, t);
+  __syncthreads();  // the tiles are read: each wave takes 2 KB of their LDS for a 32 x 32 block
+  constexpr int kShare = FI * FJ * 2048, kPer = TI * 128 / kShare;
+  static_assert(NW <= kPer || (TI == TJ && NW <= 4 * kPer));
+  const int part = wave / kPer;
+  char* const lds = part == 0 ? a0 : part == 1 ? b0 : part == 2 ? a1 : b1;
+  epi.template run<S>(acc, t, lds + wave % kPer * kShare);
 }
 
 template <class S, class Epi>
