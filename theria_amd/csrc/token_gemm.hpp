@@ -227,44 +227,57 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
   GemmFrags<H, S::B, FJ> rb;
   ra.init(t.wave_i * (TI / S::WI));
   rb.init(t.wave_j * (TJ / S::WJ));
-  // The fragments of chunk c + 1 are read while chunk c's products run, and no earlier (the barriers bound the registers).
-  auto products = [&](const char* a, const char* b) __attribute__((always_inline)) {
-    constexpr int NC = kGemmK / 16;
-    typename Mfma<H>::frag_t fa[2][FI], fb[2][FJ];
-    auto read = [&](int c) __attribute__((always_inline)) {
+  // A stage's products, chunk by chunk: chunk c + 1 is read while chunk c's products run, and no earlier (the barriers
+  // bound the registers). The last chunk's products wait for the next stage, whose first chunk is read meanwhile: after
+  // the workgroup's barrier every wave has products to run.
+  constexpr int NC = kGemmK / 16;
+  typename Mfma<H>::frag_t fa[2][FI], fb[2][FJ];
+  auto read = [&](const char* a, const char* b, int c) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < FI; ++i) fa[c & 1][i] = ra.get(a, i, c);
+    for (int i = 0; i < FI; ++i) fa[c & 1][i] = ra.get(a, i, c);
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) fb[c & 1][j] = rb.get(b, j, c);
-    };
-    read(0);
+    for (int j = 0; j < FJ; ++j) fb[c & 1][j] = rb.get(b, j, c);
+  };
+  auto products = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      __builtin_amdgcn_sched_barrier(0);
-      if (c + 1 < NC) read(c + 1);
+    for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int i = 0; i < FI; ++i)
-#pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = Mfma<H>::mma(fa[c & 1][i], fb[c & 1][j], acc[i][j]);
-    }
+      for (int j = 0; j < FJ; ++j) acc[i][j] = Mfma<H>::mma(fa[c & 1][i], fb[c & 1][j], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (steps > 0) copy(a0, b0);
-  int s = 0;
-  for (; s + 2 <= steps; s += 2) {
+  auto stage = [&](const char* a, const char* b, bool first) __attribute__((always_inline)) {
+    read(a, b, 0);
+    if (!first) products(NC - 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c + 1 < NC; ++c) {
+      read(a, b, c + 1);
+      products(c);
+    }
+  };
+  auto arrive = [&]() __attribute__((always_inline)) {
     wait_vm_all();
-    __syncthreads();  // this stage is there for every wave, and every wave is done with the other one
-    copy(a1, b1);
-    products(a0, b0);
-    wait_vm_all();
-    __syncthreads();
-    if (s + 2 < steps) copy(a0, b0);
-    products(a1, b1);
-  }
-  if (s < steps) {
-    wait_vm_all();
-    __syncthreads();
-    products(a0, b0);
+    __syncthreads();  // a stage is there for every wave, and every wave has read the other one
+  };
+  if (steps > 0) {
+    copy(a0, b0);
+    arrive();
+    if (steps > 1) copy(a1, b1);
+    stage(a0, b0, true);
+    int s = 1;
+    for (; s + 2 <= steps; s += 2) {
+      arrive();
+      copy(a0, b0);
+      stage(a1, b1, false);
+      arrive();
+      if (s + 2 < steps) copy(a1, b1);
+      stage(a0, b0, false);
+    }
+    if (s < steps) {
+      arrive();
+      stage(a1, b1, false);
+    }
+    products(NC - 1);
   }
   __syncthreads();  // the tiles are read: each wave takes 2 KB of their LDS for a 32 x 32 block
   constexpr int kShare = FI * FJ * 2048, kPer = TI * 128 / kShare;
