@@ -41,8 +41,10 @@ def _check(x, w, t, b, reduction, g, what, ignore=IGNORE):
     return got
 
 
-# few tokens (up to 64), tiles of 128 and of 256; widths and vocabularies on and off their multiples; one of each
-SIZES = [(1, 1, 1), (1, 2, 8), (3, 5, 64), (25, 5, 64), (64, 700, 72), (65, 130, 40), (48, 1000, 256), (130, 257, 129), (200, 129, 520), (300, 1031, 65),
+# few classes (up to 16 of 256 or 8 of 512) in one workgroup and in several, and just more of them; few tokens (up to
+# 64), tiles of 128 and of 256; widths and vocabularies on and off their multiples; one of each
+SIZES = [(1, 1, 1), (1, 2, 8), (3, 5, 64), (25, 5, 64), (64, 8, 512), (65, 8, 511), (300, 8, 513), (700, 16, 256), (90, 9, 257), (333, 13, 100),
+         (40, 17, 64), (20000, 3, 65), (5000, 16, 40), (64, 700, 72), (65, 130, 40), (48, 1000, 256), (130, 257, 129), (200, 129, 520), (300, 1031, 65),
          (129, 128, 128), (256, 512, 64), (513, 2050, 96), (1030, 64, 200)]
 
 

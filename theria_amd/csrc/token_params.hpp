@@ -75,7 +75,8 @@ struct CeParams {
   Rows x, w;
   const void *target, *bias;  // bias optional
   float* loss;                // n (kCeNone) or one
-  float* stats;               // 2 n: of the i-th kept row, the largest logit and the sum of exp(logit - largest)
+  float* stats;               // 2 n: of the i-th kept row, the largest logit and the sum of exp(logit - largest); few
+                              // classes (ce_head_takes): the number of kept rows in the first place
   const float* gout;          // backward: n (kCeNone) or one
   MutRows dx, dw;             // optional
   void* db;                   // optional
@@ -84,5 +85,9 @@ struct CeParams {
 int64_t ce_ws_bytes(const CeParams& p, bool backward);
 hipError_t launch_ce_fwd(const CeParams& p, hipStream_t st);
 hipError_t launch_ce_bwd(const CeParams& p, hipStream_t st);
+// Few classes (linear_ce_head.hip).
+bool ce_head_takes(const CeParams& p);
+int64_t ce_head_ws_bytes(const CeParams& p, bool backward);
+hipError_t launch_ce_head(const CeParams& p, bool backward, hipStream_t st);
 
 }  // namespace theria
