@@ -141,33 +141,53 @@ __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int
 }
 
 // ------------------------------------------------------------------------------------------ epilogues
-__device__ __forceinline__ float bias_at(const void* bias, int dtype, int64_t v) {
-  return dtype == 0 ? ((const float*)bias)[v] : dtype == 1 ? (float)((const _Float16*)bias)[v] : (float)((const __bf16*)bias)[v];
+// The accumulators' first values: the classes' bias (loaded while the first stage's copies are on their way), or zeros.
+template <typename T, class S>
+__device__ __forceinline__ void start_logits(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, const T* bias) {
+  typedef T quad_t __attribute__((ext_vector_type(4)));
+  const int g = (threadIdx.x >> 5) & 1;
+  const bool quads = (uintptr_t)bias % (4 * sizeof(T)) == 0;
+#pragma unroll
+  for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
+      quad_t b = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
+      if (bias) {
+        if (quads && i + 4 <= t.I) {
+          b = *reinterpret_cast<const quad_t*>(bias + i);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < t.I) b[e] = bias[i + e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int fj = 0; fj < S::FJ; ++fj) z[fi][fj][4 * q + e] = (float)b[e];
+    }
 }
 
-// z + bias in place; classes past the piece's end become -inf.
+// Classes past the piece's end become -inf.
 template <class S>
-__device__ __forceinline__ void finish_logits(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, const void* bias, int dtype, int64_t v0) {
-  const int g = (threadIdx.x >> 5) & 1;
-  if (bias || t.i0 + 32 * S::FI > t.I) {
+__device__ __forceinline__ void mask_logits(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) {
+  if (t.i0 + 32 * S::FI <= t.I) return;
+  const int room = t.I - t.i0 - 4 * (int)((threadIdx.x >> 5) & 1);
 #pragma unroll
-    for (int fi = 0; fi < S::FI; ++fi)
+  for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = t.i0 + 32 * fi + acc_row(r, g);
-        const bool in = i < t.I;
-        const float b = bias && in ? bias_at(bias, dtype, v0 + i) : 0.f;
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int fj = 0; fj < S::FJ; ++fj) z[fi][fj][r] = in ? z[fi][fj][r] + b : -THERIA_INF;
-      }
-  }
+      for (int fj = 0; fj < S::FJ; ++fj)
+        if (32 * fi + 8 * (r >> 2) + (r & 3) >= room) z[fi][fj][r] = -THERIA_INF;
 }
 
 // Forward: of each row (column j of the tile) the largest logit over the tile's classes and the sum of
 // exp(logit - largest), and the target's logit where it lies in the tile.
+template <typename T>
 struct LogitStats {
-  const void* bias;
-  int dtype;
+  const T* bias;      // of the piece's classes, or null
   int64_t v0;         // the piece's first class
   const int* target;
   float* at_target;   // one of each kept row
@@ -176,21 +196,27 @@ struct LogitStats {
   int tile0;          // the piece's first tile
 
   template <class S>
+  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    start_logits<T, S>(z, t, bias);
+  }
+  template <class S>
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char*) const {
     __shared__ float2 red[S::WI][S::TJ];
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
-    finish_logits<S>(z, t, bias, dtype, v0);
+    mask_logits<S>(z, t);
 #pragma unroll
     for (int fj = 0; fj < S::FJ; ++fj) {
       const int j = t.j0 + 32 * fj + li;
       if (j < t.J) {
         const int64_t want = (int64_t)target[j] - v0 - t.i0;
-        if (want >= 0 && want < 32 * S::FI) {
+        const int w = (int)want - 4 * g;  // the wanted one's place among this half's rows, if it is there
+        if (want >= 0 && want < 32 * S::FI && (want >> 2 & 1) == g) {
+          float at = 0.f;
 #pragma unroll
           for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (want == 32 * fi + acc_row(r, g)) at_target[j] = z[fi][fj][r];
+            for (int r = 0; r < 16; ++r) at = w == 32 * fi + 8 * (r >> 2) + (r & 3) ? z[fi][fj][r] : at;
+          at_target[j] = at;
         }
       }
       float top = -THERIA_INF;
@@ -228,10 +254,9 @@ struct LogitStats {
 };
 
 // Backward: dz of the tile, in 16 bits (three planes for float32 inputs), rows j of ld elements.
-template <int PLANES>
+template <typename T, int PLANES>
 struct LogitGrad {
-  const void* bias;
-  int dtype;
+  const T* bias;
   int64_t v0;
   const int *target, *map;
   const float* stats;  // [2][n]: largest logit, sum
@@ -243,10 +268,14 @@ struct LogitGrad {
   int64_t plane;
 
   template <class S>
+  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    start_logits<T, S>(z, t, bias);
+  }
+  template <class S>
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     using H = typename S::H;
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
-    finish_logits<S>(z, t, bias, dtype, v0);
+    mask_logits<S>(z, t);
 #pragma unroll
     for (int fj = 0; fj < S::FJ; ++fj) {
       const int j = t.j0 + 32 * fj + li;
@@ -274,7 +303,7 @@ struct LogitGrad {
       for (int fi = 0; fi < S::FI; ++fi) z[fi][fj] *= unit;
     }
     using Stage = GemmStage<S, 2>;
-    // each plane in turn: what the last ones held is taken off first
+    // one plane after another through the same LDS
 #pragma unroll 1
     for (int k = 0; k < PLANES; ++k) {
 #pragma unroll
@@ -286,10 +315,15 @@ struct LogitGrad {
             H out[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = z[fi][fj][4 * q + e];
-              out[e] = (H)v;
-              // an infinity or NaN is whole in its first plane
-              if constexpr (PLANES > 1) z[fi][fj][4 * q + e] = fabsf(v) < THERIA_INF ? v - (float)out[e] : 0.f;
+              float v = z[fi][fj][4 * q + e];
+              if constexpr (PLANES == 1) {
+                out[e] = (H)v;
+              } else {
+                __bf16 h, m, l;
+                asm volatile("" : "+v"(v));  // split anew for each plane: the three of a whole tile do not fit the registers
+                split3(v, h, m, l);
+                out[e] = k == 0 ? h : k == 1 ? m : l;
+              }
             }
             Stage::put(lds, 32 * fj + li, fi, q, g, out);
           }
@@ -307,6 +341,10 @@ struct SumTile {
   int ld;        // a multiple of 4
   bool add;
 
+  template <class S>
+  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile&) const {
+    gemm_zero<S>(z);
+  }
   template <class S>
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
@@ -340,6 +378,10 @@ struct OutTile {
   bool vec;  // 16 bytes at a time
   const Meta* meta;
 
+  template <class S>
+  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile&) const {
+    gemm_zero<S>(z);
+  }
   template <class S>
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
@@ -626,6 +668,7 @@ struct Call {
   int64_t plane_x() const { return 2 * p.n * l.kp; }
   int64_t plane_w() const { return 2 * l.piece * l.kp; }
   int64_t plane_z() const { return 2 * p.n * l.ldz; }
+  const T* piece_bias(int64_t v) const { return p.bias ? (const T*)p.bias + v : nullptr; }
   int segments() const { return l.planes ? 6 : 1; }
   GemmOperand x_operand(bool across) const {
     return {ws + l.xs, 2 * (int64_t)l.kp, plane_x(), across ? l.kp : (int)p.n};
@@ -658,7 +701,7 @@ struct Call {
       const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
       THERIA_TRY(lay_piece(v, have));
       const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, segments(), &meta->kept, true, false};
-      const LogitStats e{p.bias, p.dtype, v, target, (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
+      const LogitStats<T> e{piece_bias(v), v, target, (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
       THERIA_TRY((gemm<H, false, false>(l.tf, g, e, st)));
       tile0 += (int)(up(have, tile_i(l.tf)) / tile_i(l.tf));
     }
@@ -686,7 +729,7 @@ struct Call {
       THERIA_TRY(lay_piece(v, have));
       {
         const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, segments(), &meta->kept, true, false};
-        const LogitGrad<PLANES> e{p.bias, p.dtype, v, target, map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, ws + l.dz, l.ldz, plane_z()};
+        const LogitGrad<T, PLANES> e{piece_bias(v), v, target, map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, ws + l.dz, l.ldz, plane_z()};
         THERIA_TRY((gemm<H, false, false>(l.tf, g, e, st)));
       }
       if (p.dx.p) {

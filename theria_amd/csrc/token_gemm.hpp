@@ -170,6 +170,14 @@ struct GemmStage {
   }
 };
 
+template <class S>
+__device__ __forceinline__ void gemm_zero(f32x16_t (&z)[S::FI][S::FJ]) {
+#pragma unroll
+  for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FJ; ++j) z[i][j] = zero16();
+}
+
 template <class S, class Epi>
 __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi) {
   using H = typename S::H;
@@ -211,10 +219,6 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
   const uint32_t planes_a = p.segments == 1 ? 0u : 0x049u, planes_b = p.segments == 1 ? 0u : 0x121u;
 
   f32x16_t acc[FI][FJ];
-#pragma unroll
-  for (int i = 0; i < FI; ++i)
-#pragma unroll
-    for (int j = 0; j < FJ; ++j) acc[i][j] = zero16();
 
   int seg = 0, ks = 0;  // of the next step to copy
   auto copy = [&](char* a, char* b) {
@@ -259,8 +263,9 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
     wait_vm_all();
     __syncthreads();  // a stage is there for every wave, and every wave has read the other one
   };
+  if (steps > 0) copy(a0, b0);
+  epi.template start<S>(acc, t);
   if (steps > 0) {
-    copy(a0, b0);
     arrive();
     if (steps > 1) copy(a1, b1);
     stage(a0, b0, true);
