@@ -13,8 +13,15 @@
 // dz enters the products in the inputs' 16-bit type, as an operand of a matrix product does everywhere here: one rounding
 // of 2^-9 (bfloat16) or 2^-12 (float16) relative to each entry, under the rounding of the gradients themselves once
 // summed. It is held without the loss's own factor (1 / kept rows, or the largest |g|), which multiplies the float32 sums, and
-// in float16 times 2^14, so that probabilities down to 2^-38 do not vanish. float32 operands and dz are three bfloat16
-// planes each (token_gemm.hpp).
+// in float16 times 2^14, so that probabilities down to 2^-38 do not vanish.
+//
+// float32 operands are planes of 16-bit terms (token_gemm.hpp). For the logits two float16 terms, x = h + m to 2^-23, and three
+// products of them (m m, 2^-22 of the product at most and 2^-25 on average, is dropped): each row of x and W is first
+// scaled by the power of two that brings its largest element to 2^13, which the epilogue takes back, so that nothing
+// leaves float16's range. For the gradients, whose sums run over rows of any size, three bfloat16 terms and six products.
+// Against six products throughout: forward 1.7 times as fast, see the figures at Call.
+#include <type_traits>
+
 #include "token_common.hpp"
 #include "token_gemm.hpp"
 #include "token_params.hpp"
@@ -104,111 +111,177 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward
   }
 }
 
-// Rows laid out for the products: `width` elements, zeros up to kp; float32 in three planes. With map: the kept rows of src.
+// Eight elements of a row from column c, zeros past its end.
 template <typename T>
-__global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int width, const int* map, const Meta* meta, char* out, int kp, int64_t plane) {
+__device__ __forceinline__ void load8(T (&v)[8], const T* row, int c, int width, bool vec) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (vec && c + 8 <= width) {
+#pragma unroll
+    for (int q = 0; q < 8 / V; ++q) *reinterpret_cast<u32x4_t*>(v + q * V) = *reinterpret_cast<const u32x4_t*>(row + c + q * V);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < width ? row[c + e] : (T)0.f;
+  }
+}
+
+// Rows laid out for the products: `width` elements, zeros up to kp, a wave for a row. With map: the kept rows of src.
+// 16-bit: a copy. float32: two scaled float16 planes and the exponent of each row's scale at `logits`, and three bfloat16
+// planes at `grads` unless it is null.
+struct LayTo {
+  char *logits, *grads;
+  int* exponent;
+  int64_t plane;  // bytes from plane to plane
+  int kp;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int width, const int* map, const Meta* meta, LayTo to) {
   const int lane = threadIdx.x % 64;
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   if (i >= (map ? (int64_t)meta->kept : rows)) return;
   const T* row = (const T*)src.p + (map ? (int64_t)map[i] : i) * src.sr;
   constexpr int V = 16 / (int)sizeof(T);
   const bool vec = width % V == 0 && src.sr % V == 0 && (uintptr_t)src.p % 16 == 0;
-  for (int c = lane * 8; c < kp; c += 512) {
-    T v[8];
-    if (vec && c + 8 <= width) {
+  T v[8];
+  int scale = 0;
+  if constexpr (sizeof(T) == 4) {
+    float most = 0.f;  // of the finite elements
+    for (int c = lane * 8; c < width; c += 512) {
+      load8(v, row, c, width, vec);
 #pragma unroll
-      for (int q = 0; q < 8 / V; ++q) *reinterpret_cast<u32x4_t*>(v + q * V) = *reinterpret_cast<const u32x4_t*>(row + c + q * V);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c + e < width ? row[c + e] : (T)0.f;
+      for (int e = 0; e < 8; ++e) most = fabsf(v[e]) < THERIA_INF ? fmaxf(most, fabsf(v[e])) : most;
     }
-    char* to = out + i * kp * 2 + c * 2;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
+    int e = 0;
+    if (most > 0.f) frexpf(most, &e), scale = 14 - e;
+    if (lane == 0) to.exponent[i] = -scale;
+  }
+  for (int c = lane * 8; c < to.kp; c += 512) {
+    load8(v, row, c, width, vec);
+    const int64_t at = (i * to.kp + c) * 2;
     if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(v);
+      *reinterpret_cast<u32x4_t*>(to.logits + at) = *reinterpret_cast<const u32x4_t*>(v);
     } else {
-      bf16x8_t h, m, l;
+      f16x8_t h, m;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        __bf16 a, b, d;
-        split3(v[e], a, b, d);
-        h[e] = a, m[e] = b, l[e] = d;
+        const float x = ldexpf(v[e], scale);
+        h[e] = (_Float16)x;
+        m[e] = fabsf(x) < THERIA_INF ? (_Float16)(x - (float)h[e]) : (_Float16)0.f;
       }
-      *reinterpret_cast<bf16x8_t*>(to) = h;
-      *reinterpret_cast<bf16x8_t*>(to + plane) = m;
-      *reinterpret_cast<bf16x8_t*>(to + 2 * plane) = l;
+      *reinterpret_cast<f16x8_t*>(to.logits + at) = h;
+      *reinterpret_cast<f16x8_t*>(to.logits + to.plane + at) = m;
+      if (!to.grads) continue;
+      bf16x8_t a, b, d;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 x, y, z;
+        split3(v[e], x, y, z);
+        a[e] = x, b[e] = y, d[e] = z;
+      }
+      *reinterpret_cast<bf16x8_t*>(to.grads + at) = a;
+      *reinterpret_cast<bf16x8_t*>(to.grads + to.plane + at) = b;
+      *reinterpret_cast<bf16x8_t*>(to.grads + 2 * to.plane + at) = d;
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------ epilogues
-// The accumulators' first values: the classes' bias (loaded while the first stage's copies are on their way), or zeros.
-template <typename T, class S>
-__device__ __forceinline__ void start_logits(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, const T* bias) {
-  typedef T quad_t __attribute__((ext_vector_type(4)));
-  const int g = (threadIdx.x >> 5) & 1;
-  const bool quads = (uintptr_t)bias % (4 * sizeof(T)) == 0;
-#pragma unroll
-  for (int fi = 0; fi < S::FI; ++fi)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
-      quad_t b = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
-      if (bias) {
-        if (quads && i + 4 <= t.I) {
-          b = *reinterpret_cast<const quad_t*>(bias + i);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (i + e < t.I) b[e] = bias[i + e];
-        }
-      }
+// What the logits' two epilogues share. Classes are i of the product, rows j.
+template <typename T>
+struct LogitBase {
+  const T* bias;      // of the piece's classes, or null
+  int64_t v0;         // the piece's first class
+  const int* target;  // of the kept rows
+  const int *exponent_w, *exponent_x;  // float32 operands: of the scales of the classes' and of the rows' planes
+
+  // Four elements from i of an array of the classes, those past the end as they are in `q`.
+  template <typename Q, typename E>
+  __device__ __forceinline__ static void load4(Q& q, const E* p, int i, int I) {
+    if ((uintptr_t)p % (4 * sizeof(E)) == 0 && i + 4 <= I) {
+      q = *reinterpret_cast<const Q*>(p + i);
+    } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int fj = 0; fj < S::FJ; ++fj) z[fi][fj][4 * q + e] = (float)b[e];
+        if (i + e < I) q[e] = p[i + e];
     }
-}
+  }
 
-// Classes past the piece's end become -inf.
-template <class S>
-__device__ __forceinline__ void mask_logits(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) {
-  if (t.i0 + 32 * S::FI <= t.I) return;
-  const int room = t.I - t.i0 - 4 * (int)((threadIdx.x >> 5) & 1);
+  // The accumulators' first values: the bias (loaded while the first stage's copies are on their way), or zeros. Scaled
+  // products get their bias at the end.
+  template <class S>
+  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    typedef T quad_t __attribute__((ext_vector_type(4)));
+    if (sizeof(T) == 4 || !bias) return gemm_zero<S>(z);
+    const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
-  for (int fi = 0; fi < S::FI; ++fi)
+    for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+      for (int q = 0; q < 4; ++q) {
+        quad_t b = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
+        load4(b, bias, t.i0 + 32 * fi + 8 * q + 4 * g, t.I);
 #pragma unroll
-      for (int fj = 0; fj < S::FJ; ++fj)
-        if (32 * fi + 8 * (r >> 2) + (r & 3) >= room) z[fi][fj][r] = -THERIA_INF;
-}
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int fj = 0; fj < S::FJ; ++fj) z[fi][fj][4 * q + e] = (float)b[e];
+      }
+  }
+
+  // The logits: scales taken back and bias added where start() could not; classes past the piece's end become -inf.
+  template <class S>
+  __device__ __forceinline__ void finish(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
+    const int li = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
+    if constexpr (sizeof(T) == 4) {
+      int ex[S::FJ];
+#pragma unroll
+      for (int fj = 0; fj < S::FJ; ++fj) ex[fj] = t.j0 + 32 * fj + li < t.J ? exponent_x[t.j0 + 32 * fj + li] : 0;
+#pragma unroll
+      for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
+          i32x4_t ew = {0, 0, 0, 0};
+          f32x4_t b = {0.f, 0.f, 0.f, 0.f};
+          load4(ew, exponent_w, i, t.I);
+          if (bias) load4(b, bias, i, t.I);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int fj = 0; fj < S::FJ; ++fj) z[fi][fj][4 * q + e] = ldexpf(z[fi][fj][4 * q + e], ew[e] + ex[fj]) + b[e];
+          __builtin_amdgcn_sched_barrier(0);  // the loads of a whole tile do not fit the registers
+        }
+    }
+    if (t.i0 + 32 * S::FI <= t.I) return;
+    const int room = t.I - t.i0 - 4 * g;
+#pragma unroll
+    for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int fj = 0; fj < S::FJ; ++fj)
+          if (32 * fi + 8 * (r >> 2) + (r & 3) >= room) z[fi][fj][r] = -THERIA_INF;
+  }
+};
 
 // Forward: of each row (column j of the tile) the largest logit over the tile's classes and the sum of
 // exp(logit - largest), and the target's logit where it lies in the tile.
 template <typename T>
-struct LogitStats {
-  const T* bias;      // of the piece's classes, or null
-  int64_t v0;         // the piece's first class
-  const int* target;
+struct LogitStats : LogitBase<T> {
   float* at_target;   // one of each kept row
   float2* part;       // [tile][n]
   int64_t n;
   int tile0;          // the piece's first tile
 
   template <class S>
-  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
-    start_logits<T, S>(z, t, bias);
-  }
-  template <class S>
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char*) const {
     __shared__ float2 red[S::WI][S::TJ];
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
-    mask_logits<S>(z, t);
+    this->template finish<S>(z, t);
 #pragma unroll
     for (int fj = 0; fj < S::FJ; ++fj) {
       const int j = t.j0 + 32 * fj + li;
       if (j < t.J) {
-        const int64_t want = (int64_t)target[j] - v0 - t.i0;
+        const int64_t want = (int64_t)this->target[j] - this->v0 - t.i0;
         const int w = (int)want - 4 * g;  // the wanted one's place among this half's rows, if it is there
         if (want >= 0 && want < 32 * S::FI && (want >> 2 & 1) == g) {
           float at = 0.f;
@@ -255,10 +328,8 @@ struct LogitStats {
 
 // Backward: dz of the tile, in 16 bits (three planes for float32 inputs), rows j of ld elements.
 template <typename T, int PLANES>
-struct LogitGrad {
-  const T* bias;
-  int64_t v0;
-  const int *target, *map;
+struct LogitGrad : LogitBase<T> {
+  const int* map;
   const float* stats;  // [2][n]: largest logit, sum
   int64_t n;
   const float* gout;   // of each row (kCeNone), or null: 1
@@ -268,20 +339,16 @@ struct LogitGrad {
   int64_t plane;
 
   template <class S>
-  __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
-    start_logits<T, S>(z, t, bias);
-  }
-  template <class S>
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
-    using H = typename S::H;
+    using H = typename std::conditional<PLANES == 1, typename S::H, __bf16>::type;
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
-    mask_logits<S>(z, t);
+    this->template finish<S>(z, t);
 #pragma unroll
     for (int fj = 0; fj < S::FJ; ++fj) {
       const int j = t.j0 + 32 * fj + li;
       const bool in = j < t.J;
       const float top = in ? stats[j] : 0.f, inv = in ? 1.0f / stats[n + j] : 0.f;
-      float unit = __is_same(H, _Float16) ? 0x1p14f : 1.f;
+      float unit = __is_same(T, _Float16) ? 0x1p14f : 1.f;
       if (in && gout) {
         const float go = gout[map[j]], most = meta->most;
         // a gradient that is not finite keeps its own value: it is not in `most`
@@ -292,7 +359,7 @@ struct LogitGrad {
       for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[fi][fj][r] = fast_exp2((z[fi][fj][r] - top) * kLog2e) * inv;
-      const int64_t want = in ? (int64_t)target[j] - v0 - t.i0 : -1;
+      const int64_t want = in ? (int64_t)this->target[j] - this->v0 - t.i0 : -1;
       if (want >= 0 && want < 32 * S::FI) {
 #pragma unroll
         for (int fi = 0; fi < S::FI; ++fi)
@@ -565,7 +632,7 @@ int splits_for(int64_t I, int64_t J, int64_t K, Tile t) {
 
 // Where everything lies in the workspace.
 struct Layout {
-  bool planes;      // float32: operands in three bfloat16 planes
+  bool planes;      // float32: operands in planes of 16-bit terms
   bool lay_w;       // W is laid out anew, a piece at a time
   int kp;           // width rounded up to 64
   int64_t piece;    // classes of a piece
@@ -575,13 +642,13 @@ struct Layout {
   int ldx;          // of the float32 sums
   int tiles;        // of classes, over all pieces
   int bias_parts;
-  int64_t map, target, meta, xs, at_target, part, row_loss, ws_w, dz, sum_x, sum_w, bias_part, bytes;
+  int64_t map, target, meta, xs, xs_grad, ws_w, ws_w_grad, ex_x, ex_w, at_target, part, row_loss, dz, sum_x, sum_w, bias_part, bytes;
 };
 
 Layout layout_of(const CeParams& p, bool backward) {
   Layout l{};
   l.planes = p.dtype == 0;
-  const int np = l.planes ? 3 : 1;
+  const int np = l.planes ? 2 : 1, ng = l.planes ? 3 : 1;  // planes of an operand of the logits, of the gradients
   l.kp = (int)up(p.width, 64);
   // the copies take 16-byte pieces and 32-bit offsets inside a tile
   l.lay_w = l.planes || p.width % 8 || p.w.sr % 8 || (uintptr_t)p.w.p % 16 || p.w.sr > (1 << 21);
@@ -590,8 +657,8 @@ Layout layout_of(const CeParams& p, bool backward) {
     const int64_t most = kPieceBytes / row_bytes / 256 * 256;
     if (l.piece > most) l.piece = most < 256 ? 256 : most;
   };
-  if (l.lay_w) limit(2 * np * (int64_t)l.kp);
-  if (backward && p.n > 0) limit(2 * np * p.n);
+  if (l.lay_w) limit(2 * (np + (l.planes && backward ? ng : 0)) * (int64_t)l.kp);
+  if (backward && p.n > 0) limit(2 * ng * p.n);
   l.ldz = (int)l.piece;
   l.tf = tile_for(l.piece, p.n, p.width, true);
   l.tx = tile_for(p.width, p.n, l.piece, true);
@@ -612,27 +679,23 @@ Layout layout_of(const CeParams& p, bool backward) {
   l.target = take(4 * p.n);
   l.xs = take(2 * np * p.n * l.kp);
   if (l.lay_w) l.ws_w = take(2 * np * l.piece * l.kp);
+  if (l.planes) {
+    l.ex_x = take(4 * p.n);
+    l.ex_w = take(4 * l.piece);
+    if (backward) l.xs_grad = take(2 * ng * p.n * l.kp), l.ws_w_grad = take(2 * ng * l.piece * l.kp);
+  }
   if (!backward) {
     l.at_target = take(4 * p.n);
     l.part = take(8 * l.tiles * p.n);
     l.row_loss = take(4 * p.n);
   } else {
-    l.dz = take(2 * np * p.n * l.ldz);
+    l.dz = take(2 * ng * p.n * l.ldz);
     if (p.dx.p) l.sum_x = take(4 * l.sx * p.n * l.ldx);
     if (p.dw.p && l.sw > 1) l.sum_w = take(4 * l.sw * l.piece * l.ldx);
     if (p.db) l.bias_part = take(4 * (int64_t)l.bias_parts * l.ldz);
   }
   return l;
 }
-
-template <typename T>
-struct HalfOf {
-  using type = T;
-};
-template <>
-struct HalfOf<float> {
-  using type = __bf16;
-};
 
 template <typename H, bool A, bool B, class Epi>
 hipError_t gemm(Tile t, const GemmParams& g, const Epi& e, hipStream_t st) {
@@ -653,7 +716,9 @@ hipError_t gemm(Tile t, const GemmParams& g, const Epi& e, hipStream_t st) {
 
 template <typename T>
 struct Call {
-  using H = typename HalfOf<T>::type;
+  static constexpr bool kSplit = sizeof(T) == 4;
+  using L = typename std::conditional<kSplit, _Float16, T>::type;  // operands of the logits
+  using H = typename std::conditional<kSplit, __bf16, T>::type;    // operands of the gradients
   const CeParams& p;
   const Layout l;
   hipStream_t st;
@@ -668,29 +733,32 @@ struct Call {
   int64_t plane_x() const { return 2 * p.n * l.kp; }
   int64_t plane_w() const { return 2 * l.piece * l.kp; }
   int64_t plane_z() const { return 2 * p.n * l.ldz; }
-  const T* piece_bias(int64_t v) const { return p.bias ? (const T*)p.bias + v : nullptr; }
-  int segments() const { return l.planes ? 6 : 1; }
+  static constexpr int kLogitSegments = kSplit ? 3 : 1, kGradSegments = kSplit ? 6 : 1;
+  // Operands along k belong to the logits, but for dz; those across k to the gradients.
   GemmOperand x_operand(bool across) const {
-    return {ws + l.xs, 2 * (int64_t)l.kp, plane_x(), across ? l.kp : (int)p.n};
+    return {ws + (across && kSplit ? l.xs_grad : l.xs), 2 * (int64_t)l.kp, plane_x(), across ? l.kp : (int)p.n};
   }
   GemmOperand z_operand(bool across) const { return {ws + l.dz, 2 * (int64_t)l.ldz, plane_z(), across ? l.ldz : (int)p.n}; }
   // classes [v, v + have)
   GemmOperand w_operand(bool across, int64_t v, int have) const {
-    if (l.lay_w) return {ws + l.ws_w, 2 * (int64_t)l.kp, plane_w(), across ? l.kp : have};
+    if (l.lay_w) return {ws + (across && kSplit ? l.ws_w_grad : l.ws_w), 2 * (int64_t)l.kp, plane_w(), across ? l.kp : have};
     return {(const char*)p.w.p + v * p.w.sr * 2, 2 * p.w.sr, 0, across ? p.width : have};
+  }
+  LogitBase<T> base(int64_t v) const {
+    return {p.bias ? (const T*)p.bias + v : nullptr, v, target, (const int*)(ws + l.ex_w), (const int*)(ws + l.ex_x)};
   }
 
   hipError_t rows(bool backward) {
     ce_rows_kernel<<<1, 1024, 0, st>>>(p, backward, map, target, meta);
     THERIA_TRY(hipGetLastError());
     if (p.n == 0) return hipSuccess;
-    ce_lay_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, ws + l.xs, l.kp, plane_x());
+    ce_lay_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, LayTo{ws + l.xs, backward && kSplit ? ws + l.xs_grad : nullptr, (int*)(ws + l.ex_x), plane_x(), l.kp});
     return hipGetLastError();
   }
-  hipError_t lay_piece(int64_t v, int have) {
+  hipError_t lay_piece(bool backward, int64_t v, int have) {
     if (!l.lay_w) return hipSuccess;
     const Rows src{(const T*)p.w.p + v * p.w.sr, p.w.sr};
-    ce_lay_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, ws + l.ws_w, l.kp, plane_w());
+    ce_lay_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, LayTo{ws + l.ws_w, backward && kSplit ? ws + l.ws_w_grad : nullptr, (int*)(ws + l.ex_w), plane_w(), l.kp});
     return hipGetLastError();
   }
 
@@ -699,10 +767,10 @@ struct Call {
     int tile0 = 0;
     for (int64_t v = 0; v < p.classes && p.n > 0; v += l.piece) {
       const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
-      THERIA_TRY(lay_piece(v, have));
-      const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, segments(), &meta->kept, true, false};
-      const LogitStats<T> e{piece_bias(v), v, target, (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
-      THERIA_TRY((gemm<H, false, false>(l.tf, g, e, st)));
+      THERIA_TRY(lay_piece(false, v, have));
+      const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, kLogitSegments, &meta->kept, true, false};
+      const LogitStats<T> e{base(v), (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
+      THERIA_TRY((gemm<L, false, false>(l.tf, g, e, st)));
       tile0 += (int)(up(have, tile_i(l.tf)) / tile_i(l.tf));
     }
     float* row_loss = p.reduction == kCeNone ? p.loss : (float*)(ws + l.row_loss);
@@ -721,26 +789,26 @@ struct Call {
   }
 
   hipError_t backward() {
-    constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+    constexpr int PLANES = kSplit ? 3 : 1;
     THERIA_TRY(rows(true));
     const bool w4 = p.width % 4 == 0;
     for (int64_t v = 0; v < p.classes; v += l.piece) {
       const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
-      THERIA_TRY(lay_piece(v, have));
+      THERIA_TRY(lay_piece(true, v, have));
       {
-        const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, segments(), &meta->kept, true, false};
-        const LogitGrad<T, PLANES> e{piece_bias(v), v, target, map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, ws + l.dz, l.ldz, plane_z()};
-        THERIA_TRY((gemm<H, false, false>(l.tf, g, e, st)));
+        const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, kLogitSegments, &meta->kept, true, false};
+        const LogitGrad<T, PLANES> e{base(v), map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, ws + l.dz, l.ldz, plane_z()};
+        THERIA_TRY((gemm<L, false, false>(l.tf, g, e, st)));
       }
       if (p.dx.p) {
-        const GemmParams g{w_operand(true, v, have), z_operand(false), p.width, (int)p.n, have, l.sx, segments(), &meta->kept, true, false};
+        const GemmParams g{w_operand(true, v, have), z_operand(false), p.width, (int)p.n, have, l.sx, kGradSegments, &meta->kept, true, false};
         const SumTile e{(float*)(ws + l.sum_x), p.n, l.ldx, v > 0};
         THERIA_TRY((gemm<H, true, false>(l.tx, g, e, st)));
       }
       if (p.dw.p) {
         T* out = (T*)p.dw.p + v * p.dw.sr;
         const bool vec = w4 && p.dw.sr % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
-        const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.sw, segments(), &meta->kept, false, true};
+        const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.sw, kGradSegments, &meta->kept, false, true};
         if (l.sw == 1) {
           constexpr int V = 16 / (int)sizeof(T);
           const bool whole = p.width % V == 0 && p.dw.sr % V == 0 && (uintptr_t)out % 16 == 0;

@@ -5,8 +5,9 @@
 // owns a tile of TI x TJ results, walks k in steps of 64 and keeps two stages of both operands in LDS, filled by LDS DMA:
 // the next step's copies run while this step's products do.
 //
-// float32 operands come as three bfloat16 planes each, x = h + m + l (split3); their product is six passes over k with the
-// planes (m m, l h, h l, m h, h m, h h), the smallest first: the dropped terms are at most 2^-24 of the product.
+// float32 operands come as planes of 16-bit terms. Two each, x = h + m: three passes over k (m h, h m, h h). Three each, x = h
+// + m + l (split3): six passes (m m, l h, h l, m h, h m, h h), whose dropped terms are at most 2^-24 of the product. The
+// smallest come first.
 //
 // The accumulators have i along registers and j along lanes: lane l holds column j = l % 32 of a 32 x 32 block and four
 // consecutive i in each group of four registers, so sums over i stay inside a lane and i is written in pieces of four.
@@ -31,7 +32,7 @@ struct GemmParams {
   GemmOperand a, b;
   int I, J, K;
   int splits;       // parts of k, each a workgroup of its own
-  int segments;     // 1, or 6 for operands in three planes
+  int segments;     // 1; 3 for operands in two planes, 6 in three
   const int* kept;  // kept rows of the problem, read on the device
   bool j_kept, k_kept;  // J (and b's extent), or K, is *kept instead
 };
@@ -215,8 +216,9 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
   const int64_t astep = S::A ? kGemmK * p.a.ld : 2 * kGemmK, bstep = S::B ? kGemmK * p.b.ld : 2 * kGemmK;
   const char* abase = p.a.base + (S::A ? (int64_t)ti0 * 2 : (int64_t)ti0 * p.a.ld) + first * astep;
   const char* bbase = p.b.base + (S::B ? (int64_t)tj0 * 2 : (int64_t)tj0 * p.b.ld) + first * bstep;
-  // planes of the segments, two bits each, the first segment lowest: a = m l h m h h, b = m h l h m h
-  const uint32_t planes_a = p.segments == 1 ? 0u : 0x049u, planes_b = p.segments == 1 ? 0u : 0x121u;
+  // planes of the segments, two bits each, the first segment lowest: a = m l h m h h, b = m h l h m h; or m h h, h m h
+  const uint32_t planes_a = p.segments == 6 ? 0x049u : p.segments == 3 ? 0x01u : 0u;
+  const uint32_t planes_b = p.segments == 6 ? 0x121u : p.segments == 3 ? 0x04u : 0u;
 
   f32x16_t acc[FI][FJ];
 
