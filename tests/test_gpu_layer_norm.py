@@ -11,8 +11,8 @@ pytestmark = pytest.mark.gpu
 
 EPS = 1e-5
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
-# every team: vector and single-element access, 16 lanes to a workgroup of 1024, on and beside the borders
-SHAPES = [(1, 1), (3, 7), (5, 16), (17, 64), (1030, 64), (4, 65), (33, 128), (2, 136), (9, 256), (3, 257), (64, 512), (5, 1000),
+# every team, 8 lanes to a workgroup of 1024, on and beside the borders; whole and partly filled last vectors
+SHAPES = [(1, 1), (3, 7), (5, 16), (17, 64), (1030, 64), (4, 65), (33, 128), (37, 31), (50, 32), (6, 33), (129, 63), (2, 136), (4, 255), (9, 256), (3, 257), (64, 512), (5, 1000),
           (7, 1001), (3, 1024), (2, 2048), (700, 2048), (3, 4096), (2, 4104), (2, 5001), (2, 8192), (2, 16383), (1, 16384), (2100, 8)]
 
 

@@ -16,13 +16,10 @@ constexpr int64_t kMostClasses = int64_t(1) << 27, kMostLogits = int64_t(1) << 2
 
 const char* check_type(int dtype) { return dtype < 0 || dtype > 2 ? "dtype must be 0 (f32), 1 (f16) or 2 (bf16)" : nullptr; }
 
-// A view's fault, or null. vec: cleared when 16-byte access is not possible everywhere in it.
-const char* check_rows(const theria_rows_t* t, bool required, int64_t rows, int dtype, bool* vec) {
+// A view's fault, or null.
+const char* check_rows(const theria_rows_t* t, bool required, int64_t rows) {
   if (!t || !t->data) return required && rows > 0 ? "a required matrix is absent" : nullptr;
-  if (t->stride_row < 0) return "a matrix has a negative stride";
-  const int v = dtype == 0 ? 4 : 8;
-  if (vec && (reinterpret_cast<uintptr_t>(t->data) % 16 || t->stride_row % v)) *vec = false;
-  return nullptr;
+  return t->stride_row < 0 ? "a matrix has a negative stride" : nullptr;
 }
 
 Rows in(const theria_rows_t* t) { return t ? Rows{t->data, t->stride_row} : Rows{nullptr, 0}; }
@@ -51,7 +48,6 @@ const char* norm_from(const theria_layer_norm_problem_t* p, NormParams& n) {
   n.rows = p->rows;
   n.width = p->width;
   n.eps = p->eps;
-  n.vec = p->width % (p->dtype == 0 ? 4 : 8) == 0;
   return nullptr;
 }
 
@@ -70,7 +66,6 @@ const char* embed_from(const theria_embedding_problem_t* p, EmbedParams& e) {
   e.width = p->width;
   e.scale = p->scale;
   e.padding = p->padding;
-  e.vec = p->width % (p->dtype == 0 ? 4 : 8) == 0;
   return nullptr;
 }
 
@@ -95,8 +90,8 @@ const char* ce_from(const theria_linear_ce_problem_t* p, CeParams& c) {
 const char* ce_inputs(const theria_linear_ce_problem_t* p, CeParams& c, const theria_rows_t* x, const theria_rows_t* w, const void* bias,
                       const void* target, const float* stats, const void* ws) {
   if (const char* m = ce_from(p, c)) return m;
-  if (const char* m = check_rows(x, true, c.n, c.dtype, nullptr)) return m;
-  if (const char* m = check_rows(w, true, c.classes, c.dtype, nullptr)) return m;
+  if (const char* m = check_rows(x, true, c.n)) return m;
+  if (const char* m = check_rows(w, true, c.classes)) return m;
   if (c.n > 0 && (!target || !stats)) return "target and stats are required";
   if (!ws || reinterpret_cast<uintptr_t>(ws) % 256) return "a 256-byte-aligned workspace is required";
   c.x = in(x);
@@ -117,11 +112,10 @@ THERIA_API int theria_layer_norm_fwd(const theria_layer_norm_problem_t* p, const
                                      const theria_rows_t* y, float* mean, float* rstd, void* stream) {
   NormParams n;
   THERIA_CHECK(norm_from(p, n));
-  THERIA_CHECK(check_rows(x, true, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(y, true, n.rows, n.dtype, &n.vec));
+  THERIA_CHECK(check_rows(x, true, n.rows));
+  THERIA_CHECK(check_rows(y, true, n.rows));
   THERIA_NEED(n.rows == 0 || (mean && rstd), "mean and rstd are required");
   if (n.rows == 0) return THERIA_OK;
-  if (!aligned16(weight) || !aligned16(bias)) n.vec = false;
   n.x = in(x), n.y = out(y);
   n.weight = weight, n.bias = bias, n.mean = mean, n.rstd = rstd;
   return hip_status(launch_norm_fwd(n, (hipStream_t)stream), "theria_layer_norm_fwd");
@@ -138,12 +132,11 @@ THERIA_API int theria_layer_norm_bwd(const theria_layer_norm_problem_t* p, const
   NormParams n;
   THERIA_CHECK(norm_from(p, n));
   THERIA_NEED(n.rows > 0, "rows must be positive (no rows: the gradients are zeros)");
-  THERIA_CHECK(check_rows(x, true, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(dout, true, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(dx, false, n.rows, n.dtype, &n.vec));
+  THERIA_CHECK(check_rows(x, true, n.rows));
+  THERIA_CHECK(check_rows(dout, true, n.rows));
+  THERIA_CHECK(check_rows(dx, false, n.rows));
   THERIA_NEED(mean && rstd, "mean and rstd are required");
   THERIA_NEED(ws || !(dweight || dbias), "a workspace is required for dweight and dbias");
-  if (!aligned16(weight)) n.vec = false;
   n.x = in(x), n.dout = in(dout), n.dx = out(dx);
   n.weight = weight, n.mean = const_cast<float*>(mean), n.rstd = const_cast<float*>(rstd);
   n.dw = dweight, n.db = dbias, n.ws = ws;
@@ -158,14 +151,13 @@ THERIA_API int theria_layer_norm_bwd_bwd(const theria_layer_norm_problem_t* p, c
   NormParams n;
   THERIA_CHECK(norm_from(p, n));
   THERIA_NEED(n.rows > 0, "rows must be positive (no rows: the gradients are zeros)");
-  THERIA_CHECK(check_rows(x, true, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(dout, true, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(gdx, false, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(out_gx, false, n.rows, n.dtype, &n.vec));
-  THERIA_CHECK(check_rows(out_gdout, false, n.rows, n.dtype, &n.vec));
+  THERIA_CHECK(check_rows(x, true, n.rows));
+  THERIA_CHECK(check_rows(dout, true, n.rows));
+  THERIA_CHECK(check_rows(gdx, false, n.rows));
+  THERIA_CHECK(check_rows(out_gx, false, n.rows));
+  THERIA_CHECK(check_rows(out_gdout, false, n.rows));
   THERIA_NEED(mean && rstd, "mean and rstd are required");
   THERIA_NEED(ws || !out_gw, "a workspace is required for out_gw");
-  if (!aligned16(weight) || !aligned16(gdw) || !aligned16(gdb)) n.vec = false;
   n.x = in(x), n.dout = in(dout), n.gdx = in(gdx);
   n.weight = weight, n.gdw = gdw, n.gdb = gdb;
   n.mean = const_cast<float*>(mean), n.rstd = const_cast<float*>(rstd);
@@ -178,8 +170,8 @@ THERIA_API int theria_embedding_fwd(const theria_embedding_problem_t* p, const v
                                     int32_t zero_padding, const theria_rows_t* o, void* stream) {
   EmbedParams e;
   THERIA_CHECK(embed_from(p, e));
-  THERIA_CHECK(check_rows(table, true, e.n > 0 ? e.classes : 0, e.dtype, &e.vec));
-  THERIA_CHECK(check_rows(o, true, e.n, e.dtype, &e.vec));
+  THERIA_CHECK(check_rows(table, true, e.n > 0 ? e.classes : 0));
+  THERIA_CHECK(check_rows(o, true, e.n));
   THERIA_NEED(e.n == 0 || ids, "ids are required");
   if (e.n == 0) return THERIA_OK;
   e.ids = ids, e.table = in(table), e.out = out(o), e.zero_padding = zero_padding != 0;
@@ -195,8 +187,8 @@ THERIA_API int theria_embedding_bwd(const theria_embedding_problem_t* p, const v
                                     const theria_rows_t* dtable, void* ws, void* stream) {
   EmbedParams e;
   THERIA_CHECK(embed_from(p, e));
-  THERIA_CHECK(check_rows(dout, true, e.n, e.dtype, &e.vec));
-  THERIA_CHECK(check_rows(dtable, true, e.classes, e.dtype, &e.vec));
+  THERIA_CHECK(check_rows(dout, true, e.n));
+  THERIA_CHECK(check_rows(dtable, true, e.classes));
   THERIA_NEED(e.n == 0 || (ids && ws && aligned16(ws)), "ids and a 16-byte-aligned workspace are required");
   if (e.classes == 0) return THERIA_OK;
   e.ids = ids, e.dout = in(dout), e.out = out(dtable), e.ws = ws;
@@ -229,8 +221,8 @@ THERIA_API int theria_linear_ce_bwd(const theria_linear_ce_problem_t* p, const t
                                     const theria_rows_t* dx, const theria_rows_t* dweight, void* dbias, void* ws, void* stream) {
   CeParams c;
   THERIA_CHECK(ce_inputs(p, c, x, weight, bias, target, stats, ws));
-  THERIA_CHECK(check_rows(dx, false, c.n, c.dtype, nullptr));
-  THERIA_CHECK(check_rows(dweight, false, c.classes, c.dtype, nullptr));
+  THERIA_CHECK(check_rows(dx, false, c.n));
+  THERIA_CHECK(check_rows(dweight, false, c.classes));
   THERIA_NEED(dloss || (c.reduction == kCeNone && c.n == 0), "dloss is required");
   c.gout = dloss;
   c.dx = out(dx), c.dw = out(dweight), c.db = dbias;

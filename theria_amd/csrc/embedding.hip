@@ -47,18 +47,18 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int c = ((2 * blockIdx.y + i) * TPR + t) * VEC;
-    if (known && c < p.width) raw[i].load(row + c);
+    raw[i].load(row + c, known ? p.width - c : 0);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int c = ((2 * blockIdx.y + i) * TPR + t) * VEC;
     if (c >= p.width) continue;
     float f[VEC];
-    if (known) raw[i].get(f);
+    raw[i].get(f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = zero ? 0.f : known ? f[e] * p.scale : __builtin_nanf("");
     raw[i].set(f);
-    raw[i].store((T*)p.out.p + n * p.out.sr + c);
+    raw[i].store((T*)p.out.p + n * p.out.sr + c, p.width - c);
   }
 }
 
@@ -226,10 +226,8 @@ __device__ __forceinline__ void add_tokens(float (&acc)[VEC], const EmbedParams&
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t at = j + u * step;
-      if (at < e && c < p.width)
-        raw[u].load((const T*)p.dout.p + (int64_t)order[at] * p.dout.sr + c);
-      else
-        raw[u].zero();
+      raw[u].zero();
+      if (at < e) raw[u].load((const T*)p.dout.p + (int64_t)order[at] * p.dout.sr + c, p.width - c);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -283,7 +281,7 @@ __global__ __launch_bounds__(256) void embed_piece_kernel(EmbedParams p, const u
   if (team == 0 && c < p.width) {
     RawVec<float, VEC> out;
     out.set(acc);
-    out.store(pieces + (int64_t)blockIdx.x * p.width + c);
+    out.store(pieces + (int64_t)blockIdx.x * p.width + c, p.width - c);
   }
 }
 
@@ -309,7 +307,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const ui
     for (int k = 0; k < VEC; ++k) f[k] = acc[k] * p.scale;
     RawVec<T, VEC> out;
     out.set(f);
-    out.store((T*)p.out.p + v * p.out.sr + c);
+    out.store((T*)p.out.p + v * p.out.sr + c, p.width - c);
   };
   for (int r = team; r < have; r += TEAMS) {
     const int2 at = bound[r];
@@ -329,7 +327,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const ui
 #pragma unroll 4
         for (int q = a + team; q < b; q += TEAMS) {
           RawVec<float, VEC> raw;
-          raw.load(pieces + (int64_t)q * p.width + c);
+          raw.load(pieces + (int64_t)q * p.width + c, p.width - c);
           float f[VEC];
           raw.get(f);
 #pragma unroll
@@ -450,21 +448,13 @@ hipError_t bwd(const EmbedParams& p, hipStream_t st) {
 template <typename T, bool GRAD>
 hipError_t by_width(const EmbedParams& p, hipStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int n = p.vec ? p.width / V : p.width;
-#define THERIA_EMBED_CASE(VEC, TPR)                       \
-  if constexpr (GRAD)                                     \
-    return bwd<T, VEC, TPR == 16 ? 16 : 64>(p, st);       \
-  else                                                    \
-    return fwd<T, VEC, TPR>(p, st);
-  if (p.vec) {
-    if (n <= 16) { THERIA_EMBED_CASE(V, 16) }
-    if (n <= 128) { THERIA_EMBED_CASE(V, 64) }
-    THERIA_EMBED_CASE(V, 256)
+  const int n = (p.width + V - 1) / V;
+  if constexpr (GRAD) {
+    return n <= 16 ? bwd<T, V, 16>(p, st) : bwd<T, V, 64>(p, st);
+  } else {
+    if (n <= 16) return fwd<T, V, 16>(p, st);
+    return n <= 128 ? fwd<T, V, 64>(p, st) : fwd<T, V, 256>(p, st);
   }
-  if (n <= 16) { THERIA_EMBED_CASE(1, 16) }
-  if (n <= 128) { THERIA_EMBED_CASE(1, 64) }
-  THERIA_EMBED_CASE(1, 256)
-#undef THERIA_EMBED_CASE
 }
 
 template <bool GRAD>

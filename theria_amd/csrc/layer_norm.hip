@@ -10,7 +10,7 @@
 //                    sums over the row of products of the inputs, taken in one sweep: h enters them linearly.
 //
 // All are bound by memory: each tensor is read once and written once, a row held in registers between its sums and
-// its outputs. A row belongs to a team of 16 or 64 lanes or of a whole workgroup, by its width, so that a thread holds
+// its outputs. A row belongs to a team of 8 to 64 lanes or of a whole workgroup, by its width, so that a thread holds
 // at most 16 of its elements of each tensor. Sums over the rows (dw, db, G_w) stay in the threads' registers while a
 // workgroup walks its rows; each workgroup writes one partial row of them and a second launch adds the partial rows in
 // a fixed order (no atomics: the same bits on every run).
@@ -23,30 +23,30 @@ namespace {
 template <int TPR>
 constexpr int kBlock = TPR > 256 ? TPR : 256;
 
+// TAIL: the width is no multiple of VEC, so that a row's last vector is partly filled (a template parameter, since the
+// branch costs whole vectors too: backward of (8192, 4096) bfloat16 56 us with it, 45 us without).
+//
 // The columns that thread t of a team holds: NPT vectors of VEC, TPR vectors apart.
 template <int VEC, int TPR>
 __device__ __forceinline__ int col_of(int i, int t) {
   return (i * TPR + t) * VEC;
 }
 
-template <typename T, int VEC, int NPT, int TPR>
+template <typename T, int VEC, int NPT, int TPR, bool TAIL>
 __device__ __forceinline__ void load_row(RawVec<T, VEC> (&raw)[NPT], const T* row, int t, int width, bool live) {
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const int c = col_of<VEC, TPR>(i, t);
-    if (live && c < width)
-      raw[i].load(row + c);
-    else
-      raw[i].zero();
+    raw[i].template load<TAIL>(row + c, live ? width - c : 0);
   }
 }
 
 // VEC parameters from column c, or the given constant where the parameter is absent.
-template <typename WT, int VEC>
-__device__ __forceinline__ void load_param(float (&f)[VEC], const void* p, int c, float absent) {
+template <typename WT, int VEC, bool TAIL>
+__device__ __forceinline__ void load_param(float (&f)[VEC], const void* p, int c, int width, float absent) {
   if (p) {
     RawVec<WT, VEC> r;
-    r.load((const WT*)p + c);
+    r.template load<TAIL>((const WT*)p + c, width - c);
     r.get(f);
   } else {
 #pragma unroll
@@ -54,7 +54,7 @@ __device__ __forceinline__ void load_param(float (&f)[VEC], const void* p, int c
   }
 }
 
-template <typename T, typename WT, int VEC, int NPT, int TPR>
+template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
   constexpr int TEAMS = kBlock<TPR> / TPR;
   __shared__ float red[2][16];
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
   const int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
   const bool live = row < p.rows;
   RawVec<T, VEC> raw[NPT];
-  load_row<T, VEC, NPT, TPR>(raw, (const T*)p.x.p + row * p.x.sr, t, p.width, live);
+  load_row<T, VEC, NPT, TPR, TAIL>(raw, (const T*)p.x.p + row * p.x.sr, t, p.width, live);
   float x[NPT][VEC];
   float s[1] = {0.f};
 #pragma unroll
@@ -77,11 +77,11 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
   float q[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
-    const bool in = col_of<VEC, TPR>(i, t) < p.width;
+    const int have = p.width - col_of<VEC, TPR>(i, t);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       x[i][e] -= mean;
-      q[0] += in ? x[i][e] * x[i][e] : 0.f;
+      q[0] += e * TAIL < have ? x[i][e] * x[i][e] : 0.f;
     }
   }
   team_sum<TPR, 1>(q, red[1]);
@@ -92,13 +92,13 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
     const int c = col_of<VEC, TPR>(i, t);
     if (c >= p.width) continue;
     float w[VEC], b[VEC];
-    load_param<WT, VEC>(w, p.weight, c, 1.f);
-    load_param<WT, VEC>(b, p.bias, c, 0.f);
+    load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
+    load_param<WT, VEC, TAIL>(b, p.bias, c, p.width, 0.f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) x[i][e] = x[i][e] * rstd * w[e] + b[e];
     RawVec<T, VEC> out;
     out.set(x[i]);
-    out.store((T*)p.y.p + row * p.y.sr + c);
+    out.template store<TAIL>((T*)p.y.p + row * p.y.sr + c, p.width - c);
   }
   if (t == 0) {
     p.mean[row] = mean;
@@ -111,11 +111,11 @@ template <int VEC, int NPT, int TPR>
 __device__ __forceinline__ void write_partial(float (&acc)[NPT][VEC], float* out, int width, float* lds) {
   constexpr int COLS = VEC * NPT * TPR, WAVES = 4;
   const int t = threadIdx.x % TPR, wave = threadIdx.x / 64;
-  if constexpr (TPR == 16) {
+  if constexpr (TPR < 64) {
 #pragma unroll
     for (int i = 0; i < NPT; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[i][e] = group16_sum(acc[i][e]);
+      for (int e = 0; e < VEC; ++e) acc[i][e] = across_groups<TPR>(acc[i][e]);
   }
   if constexpr (TPR <= 64) {
     __syncthreads();
@@ -136,10 +136,9 @@ __device__ __forceinline__ void write_partial(float (&acc)[NPT][VEC], float* out
 #pragma unroll
     for (int i = 0; i < NPT; ++i) {
       const int c = col_of<VEC, TPR>(i, t);
-      if (c < width) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) out[c + e] = acc[i][e];
-      }
+      for (int e = 0; e < VEC; ++e)
+        if (c + e < width) out[c + e] = acc[i][e];
     }
   }
 }
@@ -147,7 +146,7 @@ __device__ __forceinline__ void write_partial(float (&acc)[NPT][VEC], float* out
 template <int VEC, int NPT, int TPR>
 constexpr int kPartialLds = TPR <= 64 ? 4 * VEC * NPT * TPR : 1;
 
-template <typename T, typename WT, int VEC, int NPT, int TPR>
+template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   constexpr int TEAMS = kBlock<TPR> / TPR;
   __shared__ float red[2][2 * 16];
@@ -164,10 +163,11 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   const int64_t step = (int64_t)gridDim.x * TEAMS;
   int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
   RawVec<T, VEC> rx[NPT], rg[NPT];
-  load_row<T, VEC, NPT, TPR>(rx, (const T*)p.x.p + row * p.x.sr, t, width, row < p.rows);
-  load_row<T, VEC, NPT, TPR>(rg, (const T*)p.dout.p + row * p.dout.sr, t, width, row < p.rows);
+  load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + row * p.x.sr, t, width, row < p.rows);
+  load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + row * p.dout.sr, t, width, row < p.rows);
   int turn = 0;
   // teams of a wave leave the loop apart; a workgroup-wide team leaves it as one (its row is the workgroup's)
+#pragma unroll 1
   while (row < p.rows) {
     float x[NPT][VEC], g[NPT][VEC];
 #pragma unroll
@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
     }
     // the next row's loads go out before this row's sums
     const int64_t next = row + step;
-    load_row<T, VEC, NPT, TPR>(rx, (const T*)p.x.p + next * p.x.sr, t, width, next < p.rows);
-    load_row<T, VEC, NPT, TPR>(rg, (const T*)p.dout.p + next * p.dout.sr, t, width, next < p.rows);
+    load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + next * p.x.sr, t, width, next < p.rows);
+    load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + next * p.dout.sr, t, width, next < p.rows);
     const float mean = p.mean[row], rstd = p.rstd[row];
     float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
       const int c = col_of<VEC, TPR>(i, t);
       if (c < width) {
         float w[VEC];
-        load_param<WT, VEC>(w, p.weight, c, 1.f);
+        load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[i][e] = (x[i][e] - mean) * rstd;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
           for (int e = 0; e < VEC; ++e) g[i][e] = rstd * (g[i][e] - m1 - x[i][e] * m2);
           RawVec<T, VEC> out;
           out.set(g[i]);
-          out.store((T*)p.dx.p + row * p.dx.sr + c);
+          out.template store<TAIL>((T*)p.dx.p + row * p.dx.sr + c, width - c);
         }
       }
     }
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   write_partial<VEC, NPT, TPR>(db, part + width, width, lds);
 }
 
-template <typename T, typename WT, int VEC, int NPT, int TPR>
+template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p) {
   constexpr int TEAMS = kBlock<TPR> / TPR;
   __shared__ float red[2][7 * 16];
@@ -236,11 +236,12 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
     for (int e = 0; e < VEC; ++e) gw_sum[i][e] = 0.f;
 
   int turn = 0;
+#pragma unroll 1
   for (int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * TEAMS) {
     RawVec<T, VEC> rx[NPT], rg[NPT], ru[NPT];
-    load_row<T, VEC, NPT, TPR>(rx, (const T*)p.x.p + row * p.x.sr, t, width, true);
-    load_row<T, VEC, NPT, TPR>(rg, (const T*)p.dout.p + row * p.dout.sr, t, width, true);
-    load_row<T, VEC, NPT, TPR>(ru, (const T*)p.gdx.p + row * p.gdx.sr, t, width, p.gdx.p != nullptr);
+    load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + row * p.x.sr, t, width, true);
+    load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + row * p.dout.sr, t, width, true);
+    load_row<T, VEC, NPT, TPR, TAIL>(ru, (const T*)p.gdx.p + row * p.gdx.sr, t, width, p.gdx.p != nullptr);
     const float mean = p.mean[row], rstd = p.rstd[row];
     float x[NPT][VEC], g[NPT][VEC], u[NPT][VEC];
     // sums over the row: gw, gw xh, u, u xh, u gw, a dout, a dout xh
@@ -253,8 +254,8 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
       ru[i].get(u[i]);
       if (c < width) {
         float w[VEC], a[VEC];
-        load_param<WT, VEC>(w, p.weight, c, 1.f);
-        load_param<WT, VEC>(a, p.gdw, c, 0.f);
+        load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
+        load_param<WT, VEC, TAIL>(a, p.gdw, c, p.width, 0.f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[i][e] = (x[i][e] - mean) * rstd;
@@ -281,9 +282,9 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
       const int c = col_of<VEC, TPR>(i, t);
       if (c >= width) continue;
       float w[VEC], a[VEC], b[VEC];
-      load_param<WT, VEC>(w, p.weight, c, 1.f);
-      load_param<WT, VEC>(a, p.gdw, c, 0.f);
-      load_param<WT, VEC>(b, p.gdb, c, 0.f);
+      load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
+      load_param<WT, VEC, TAIL>(a, p.gdw, c, p.width, 0.f);
+      load_param<WT, VEC, TAIL>(b, p.gdb, c, p.width, 0.f);
       float gx[VEC], gg[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -296,43 +297,49 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
       RawVec<T, VEC> out;
       if (p.out_gx.p) {
         out.set(gx);
-        out.store((T*)p.out_gx.p + row * p.out_gx.sr + c);
+        out.template store<TAIL>((T*)p.out_gx.p + row * p.out_gx.sr + c, width - c);
       }
       if (p.out_gdout.p) {
         out.set(gg);
-        out.store((T*)p.out_gdout.p + row * p.out_gdout.sr + c);
+        out.template store<TAIL>((T*)p.out_gdout.p + row * p.out_gdout.sr + c, width - c);
       }
     }
   }
   if (p.out_gw) write_partial<VEC, NPT, TPR>(gw_sum, p.ws + (int64_t)blockIdx.x * width, width, lds);
 }
 
-// Workgroups of a launch that sums over the rows: two for each CU walk the rows (more would write more partial rows than
-// they hide latency), fewer where a team would get fewer than two rows.
-int walkers(int64_t rows, int teams) {
-  const int64_t most = 2 * (int64_t)device_cu_count();
-  const int64_t want = (rows + 2 * teams - 1) / (2 * teams);
+// Teams by width, in vectors of 16 bytes: at most 16 elements of a tensor for each thread.
+struct Plan {
+  int npt, tpr;
+};
+Plan plan_of(const NormParams& p) {
+  const int vec = p.dtype == 0 ? 4 : 8, n = (p.width + vec - 1) / vec;
+  if (n <= 64) return {1, n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64};
+  if (n <= 128) return {2, 64};
+  if (vec == 4) return n <= 256 ? Plan{4, 64} : n <= 512 ? Plan{2, 256} : n <= 1024 ? Plan{4, 256} : n <= 2048 ? Plan{2, 1024} : Plan{4, 1024};
+  return n <= 256 ? Plan{1, 256} : n <= 512 ? Plan{2, 256} : n <= 1024 ? Plan{1, 1024} : Plan{2, 1024};
+}
+
+// Teams of a workgroup.
+int teams_of(const Plan& pl) { return pl.tpr >= 256 ? 1 : 256 / pl.tpr; }
+
+// Workgroups of a launch that sums over the rows. More hide more latency and write more partial rows, eight bytes of traffic
+// a column each: two a CU while those are over a fourteenth of the rows' own bytes, up to four (16-bit) or three. Teams of
+// 1024 threads, one a CU. Backward in us with 1, 2, 3, 4, 6 a CU: (8192, 4096) bfloat16 69, 53, 56, 60, 74; (65536, 2048)
+// bfloat16 371, 214, 175, 169, 168, float32 399, 302, 303, 310, 318; (400000, 64) float32 102, 62, 56, 57, 62; (4096, 16384)
+// bfloat16 109, 131, 159, 188, 244. Fewer where a team would get fewer than two rows.
+int walkers(const NormParams& p, const Plan& pl) {
+  const int64_t cus = device_cu_count(), two = 2 * teams_of(pl), want = (p.rows + two - 1) / two;
+  int64_t most = cus;
+  if (pl.tpr < 1024) {
+    const int64_t few = 2 * cus, many = (p.dtype == 0 ? pl.tpr == 256 ? 2 : 3 : 4) * cus, cheap = p.rows * (p.dtype == 0 ? 4 : 2) / 76;
+    most = cheap < few ? few : cheap < many ? cheap : many;
+  }
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-// Teams by width: vectors of 16 bytes where every view allows them, else single elements; at most 16 elements of a
-// tensor for each thread.
-struct Plan {
-  int vec, npt, tpr;
-};
-Plan plan_of(const NormParams& p) {
-  const int vec = p.vec ? (p.dtype == 0 ? 4 : 8) : 1, n = p.width / vec;
-  if (n <= 16) return {vec, 1, 16};
-  if (n <= 64) return {vec, 1, 64};
-  if (vec == 1) return n <= 256 ? Plan{1, 4, 64} : n <= 1024 ? Plan{1, 16, 64} : n <= 4096 ? Plan{1, 16, 256} : Plan{1, 16, 1024};
-  if (n <= 128) return {vec, 2, 64};
-  if (vec == 4) return n <= 256 ? Plan{4, 4, 64} : n <= 512 ? Plan{4, 2, 256} : n <= 1024 ? Plan{4, 4, 256} : n <= 2048 ? Plan{4, 2, 1024} : Plan{4, 4, 1024};
-  return n <= 256 ? Plan{8, 1, 256} : n <= 512 ? Plan{8, 2, 256} : n <= 1024 ? Plan{8, 1, 1024} : Plan{8, 2, 1024};
-}
-int teams_of(const Plan& pl) { return pl.tpr >= 256 ? 1 : 256 / pl.tpr; }
-
 struct Fwd {
-  template <typename T, typename WT, int VEC, int NPT, int TPR>
+  template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
   static hipError_t run(const NormParams& p, hipStream_t st) {
     constexpr int TEAMS = kBlock<TPR> / TPR;
     constexpr int64_t most = int64_t(1) << 21;  // rows: a launch holds fewer than 2^32 threads
@@ -342,7 +349,7 @@ struct Fwd {
       q.x.p = (const T*)p.x.p + r * p.x.sr;
       q.y.p = (T*)p.y.p + r * p.y.sr;
       q.mean = p.mean + r, q.rstd = p.rstd + r;
-      norm_fwd_kernel<T, WT, VEC, NPT, TPR><<<dim3((unsigned)((q.rows + TEAMS - 1) / TEAMS)), kBlock<TPR>, 0, st>>>(q);
+      norm_fwd_kernel<T, WT, VEC, NPT, TPR, TAIL><<<dim3((unsigned)((q.rows + TEAMS - 1) / TEAMS)), kBlock<TPR>, 0, st>>>(q);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
@@ -357,10 +364,10 @@ hipError_t finish(const NormParams& p, int parts, int64_t cols, void* out0, void
 }
 
 struct Bwd {
-  template <typename T, typename WT, int VEC, int NPT, int TPR>
+  template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
   static hipError_t run(const NormParams& p, hipStream_t st) {
-    const int n = walkers(p.rows, kBlock<TPR> / TPR);
-    norm_bwd_kernel<T, WT, VEC, NPT, TPR><<<n, kBlock<TPR>, 0, st>>>(p);
+    const int n = walkers(p, Plan{NPT, TPR});
+    norm_bwd_kernel<T, WT, VEC, NPT, TPR, TAIL><<<n, kBlock<TPR>, 0, st>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !(p.dw || p.db)) return e;
     return finish<WT>(p, n, 2 * (int64_t)p.width, p.dw, p.db, st);
@@ -368,10 +375,10 @@ struct Bwd {
 };
 
 struct BwdBwd {
-  template <typename T, typename WT, int VEC, int NPT, int TPR>
+  template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
   static hipError_t run(const NormParams& p, hipStream_t st) {
-    const int n = walkers(p.rows, kBlock<TPR> / TPR);
-    norm_bwd_bwd_kernel<T, WT, VEC, NPT, TPR><<<n, kBlock<TPR>, 0, st>>>(p);
+    const int n = walkers(p, Plan{NPT, TPR});
+    norm_bwd_bwd_kernel<T, WT, VEC, NPT, TPR, TAIL><<<n, kBlock<TPR>, 0, st>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.out_gw) return e;
     return finish<WT>(p, n, p.width, p.out_gw, nullptr, st);
@@ -382,26 +389,23 @@ template <typename L, typename T, typename WT>
 hipError_t by_plan(const NormParams& p, hipStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const Plan pl = plan_of(p);
-#define THERIA_NORM_CASE(VEC, NPT, TPR) \
-  if (pl.vec == VEC && pl.npt == NPT && pl.tpr == TPR) return L::template run<T, WT, VEC, NPT, TPR>(p, st);
-  THERIA_NORM_CASE(1, 1, 16)
-  THERIA_NORM_CASE(1, 1, 64)
-  THERIA_NORM_CASE(1, 4, 64)
-  THERIA_NORM_CASE(1, 16, 64)
-  THERIA_NORM_CASE(1, 16, 256)
-  THERIA_NORM_CASE(1, 16, 1024)
-  THERIA_NORM_CASE(V, 1, 16)
-  THERIA_NORM_CASE(V, 1, 64)
-  THERIA_NORM_CASE(V, 2, 64)
-  THERIA_NORM_CASE(V, 2, 256)
-  THERIA_NORM_CASE(V, 2, 1024)
+#define THERIA_NORM_CASE(NPT, TPR)               \
+  if (pl.npt == NPT && pl.tpr == TPR)            \
+    return p.width % V ? L::template run<T, WT, V, NPT, TPR, true>(p, st) : L::template run<T, WT, V, NPT, TPR, false>(p, st);
+  THERIA_NORM_CASE(1, 8)
+  THERIA_NORM_CASE(1, 16)
+  THERIA_NORM_CASE(1, 32)
+  THERIA_NORM_CASE(1, 64)
+  THERIA_NORM_CASE(2, 64)
+  THERIA_NORM_CASE(2, 256)
+  THERIA_NORM_CASE(2, 1024)
   if constexpr (V == 4) {
-    THERIA_NORM_CASE(4, 4, 64)
-    THERIA_NORM_CASE(4, 4, 256)
-    THERIA_NORM_CASE(4, 4, 1024)
+    THERIA_NORM_CASE(4, 64)
+    THERIA_NORM_CASE(4, 256)
+    THERIA_NORM_CASE(4, 1024)
   } else {
-    THERIA_NORM_CASE(8, 1, 256)
-    THERIA_NORM_CASE(8, 1, 1024)
+    THERIA_NORM_CASE(1, 256)
+    THERIA_NORM_CASE(1, 1024)
   }
 #undef THERIA_NORM_CASE
   return hipErrorInvalidValue;
@@ -417,8 +421,7 @@ hipError_t by_type(const NormParams& p, hipStream_t st) {
 }  // namespace
 
 int64_t norm_ws_floats(const NormParams& p) {
-  // at most as many workgroups as single-row teams would give: the plan depends on the views' alignment
-  return p.rows > 0 ? (int64_t)walkers(p.rows, 1) * 2 * p.width : 0;
+  return p.rows > 0 ? (int64_t)walkers(p, plan_of(p)) * 2 * p.width : 0;
 }
 hipError_t launch_norm_fwd(const NormParams& p, hipStream_t st) { return by_type<Fwd>(p, st); }
 hipError_t launch_norm_bwd(const NormParams& p, hipStream_t st) { return by_type<Bwd>(p, st); }

@@ -113,19 +113,6 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward
   }
 }
 
-// Eight elements of a row from column c, zeros past its end.
-template <typename T>
-__device__ __forceinline__ void load8(T (&v)[8], const T* row, int c, int width, bool vec) {
-  constexpr int V = 16 / (int)sizeof(T);
-  if (vec && c + 8 <= width) {
-#pragma unroll
-    for (int q = 0; q < 8 / V; ++q) *reinterpret_cast<u32x4_t*>(v + q * V) = *reinterpret_cast<const u32x4_t*>(row + c + q * V);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < width ? row[c + e] : (T)0.f;
-  }
-}
-
 // Rows laid out for the products: `width` elements, zeros up to kp, a wave for a row. With map: the kept rows of src.
 // 16-bit: a copy. float32: two scaled float16 planes and the exponent of each row's scale at `logits`, and three bfloat16
 // planes at `grads` unless it is null.
@@ -141,14 +128,14 @@ __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   if (i >= (map ? (int64_t)meta->kept : rows)) return;
   const T* row = (const T*)src.p + (map ? (int64_t)map[i] : i) * src.sr;
-  constexpr int V = 16 / (int)sizeof(T);
-  const bool vec = width % V == 0 && src.sr % V == 0 && (uintptr_t)src.p % 16 == 0;
-  T v[8];
+  RawVec<T, 8> raw;
   int scale = 0;
   if constexpr (sizeof(T) == 4) {
     float most = 0.f;  // of the finite elements
     for (int c = lane * 8; c < width; c += 512) {
-      load8(v, row, c, width, vec);
+      float v[8];
+      raw.load(row + c, width - c);
+      raw.get(v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fabsf(v[e]) < THERIA_INF ? fmaxf(most, fabsf(v[e])) : most;
     }
@@ -159,11 +146,13 @@ __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int
     if (lane == 0) to.exponent[i] = -scale;
   }
   for (int c = lane * 8; c < to.kp; c += 512) {
-    load8(v, row, c, width, vec);
+    raw.load(row + c, width - c);
     const int64_t at = (i * to.kp + c) * 2;
     if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<u32x4_t*>(to.logits + at) = *reinterpret_cast<const u32x4_t*>(v);
+      *reinterpret_cast<u32x4_t*>(to.logits + at) = raw.v[0];
     } else {
+      float v[8];
+      raw.get(v);
       f16x8_t h, m;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -415,7 +404,7 @@ struct LogitGrad : LogitBase<T> {
 struct SumTile {
   float* sums;
   int64_t rows;  // of a split
-  int ld;        // a multiple of 4
+  int ld;        // a multiple of 8
   bool add;
 
   template <class S>
@@ -452,7 +441,6 @@ template <typename T>
 struct OutTile {
   T* out;
   int64_t sr;
-  bool vec;  // 16 bytes at a time
   const Meta* meta;
 
   template <class S>
@@ -483,14 +471,9 @@ struct OutTile {
       Stage::each(lds, 32 * kBlocks, [&](int r, int i, const i32x4_t& c) {
         if (j0 + r >= t.J || t.i0 + i >= t.I) return;
         T* to = out + (j0 + r) * sr + t.i0 + i;
-        if (vec) {
-          *reinterpret_cast<i32x4_t*>(to) = c;
-        } else {
-          const T* v = reinterpret_cast<const T*>(&c);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e)
-            if (t.i0 + i + e < t.I) to[e] = v[e];
-        }
+        RawVec<T, kPer> v;
+        __builtin_memcpy(v.v, &c, 16);
+        v.store(to, t.I - t.i0 - i);
       });
     }
   }
@@ -557,7 +540,7 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(CeParams p, const float*
 // be added with the target's row of w.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_join_rows_kernel(const float* sums, int splits, int64_t rows, int ld, int width, const int* map,
-                                                           const Meta* meta, T* out, int64_t sr, bool vec, const float* rest,
+                                                           const Meta* meta, T* out, int64_t sr, const float* rest,
                                                            const int* target, Rows w) {
   const int lane = threadIdx.x % 64;
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
@@ -574,30 +557,29 @@ __global__ __launch_bounds__(256) void ce_join_rows_kernel(const float* sums, in
   const float f = meta->factor;
   const float left = rest && have ? rest[i] : 0.f;
   const T* row_w = left != 0.f ? (const T*)w.p + target[i] * w.sr : nullptr;
-  for (int c = lane * 4; c < width; c += 256) {
-    f32x4_t v = {fill, fill, fill, fill};
+  for (int c = lane * 8; c < width; c += 512) {
+    float v[8];
+    RawVec<T, 8> o;
     if (have) {
-      v = *reinterpret_cast<const f32x4_t*>(sums + i * ld + c);
-      for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
-      if (row_w) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < width) v[e] += left * (float)row_w[c + e];
+      f32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;  // ld is a multiple of 8
+      for (int s = 0; s < splits; ++s) {
+        const f32x4_t* from = reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
+        a += from[0], b += from[1];
       }
-      v *= f;
-    }
-    T o[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-    T* to = out + row * sr + c;
-    if (vec) {
-      if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(o);
-      else
-        *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(o);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < width) to[e] = o[e];
+      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+      if (row_w) {
+        float w8[8];
+        o.load(row_w + c, width - c);
+        o.get(w8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += left * w8[e];
+      }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = have ? v[e] * f : fill;
+    o.set(v);
+    o.store(out + row * sr + c, width - c);
   }
 }
 
@@ -684,7 +666,7 @@ Layout layout_of(const CeParams& p, bool backward) {
   l.tw = tile_for(p.width, l.piece, p.n, false);
   l.sx = splits_for(p.width, p.n, l.piece, l.tx);
   l.sw = splits_for(p.width, l.piece, p.n, l.tw);
-  l.ldx = (int)up(p.width, 4);
+  l.ldx = (int)up(p.width, 8);
   l.bias_parts = (int)(p.n < 64 ? 1 : p.n / 64 < 64 ? p.n / 64 : 64);
   for (int64_t v = 0; v < p.classes; v += l.piece)
     l.tiles += (int)(up(p.classes - v < l.piece ? p.classes - v : l.piece, tile_i(l.tf)) / tile_i(l.tf));
@@ -811,7 +793,6 @@ struct Call {
   hipError_t backward() {
     constexpr int PLANES = kSplit ? 3 : 1;
     THERIA_TRY(rows(true));
-    const bool w4 = p.width % 4 == 0;
     for (int64_t v = 0; v < p.classes; v += l.piece) {
       const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
       THERIA_TRY(lay_piece(true, v, have));
@@ -827,16 +808,13 @@ struct Call {
       }
       if (p.dw.p) {
         T* out = (T*)p.dw.p + v * p.dw.sr;
-        const bool vec = w4 && p.dw.sr % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
         const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.sw, kGradSegments, &meta->kept, false, true};
         if (l.sw == 1) {
-          constexpr int V = 16 / (int)sizeof(T);
-          const bool whole = p.width % V == 0 && p.dw.sr % V == 0 && (uintptr_t)out % 16 == 0;
-          THERIA_TRY((gemm<H, true, true>(l.tw, g, OutTile<T>{out, p.dw.sr, whole, meta}, st)));
+          THERIA_TRY((gemm<H, true, true>(l.tw, g, OutTile<T>{out, p.dw.sr, meta}, st)));
         } else {
           float* sums = (float*)(ws + l.sum_w);
           THERIA_TRY((gemm<H, true, true>(l.tw, g, SumTile{sums, l.piece, l.ldx, false}, st)));
-          ce_join_rows_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(sums, l.sw, l.piece, l.ldx, p.width, nullptr, meta, out, p.dw.sr, vec, nullptr, nullptr, Rows{});
+          ce_join_rows_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(sums, l.sw, l.piece, l.ldx, p.width, nullptr, meta, out, p.dw.sr, nullptr, nullptr, Rows{});
           THERIA_TRY(hipGetLastError());
         }
       }
@@ -849,8 +827,7 @@ struct Call {
       }
     }
     if (p.dx.p && p.n > 0) {
-      const bool vec = w4 && p.dx.sr % 4 == 0 && (uintptr_t)p.dx.p % (4 * sizeof(T)) == 0;
-      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>((const float*)(ws + l.sum_x), l.sx, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, vec, kSplit ? nullptr : (const float*)(ws + l.rest), target, p.w);
+      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>((const float*)(ws + l.sum_x), l.sx, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, kSplit ? nullptr : (const float*)(ws + l.rest), target, p.w);
       THERIA_TRY(hipGetLastError());
     }
     return hipSuccess;

@@ -29,7 +29,6 @@ struct NormParams {
   int64_t rows;
   int width;
   float eps;
-  bool vec;  // every view allows 16-byte access
   Rows x, dout, gdx;
   const void *weight, *bias;   // optional
   const void *gdw, *gdb;       // double backward: cotangents of dweight and dbias, optional
@@ -47,7 +46,6 @@ hipError_t launch_norm_bwd_bwd(const NormParams& p, hipStream_t st);
 struct EmbedParams {
   int dtype;
   bool ids64;
-  bool vec;
   bool zero_padding;  // lookup: rows of the padding id are zeros (the gradient's own lookup)
   int64_t n, classes;
   int width;
