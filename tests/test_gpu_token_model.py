@@ -89,3 +89,80 @@ def test_one_attention_layer_in_bfloat16_end_to_end(hip_device):
         for a, b in zip(out, eager):
             assert torch.equal(a, b), f"replay {i}"
         step()
+
+
+def _calls(dev):
+    x, w = torch.randn(6, 16, device=dev), torch.randn(9, 16, device=dev)
+    ids = torch.arange(6, device=dev)
+    return x, w, [lambda x, w: hip_layer_norm(x, w[0]).sum(), lambda x, w: hip_embedding(ids, w).sum(), lambda x, w: hip_linear_cross_entropy(x, w, ids)]
+
+
+def test_transforms_and_forward_mode_are_refused(hip_device):
+    """Neither gives a wrong result: both raise."""
+    import torch.autograd.forward_ad as fwAD
+
+    x, w, calls = _calls(hip_device)
+    for call in calls:
+        with pytest.raises(AssertionError, match="torch.func"):
+            torch.func.grad(lambda w: call(x, w))(w)
+        with pytest.raises(AssertionError, match="torch.func"):
+            torch.func.vmap(lambda w: call(x, w))(w.expand(2, 9, 16).contiguous())
+        with fwAD.dual_level(), pytest.raises(RuntimeError):
+            fwAD.unpack_dual(call(x, fwAD.make_dual(w, torch.ones_like(w)))).tangent.sum()
+
+
+def test_inputs_changed_after_the_forward_are_noticed(hip_device):
+    x, w, calls = _calls(hip_device)
+    for call, changed in zip(calls[:1] + calls[2:], (x, w)):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        a, b = xl * 1, wl * 1
+        loss = call(a, b)
+        (a if changed is x else b).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_accumulated_gradients_and_checkpointing(hip_device):
+    """backward() into .grad twice, with a tied table and head, directly and recomputed by torch's checkpointing."""
+    from torch.utils.checkpoint import checkpoint
+
+    gen = torch.Generator().manual_seed(5)
+    table = torch.randn(50, 32, generator=gen).to(hip_device).requires_grad_(True)
+    ids, t = torch.randint(0, 50, (70,), generator=gen).to(hip_device), torch.randint(0, 50, (70,), generator=gen).to(hip_device)
+    body = lambda: hip_linear_cross_entropy(hip_layer_norm(hip_embedding(ids, table)), table, t)  # noqa: E731
+    body().backward()
+    once = table.grad.clone()
+    body().backward()
+    assert torch.equal(table.grad, 2 * once)
+    table.grad = None
+    checkpoint(lambda _: body(), torch.zeros(1, device=hip_device, requires_grad=True), use_reentrant=False).backward()
+    assert torch.equal(table.grad, once)
+
+
+def test_a_thread_of_its_own(hip_device):
+    """Calls and their backward passes from two Python threads at once, on streams of their own."""
+    import threading
+
+    x, w, calls = _calls(hip_device)
+    want = []
+    for call in calls:
+        wl = w.clone().requires_grad_(True)
+        want.append(torch.autograd.grad(call(x, wl), wl)[0])
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                for call, ref in zip(calls, want):
+                    wl = w.clone().requires_grad_(True)
+                    if not torch.equal(torch.autograd.grad(call(x, wl), wl)[0], ref):
+                        wrong.append(call)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong

@@ -301,11 +301,14 @@ std::string shape_text(const Tensor& t) {
   return s + (t.dim() == 1 ? ",)" : ")");
 }
 
+// A torch.func transform wraps its tensors; the C++ Functions know nothing of that.
+void check_plain(const Tensor& t, const char* what) { must(t.has_storage(), std::string(what) + " does not run under torch.func transforms"); }
+
 // Device, dtype and size contract of the operators' matrices.
 void check_matrix(const Tensor& t, const char* name, const char* what) {
   must(t.defined(), std::string(what) + ": " + name + " must be a tensor");
   must(t.is_cuda(), std::string(what) + " requires GPU (HIP) tensors; " + name + " is on " + t.device().str());
-  must(t.has_storage(), std::string(what) + " does not run under torch.func transforms");
+  check_plain(t, what);
   const auto st = t.scalar_type();
   must(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, std::string("Unsupported dtype for ") + name + ": " + c10::toString(st));
   must(t.dim() == 0 || t.size(-1) == 0 || t.numel() / t.size(-1) <= kMaxRows, std::string(what) + ": " + name + " has more rows than 32-bit indexes reach");
@@ -314,7 +317,7 @@ void check_matrix(const Tensor& t, const char* name, const char* what) {
 void check_indexes(const Tensor& t, const char* name, const Tensor& like, const char* what) {
   must(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, std::string(what) + ": " + name + " must be an int32 or int64 tensor");
   must(t.device() == like.device(), std::string(what) + ": " + name + " must be on " + like.device().str() + ", got " + t.device().str());
-  must(t.has_storage(), std::string(what) + " does not run under torch.func transforms");
+  check_plain(t, what);
   must(t.numel() <= kMaxRows, std::string(what) + ": " + name + " has more elements than 32-bit indexes reach");
 }
 
@@ -527,8 +530,9 @@ Tensor layer_norm(const Tensor& x, const OptT& weight_in, const OptT& bias_in, d
        std::string(what) + " supports rows of 1 to " + std::to_string(kMaxNormWidth) + " elements, got shape " + shape_text(x));
   for (const auto& [name, t] : {std::pair<const char*, const Tensor&>("weight", weight), std::pair<const char*, const Tensor&>("bias", bias)}) {
     if (!t.defined()) continue;
+    check_plain(t, what);
     must(t.dim() == 1 && t.size(0) == x.size(-1), std::string(name) + " must have shape (" + std::to_string(x.size(-1)) + ",), got " + shape_text(t));
-    must((t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat) && t.device() == x.device() && t.has_storage(),
+    must((t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat) && t.device() == x.device(),
          std::string(what) + ": " + name + " must be on " + x.device().str() + " in " + c10::toString(x.scalar_type()) + " or float32, got " +
              c10::toString(t.scalar_type()) + " on " + t.device().str());
   }
@@ -739,8 +743,9 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   must(weight.size(0) >= 1 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
        w + " supports V >= 1 and 1 <= D <= " + std::to_string(kMaxRowWidth) + ", got weight " + shape_text(weight));
   must(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(), w + ": weight must match x in dtype and device");
+  if (bias.defined()) check_plain(bias, what);
   must(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0) && bias.scalar_type() == x.scalar_type() &&
-                           bias.device() == x.device() && bias.has_storage()),
+                           bias.device() == x.device()),
        w + ": bias must be (" + std::to_string(weight.size(0)) + ",) and match x in dtype and device");
   check_indexes(target, "target", x, what);
   must(target.sizes() == x.sizes().slice(0, x.dim() - 1), w + ": target must have shape " + "x's without its last dimension, got " + shape_text(target) +
