@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const ui
     for (int k = 0; k < VEC; ++k) f[k] = acc[k] * p.scale;
     RawVec<T, VEC> out;
     out.set(f);
-    out.store((T*)p.out.p + v * p.out.sr + c, p.width - c);
+    out.stream((T*)p.out.p + v * p.out.sr + c, p.width - c);
   };
   for (int r = team; r < have; r += TEAMS) {
     const int2 at = bound[r];
