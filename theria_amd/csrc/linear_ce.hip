@@ -17,11 +17,12 @@
 // dz is held without the loss's own factor (1 / kept rows, or the largest |g|), which multiplies the float32 sums, and
 // in float16 times 2^14, so that probabilities down to 2^-38 do not vanish.
 //
-// float32 operands are planes of 16-bit terms (token_gemm.hpp). For the logits two float16 terms, x = h + m to 2^-23, and three
-// products of them (m m, 2^-22 of the product at most and 2^-25 on average, is dropped): each row of x and W is first
-// scaled by the power of two that brings its largest element to 2^13, which the epilogue takes back, so that nothing
-// leaves float16's range. For the gradients, whose sums run over rows of any size, three bfloat16 terms and six products.
-// Against six products throughout: forward 1.7 times as fast, see the figures at Call.
+// float32. Up to 256 rows the operands are multiplied as they are (v_mfma_f32_32x32x2_f32): reading W is most of the work. More
+// rows take planes of 16-bit terms (token_gemm.hpp), laid out by a launch before. For the logits two float16 terms, x = h
+// + m to 2^-22, and three products of them (m m, 2^-22 of the product at most and 2^-25 on average, is dropped): each row of
+// x and W is first scaled by the power of two that brings its largest element to 2^13, which the epilogue takes back, so that
+// nothing leaves float16's range. For the gradients, whose sums run over rows of any size, three bfloat16 terms and six
+// products. XXNATIVE
 #include <type_traits>
 
 #include "token_common.hpp"
@@ -31,7 +32,9 @@
 namespace theria {
 namespace {
 
-constexpr int64_t kPieceBytes = int64_t(256) << 20;  // most of a piece's dz (and of a piece of W laid out anew)
+constexpr int64_t kPieceBytes = int64_t(256) << 20;  // most of a piece's dz
+constexpr int64_t kLayBytes = int64_t(1) << 30;      // most of a piece of W laid out anew
+constexpr int64_t kNativeRows = 256;                 // most rows of float32 products without planes
 
 // ------------------------------------------------------------------------------------------ rows
 struct Meta {
@@ -114,15 +117,15 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward
 }
 
 // Rows laid out for the products: `width` elements, zeros up to kp, a wave for a row. With map: the kept rows of src.
-// 16-bit: a copy. float32: two scaled float16 planes and the exponent of each row's scale at `logits`, and three bfloat16
-// planes at `grads` unless it is null.
+// SPLIT false: a copy. true (float32): two scaled float16 planes and the exponent of each row's scale at `logits`, and three
+// bfloat16 planes at `grads` unless it is null.
 struct LayTo {
   char *logits, *grads;
   int* exponent;
   int64_t plane;  // bytes from plane to plane
   int kp;
 };
-template <typename T>
+template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int width, const int* map, const Meta* meta, LayTo to) {
   const int lane = threadIdx.x % 64;
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int
   const T* row = (const T*)src.p + (map ? (int64_t)map[i] : i) * src.sr;
   RawVec<T, 8> raw;
   int scale = 0;
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (SPLIT) {
     float most = 0.f;  // of the finite elements
     for (int c = lane * 8; c < width; c += 512) {
       float v[8];
@@ -148,8 +151,8 @@ __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int
   for (int c = lane * 8; c < to.kp; c += 512) {
     raw.load(row + c, width - c);
     const int64_t at = (i * to.kp + c) * 2;
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<u32x4_t*>(to.logits + at) = raw.v[0];
+    if constexpr (!SPLIT) {
+      raw.store((T*)to.logits + i * to.kp + c);
     } else {
       float v[8];
       raw.get(v);
@@ -179,7 +182,8 @@ __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int
 
 // ------------------------------------------------------------------------------------------ epilogues
 // What the logits' two epilogues share. Classes are i of the product, rows j.
-template <typename T>
+// SCALED: products of scaled planes.
+template <typename T, bool SCALED>
 struct LogitBase {
   const T* bias;      // of the piece's classes, or null
   int64_t v0;         // the piece's first class
@@ -203,7 +207,7 @@ struct LogitBase {
   template <class S>
   __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
     typedef T quad_t __attribute__((ext_vector_type(4)));
-    if (sizeof(T) == 4 || !bias) return gemm_zero<S>(z);
+    if (SCALED || !bias) return gemm_zero<S>(z);
     const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int fi = 0; fi < S::FI; ++fi)
@@ -222,7 +226,7 @@ struct LogitBase {
   template <class S>
   __device__ __forceinline__ void finish(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t) const {
     const int li = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (SCALED) {
       int ex[S::FJ];
 #pragma unroll
       for (int fj = 0; fj < S::FJ; ++fj) ex[fj] = t.j0 + 32 * fj + li < t.J ? exponent_x[t.j0 + 32 * fj + li] : 0;
@@ -256,8 +260,8 @@ struct LogitBase {
 
 // Forward: of each row (column j of the tile) the largest logit over the tile's classes and the sum of
 // exp(logit - largest), and the target's logit where it lies in the tile.
-template <typename T>
-struct LogitStats : LogitBase<T> {
+template <typename T, bool SCALED>
+struct LogitStats : LogitBase<T, SCALED> {
   float* at_target;   // one of each kept row
   float2* part;       // [tile][n]
   int64_t n;
@@ -317,9 +321,10 @@ struct LogitStats : LogitBase<T> {
   }
 };
 
-// Backward: dz of the tile, in 16 bits (three planes for float32 inputs), rows j of ld elements.
-template <typename T, int PLANES>
-struct LogitGrad : LogitBase<T> {
+// Backward: dz of the tile in the operands' type, or of scaled products in three bfloat16 planes; rows j of ld elements.
+template <typename T, bool SCALED>
+struct LogitGrad : LogitBase<T, SCALED> {
+  static constexpr int PLANES = SCALED ? 3 : 1;
   const int* map;
   const float* stats;  // [2][n]: largest logit, sum
   int64_t n;
@@ -363,39 +368,46 @@ struct LogitGrad : LogitBase<T> {
             z[fi][fj][r] -= it ? 1.f : 0.f;
             at = it ? z[fi][fj][r] * unit : at;
           }
-        if constexpr (PLANES == 1) rest[j] = at - (float)(H)at;
+        if constexpr (sizeof(T) == 2) rest[j] = at - (float)(H)at;
       }
 #pragma unroll
       for (int fi = 0; fi < S::FI; ++fi) z[fi][fj] *= unit;
     }
-    using Stage = GemmStage<S, 2>;
+    using Stage = GemmStage<S, (int)sizeof(H)>;
+    // the share holds every row of 16-bit values, or one block's rows of float32 ones
+    constexpr int kBlocks = sizeof(H) == 2 ? S::FJ : 1;
     // one plane after another through the same LDS
 #pragma unroll 1
     for (int k = 0; k < PLANES; ++k) {
 #pragma unroll
-      for (int fj = 0; fj < S::FJ; ++fj)
+      for (int f0 = 0; f0 < S::FJ; f0 += kBlocks) {
 #pragma unroll
-        for (int fi = 0; fi < S::FI; ++fi)
+        for (int fj = f0; fj < f0 + kBlocks; ++fj)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            H out[4];
+          for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = z[fi][fj][4 * q + e];
-              if constexpr (PLANES == 1) {
-                out[e] = (H)v;
-              } else {
-                __bf16 h, m, l;
-                asm volatile("" : "+v"(v));  // split anew for each plane: the three of a whole tile do not fit the registers
-                split3(v, h, m, l);
-                out[e] = k == 0 ? h : k == 1 ? m : l;
+            for (int q = 0; q < 4; ++q) {
+              H out[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v = z[fi][fj][4 * q + e];
+                if constexpr (PLANES == 1) {
+                  out[e] = (H)v;
+                } else {
+                  __bf16 h, m, l;
+                  asm volatile("" : "+v"(v));  // split anew for each plane: the three of a whole tile do not fit the registers
+                  split3(v, h, m, l);
+                  out[e] = k == 0 ? h : k == 1 ? m : l;
+                }
               }
+              Stage::put(lds, 32 * (fj - f0) + li, fi, q, g, out);
             }
-            Stage::put(lds, 32 * fj + li, fi, q, g, out);
-          }
-      Stage::each(lds, 32 * S::FJ, [&](int r, int i, const i32x4_t& v) {
-        if (t.j0 + r < t.J && t.i0 + i < ld) *reinterpret_cast<i32x4_t*>(dz + k * plane + ((int64_t)(t.j0 + r) * ld + t.i0 + i) * 2) = v;
-      });
+        const int j0 = t.j0 + 32 * f0;
+        Stage::each(lds, 32 * kBlocks, [&](int r, int i, const i32x4_t& v) {
+          if (j0 + r < t.J && t.i0 + i < ld)
+            *reinterpret_cast<i32x4_t*>(dz + k * plane + ((int64_t)(j0 + r) * ld + t.i0 + i) * sizeof(H)) = v;
+        });
+      }
     }
   }
 };
@@ -542,9 +554,9 @@ template <typename T>
 __global__ __launch_bounds__(256) void ce_join_rows_kernel(const float* sums, int splits, int64_t rows, int ld, int width, const int* map,
                                                            const Meta* meta, T* out, int64_t sr, const float* rest,
                                                            const int* target, Rows w) {
-  const int lane = threadIdx.x % 64;
+  const int c = blockIdx.y * 512 + threadIdx.x % 64 * 8;
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  if (i >= rows) return;
+  if (i >= rows || c >= width) return;
   int64_t row = i;
   bool have = true;
   float fill = 0.f;
@@ -557,30 +569,29 @@ __global__ __launch_bounds__(256) void ce_join_rows_kernel(const float* sums, in
   const float f = meta->factor;
   const float left = rest && have ? rest[i] : 0.f;
   const T* row_w = left != 0.f ? (const T*)w.p + target[i] * w.sr : nullptr;
-  for (int c = lane * 8; c < width; c += 512) {
-    float v[8];
-    RawVec<T, 8> o;
-    if (have) {
-      f32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;  // ld is a multiple of 8
-      for (int s = 0; s < splits; ++s) {
-        const f32x4_t* from = reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
-        a += from[0], b += from[1];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
-      if (row_w) {
-        float w8[8];
-        o.load(row_w + c, width - c);
-        o.get(w8);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += left * w8[e];
-      }
+  float v[8];
+  RawVec<T, 8> o;
+  if (have) {
+    f32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;  // ld is a multiple of 8
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const f32x4_t* from = reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
+      a += from[0], b += from[1];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = have ? v[e] * f : fill;
-    o.set(v);
-    o.store(out + row * sr + c, width - c);
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    if (row_w) {
+      float w8[8];
+      o.load(row_w + c, width - c);
+      o.get(w8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += left * w8[e];
+    }
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = have ? v[e] * f : fill;
+  o.set(v);
+  o.store(out + row * sr + c, width - c);
 }
 
 // Column sums of a piece's dz: a thread adds eight columns over its share of the kept rows.
@@ -609,26 +620,45 @@ __global__ __launch_bounds__(256) void ce_bias_kernel(const char* dz, int ld, in
 // ------------------------------------------------------------------------------------------ layout of a call
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// Product tiles: by how many tokens there are, and whether large tiles fill the GPU (a workgroup of 256 x 256 holds a CU by
-// itself and reads half the operand bytes of 128 x 128 for each product). Short products, whose tiles do not last long,
-// take small tiles where large ones would leave over 30% of the CUs without one in their last round: forward of (2000,
-// 10000, 512) bf16 54 -> 48 us, but of (2000, 10000, 1024) 81 us against 87, and of (4096, 32000, 512) 172 against 181.
+// Product tiles, and parts of k for products with few of them. A workgroup of 256 x 256 holds a CU by itself and reads half
+// the operand bytes of 128 x 128 for each product; two of those share a CU, and one's epilogue runs beside the other's
+// products. Up to 64 rows: 128 x 64.
 enum class Tile { kFew, kMid, kLarge };
-Tile tile_for(int64_t I, int64_t J, int64_t K, bool few_columns) {
-  if (few_columns && J <= 64) return Tile::kFew;
-  const int64_t tiles = up(I, 256) / 256 * (up(J, 256) / 256), cus = device_cu_count(), rounds = (tiles + cus - 1) / cus;
-  if (tiles * 5 < cus * 4) return Tile::kMid;
-  return K < 1024 && tiles * 10 < rounds * cus * 7 ? Tile::kMid : Tile::kLarge;
-}
 int tile_i(Tile t) { return t == Tile::kLarge ? 256 : 128; }
 int tile_j(Tile t) { return t == Tile::kLarge ? 256 : t == Tile::kMid ? 128 : 64; }
+int64_t tiles_of(Tile t, int64_t I, int64_t J) { return up(I, tile_i(t)) / tile_i(t) * (up(J, tile_j(t)) / tile_j(t)); }
 
-// Parts of k so that the tiles of I x J fill the GPU, each at least 8 steps long.
-int splits_for(int64_t I, int64_t J, int64_t K, Tile t) {
-  const int64_t tiles = up(I, tile_i(t)) / tile_i(t) * (up(J, tile_j(t)) / tile_j(t)), most = K / (8 * kGemmK);
-  if (tiles == 0) return 1;
-  const int64_t want = (2 * (int64_t)device_cu_count() + tiles - 1) / tiles;
-  return (int)(tiles >= device_cu_count() || most < 2 ? 1 : want < most ? (want < 32 ? want : 32) : (most < 32 ? most : 32));
+struct Pick {
+  Tile tile;
+  int splits;
+};
+
+// The pick with the least time for I x J results of K k by a model of the measured kernels, in us: a step of 64 k takes 1.65
+// in a large workgroup, 1.1 in two small ones on a CU and 0.9 in one alone, an epilogue 6 and 3, and a part's float32 sums
+// are written and read at 4.5 TB/s. (Before, large tiles wherever they alone filled the GPU, dx of (4096, 32000, 1024)
+// bfloat16 took XXPICK; forward of (2000, 10000, 512) takes 48 us in small tiles and 54 us in large ones, of (4096,
+// 32000, 512) 181 and 172.) parts: most parts of k. Parts have at least 8 steps.
+Pick pick(int64_t I, int64_t J, int64_t K, int segments, bool few, bool large, bool parts) {
+  const int64_t cus = device_cu_count();
+  if (I == 0 || J == 0) return {few && J <= 64 ? Tile::kFew : Tile::kMid, 1};
+  const int64_t most = !parts ? 1 : K / 512 < 1 ? 1 : K / 512 < 32 ? K / 512 : 32;
+  if ((few && J <= 64) || !large) {
+    // bound by reading one operand, or by few products: parts until there are two workgroups for each CU
+    const Tile t = few && J <= 64 ? Tile::kFew : Tile::kMid;
+    const int64_t tiles = tiles_of(t, I, J), want = tiles >= cus ? 1 : (2 * cus + tiles - 1) / tiles;
+    return {t, (int)(want < most ? want : most)};
+  }
+  Pick best{Tile::kLarge, 1};
+  double least = 1e30;
+  for (int s = 1; s <= (most < 16 ? most : 16); ++s) {
+    const double steps = (double)((K + 64 * s - 1) / (64 * s)) * segments, sums = parts && s > 1 ? s * 8.0 * I * J / 4.5e6 : 0;
+    const int64_t nl = tiles_of(Tile::kLarge, I, J) * s, nm = tiles_of(Tile::kMid, I, J) * s;
+    const double tl = (double)((nl + cus - 1) / cus) * (1.65 * steps + 6) + sums;
+    const double tm = nm <= cus ? 0.9 * steps + 3 + sums : (double)((nm + 2 * cus - 1) / (2 * cus)) * (1.1 * steps + 3) + sums;
+    if (tl < least) least = tl, best = {Tile::kLarge, s};
+    if (tm < least) least = tm, best = {Tile::kMid, s};
+  }
+  return best;
 }
 
 // Where everything lies in the workspace.
@@ -638,8 +668,7 @@ struct Layout {
   int kp;           // width rounded up to 64
   int64_t piece;    // classes of a piece
   int ldz;          // of a piece's dz
-  Tile tf, tx, tw;  // tiles of the logits, dx, dW
-  int sx, sw;       // splits of dx, dW
+  Pick f, x, w;     // of the logits, dx, dW
   int ldx;          // of the float32 sums
   int tiles;        // of classes, over all pieces
   int bias_parts;
@@ -648,28 +677,29 @@ struct Layout {
 
 Layout layout_of(const CeParams& p, bool backward) {
   Layout l{};
-  l.planes = p.dtype == 0;
-  const int np = l.planes ? 2 : 1, ng = l.planes ? 3 : 1;  // planes of an operand of the logits, of the gradients
+  l.planes = p.dtype == 0 && p.n > kNativeRows;
+  const bool f32 = p.dtype == 0, native = f32 && !l.planes;
+  // bytes of an element of the logits' operands and of the gradients', all planes
+  const int es = f32 ? 4 : 2, bl = es, bg = l.planes ? 6 : es, per = 16 / es;
   l.kp = (int)up(p.width, 64);
   // the copies take 16-byte pieces and 32-bit offsets inside a tile
-  l.lay_w = l.planes || p.width % 8 || p.w.sr % 8 || (uintptr_t)p.w.p % 16 || p.w.sr > (1 << 21);
+  l.lay_w = l.planes || p.width % per || p.w.sr % per || (uintptr_t)p.w.p % 16 || p.w.sr > (1 << 20);
   l.piece = up(p.classes, 64);
-  auto limit = [&](int64_t row_bytes) {  // bytes of one class
-    const int64_t most = kPieceBytes / row_bytes / 256 * 256;
+  auto limit = [&](int64_t bytes, int64_t row_bytes) {  // bytes of one class
+    const int64_t most = bytes / row_bytes / 256 * 256;
     if (l.piece > most) l.piece = most < 256 ? 256 : most;
   };
-  if (l.lay_w) limit(2 * (np + (l.planes && backward ? ng : 0)) * (int64_t)l.kp);
-  if (backward && p.n > 0) limit(2 * ng * p.n);
+  if (l.lay_w) limit(kLayBytes, (bl + (l.planes && backward ? bg : 0)) * (int64_t)l.kp);
+  if (backward && p.n > 0) limit(kPieceBytes, bg * p.n);
   l.ldz = (int)l.piece;
-  l.tf = tile_for(l.piece, p.n, p.width, true);
-  l.tx = tile_for(p.width, p.n, l.piece, true);
-  l.tw = tile_for(p.width, l.piece, p.n, false);
-  l.sx = splits_for(p.width, p.n, l.piece, l.tx);
-  l.sw = splits_for(p.width, l.piece, p.n, l.tw);
+  const int segments_l = l.planes ? 3 : 1, segments_g = l.planes ? 6 : 1;
+  l.f = pick(l.piece, p.n, p.width, segments_l, true, !native, false);
+  l.x = pick(p.width, p.n, l.piece, segments_g, true, !native, true);
+  l.w = pick(p.width, l.piece, p.n, segments_g, false, !native, true);
   l.ldx = (int)up(p.width, 8);
   l.bias_parts = (int)(p.n < 64 ? 1 : p.n / 64 < 64 ? p.n / 64 : 64);
   for (int64_t v = 0; v < p.classes; v += l.piece)
-    l.tiles += (int)(up(p.classes - v < l.piece ? p.classes - v : l.piece, tile_i(l.tf)) / tile_i(l.tf));
+    l.tiles += (int)(up(p.classes - v < l.piece ? p.classes - v : l.piece, tile_i(l.f.tile)) / tile_i(l.f.tile));
   auto take = [&](int64_t bytes) {
     const int64_t at = l.bytes;
     l.bytes += up(bytes, 256);
@@ -678,12 +708,12 @@ Layout layout_of(const CeParams& p, bool backward) {
   l.meta = take(sizeof(Meta));
   l.map = take(4 * p.n);
   l.target = take(4 * p.n);
-  l.xs = take(2 * np * p.n * l.kp);
-  if (l.lay_w) l.ws_w = take(2 * np * l.piece * l.kp);
+  l.xs = take(bl * p.n * l.kp);
+  if (l.lay_w) l.ws_w = take(bl * l.piece * l.kp);
   if (l.planes) {
     l.ex_x = take(4 * p.n);
     l.ex_w = take(4 * l.piece);
-    if (backward) l.xs_grad = take(2 * ng * p.n * l.kp), l.ws_w_grad = take(2 * ng * l.piece * l.kp);
+    if (backward) l.xs_grad = take(bg * p.n * l.kp), l.ws_w_grad = take(bg * l.piece * l.kp);
   }
   if (!backward) {
     l.at_target = take(4 * p.n);
@@ -691,9 +721,9 @@ Layout layout_of(const CeParams& p, bool backward) {
     l.row_loss = take(4 * p.n);
   } else {
     l.rest = take(4 * p.n);
-    l.dz = take(2 * ng * p.n * l.ldz);
-    if (p.dx.p) l.sum_x = take(4 * l.sx * p.n * l.ldx);
-    if (p.dw.p && l.sw > 1) l.sum_w = take(4 * l.sw * l.piece * l.ldx);
+    l.dz = take(bg * p.n * l.ldz);
+    if (p.dx.p) l.sum_x = take(4 * l.x.splits * p.n * l.ldx);
+    if (p.dw.p && l.w.splits > 1) l.sum_w = take(4 * l.w.splits * l.piece * l.ldx);
     if (p.db) l.bias_part = take(4 * (int64_t)l.bias_parts * l.ldz);
   }
   return l;
@@ -702,7 +732,9 @@ Layout layout_of(const CeParams& p, bool backward) {
 template <typename H, bool A, bool B, class Epi>
 hipError_t gemm(Tile t, const GemmParams& g, const Epi& e, hipStream_t st) {
   switch (t) {
-    case Tile::kLarge: return launch_gemm<GemmShape<H, 256, 256, 2, 4, A, B>>(g, e, st);
+    case Tile::kLarge:
+      if constexpr (sizeof(H) == 2) return launch_gemm<GemmShape<H, 256, 256, 2, 4, A, B>>(g, e, st);
+      break;
     case Tile::kMid: return launch_gemm<GemmShape<H, 128, 128, 2, 2, A, B>>(g, e, st);
     case Tile::kFew:
       if constexpr (!B) return launch_gemm<GemmShape<H, 128, 64, 4, 1, A, B>>(g, e, st);
@@ -716,11 +748,11 @@ hipError_t gemm(Tile t, const GemmParams& g, const Epi& e, hipStream_t st) {
     if (e_ != hipSuccess) return e_;    \
   } while (0)
 
-template <typename T>
+// SPLIT: float32 operands in planes.
+template <typename T, bool SPLIT>
 struct Call {
-  static constexpr bool kSplit = sizeof(T) == 4;
-  using L = typename std::conditional<kSplit, _Float16, T>::type;  // operands of the logits
-  using H = typename std::conditional<kSplit, __bf16, T>::type;    // operands of the gradients
+  using L = typename std::conditional<SPLIT, _Float16, T>::type;  // operands of the logits
+  using H = typename std::conditional<SPLIT, __bf16, T>::type;    // operands of the gradients
   const CeParams& p;
   const Layout l;
   hipStream_t st;
@@ -732,21 +764,23 @@ struct Call {
   Call(const CeParams& p_, bool backward, hipStream_t st_)
       : p(p_), l(layout_of(p_, backward)), st(st_), ws((char*)p_.ws), map((int*)(ws + l.map)), target((int*)(ws + l.target)), meta((Meta*)(ws + l.meta)) {}
 
-  int64_t plane_x() const { return 2 * p.n * l.kp; }
-  int64_t plane_w() const { return 2 * l.piece * l.kp; }
-  int64_t plane_z() const { return 2 * p.n * l.ldz; }
-  static constexpr int kLogitSegments = kSplit ? 3 : 1, kGradSegments = kSplit ? 6 : 1;
+  static constexpr int ES = sizeof(H);
+  static_assert(sizeof(L) == ES);
+  int64_t plane_x() const { return ES * p.n * l.kp; }
+  int64_t plane_w() const { return ES * l.piece * l.kp; }
+  int64_t plane_z() const { return ES * p.n * l.ldz; }
+  static constexpr int kLogitSegments = SPLIT ? 3 : 1, kGradSegments = SPLIT ? 6 : 1;
   // Operands along k belong to the logits, but for dz; those across k to the gradients.
   GemmOperand x_operand(bool across) const {
-    return {ws + (across && kSplit ? l.xs_grad : l.xs), 2 * (int64_t)l.kp, plane_x(), across ? l.kp : (int)p.n};
+    return {ws + (across && SPLIT ? l.xs_grad : l.xs), ES * (int64_t)l.kp, plane_x(), across ? l.kp : (int)p.n};
   }
-  GemmOperand z_operand(bool across) const { return {ws + l.dz, 2 * (int64_t)l.ldz, plane_z(), across ? l.ldz : (int)p.n}; }
+  GemmOperand z_operand(bool across) const { return {ws + l.dz, ES * (int64_t)l.ldz, plane_z(), across ? l.ldz : (int)p.n}; }
   // classes [v, v + have)
   GemmOperand w_operand(bool across, int64_t v, int have) const {
-    if (l.lay_w) return {ws + (across && kSplit ? l.ws_w_grad : l.ws_w), 2 * (int64_t)l.kp, plane_w(), across ? l.kp : have};
-    return {(const char*)p.w.p + v * p.w.sr * 2, 2 * p.w.sr, 0, across ? p.width : have};
+    if (l.lay_w) return {ws + (across && SPLIT ? l.ws_w_grad : l.ws_w), ES * (int64_t)l.kp, plane_w(), across ? l.kp : have};
+    return {(const char*)p.w.p + v * p.w.sr * ES, ES * p.w.sr, 0, across ? p.width : have};
   }
-  LogitBase<T> base(int64_t v) const {
+  LogitBase<T, SPLIT> base(int64_t v) const {
     return {p.bias ? (const T*)p.bias + v : nullptr, v, target, (const int*)(ws + l.ex_w), (const int*)(ws + l.ex_x)};
   }
 
@@ -754,13 +788,13 @@ struct Call {
     ce_rows_kernel<<<1, 1024, 0, st>>>(p, backward, map, target, meta);
     THERIA_TRY(hipGetLastError());
     if (p.n == 0) return hipSuccess;
-    ce_lay_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, LayTo{ws + l.xs, backward && kSplit ? ws + l.xs_grad : nullptr, (int*)(ws + l.ex_x), plane_x(), l.kp});
+    ce_lay_kernel<T, SPLIT><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, LayTo{ws + l.xs, backward && SPLIT ? ws + l.xs_grad : nullptr, (int*)(ws + l.ex_x), plane_x(), l.kp});
     return hipGetLastError();
   }
   hipError_t lay_piece(bool backward, int64_t v, int have) {
     if (!l.lay_w) return hipSuccess;
     const Rows src{(const T*)p.w.p + v * p.w.sr, p.w.sr};
-    ce_lay_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, LayTo{ws + l.ws_w, backward && kSplit ? ws + l.ws_w_grad : nullptr, (int*)(ws + l.ex_w), plane_w(), l.kp});
+    ce_lay_kernel<T, SPLIT><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, LayTo{ws + l.ws_w, backward && SPLIT ? ws + l.ws_w_grad : nullptr, (int*)(ws + l.ex_w), plane_w(), l.kp});
     return hipGetLastError();
   }
 
@@ -771,9 +805,9 @@ struct Call {
       const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
       THERIA_TRY(lay_piece(false, v, have));
       const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, kLogitSegments, &meta->kept, true, false};
-      const LogitStats<T> e{base(v), (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
-      THERIA_TRY((gemm<L, false, false>(l.tf, g, e, st)));
-      tile0 += (int)(up(have, tile_i(l.tf)) / tile_i(l.tf));
+      const LogitStats<T, SPLIT> e{base(v), (float*)(ws + l.at_target), (float2*)(ws + l.part), p.n, tile0};
+      THERIA_TRY((gemm<L, false, false>(l.f.tile, g, e, st)));
+      tile0 += (int)(up(have, tile_i(l.f.tile)) / tile_i(l.f.tile));
     }
     float* row_loss = p.reduction == kCeNone ? p.loss : (float*)(ws + l.row_loss);
     // few rows: a workgroup for each, so that the tiles' partial sums are read by more threads
@@ -791,30 +825,30 @@ struct Call {
   }
 
   hipError_t backward() {
-    constexpr int PLANES = kSplit ? 3 : 1;
+    constexpr int PLANES = SPLIT ? 3 : 1;
     THERIA_TRY(rows(true));
     for (int64_t v = 0; v < p.classes; v += l.piece) {
       const int have = (int)(p.classes - v < l.piece ? p.classes - v : l.piece);
       THERIA_TRY(lay_piece(true, v, have));
       {
         const GemmParams g{w_operand(false, v, have), x_operand(false), have, (int)p.n, p.width, 1, kLogitSegments, &meta->kept, true, false};
-        const LogitGrad<T, PLANES> e{base(v), map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, (float*)(ws + l.rest), ws + l.dz, l.ldz, plane_z()};
-        THERIA_TRY((gemm<L, false, false>(l.tf, g, e, st)));
+        const LogitGrad<T, SPLIT> e{base(v), map, p.stats, p.n, p.reduction == kCeNone ? p.gout : nullptr, meta, (float*)(ws + l.rest), ws + l.dz, l.ldz, plane_z()};
+        THERIA_TRY((gemm<L, false, false>(l.f.tile, g, e, st)));
       }
       if (p.dx.p) {
-        const GemmParams g{w_operand(true, v, have), z_operand(false), p.width, (int)p.n, have, l.sx, kGradSegments, &meta->kept, true, false};
+        const GemmParams g{w_operand(true, v, have), z_operand(false), p.width, (int)p.n, have, l.x.splits, kGradSegments, &meta->kept, true, false};
         const SumTile e{(float*)(ws + l.sum_x), p.n, l.ldx, v > 0};
-        THERIA_TRY((gemm<H, true, false>(l.tx, g, e, st)));
+        THERIA_TRY((gemm<H, true, false>(l.x.tile, g, e, st)));
       }
       if (p.dw.p) {
         T* out = (T*)p.dw.p + v * p.dw.sr;
-        const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.sw, kGradSegments, &meta->kept, false, true};
-        if (l.sw == 1) {
-          THERIA_TRY((gemm<H, true, true>(l.tw, g, OutTile<T>{out, p.dw.sr, meta}, st)));
+        const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.w.splits, kGradSegments, &meta->kept, false, true};
+        if (l.w.splits == 1) {
+          THERIA_TRY((gemm<H, true, true>(l.w.tile, g, OutTile<T>{out, p.dw.sr, meta}, st)));
         } else {
           float* sums = (float*)(ws + l.sum_w);
-          THERIA_TRY((gemm<H, true, true>(l.tw, g, SumTile{sums, l.piece, l.ldx, false}, st)));
-          ce_join_rows_kernel<T><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(sums, l.sw, l.piece, l.ldx, p.width, nullptr, meta, out, p.dw.sr, nullptr, nullptr, Rows{});
+          THERIA_TRY((gemm<H, true, true>(l.w.tile, g, SumTile{sums, l.piece, l.ldx, false}, st)));
+          ce_join_rows_kernel<T><<<dim3((unsigned)((have + 3) / 4), (p.width + 511) / 512), 256, 0, st>>>(sums, l.w.splits, l.piece, l.ldx, p.width, nullptr, meta, out, p.dw.sr, nullptr, nullptr, Rows{});
           THERIA_TRY(hipGetLastError());
         }
       }
@@ -827,23 +861,23 @@ struct Call {
       }
     }
     if (p.dx.p && p.n > 0) {
-      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>((const float*)(ws + l.sum_x), l.sx, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, kSplit ? nullptr : (const float*)(ws + l.rest), target, p.w);
+      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4), (p.width + 511) / 512), 256, 0, st>>>((const float*)(ws + l.sum_x), l.x.splits, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, sizeof(T) == 4 ? nullptr : (const float*)(ws + l.rest), target, p.w);
       THERIA_TRY(hipGetLastError());
     }
     return hipSuccess;
   }
 };
 
-template <typename T>
+template <typename T, bool SPLIT>
 hipError_t run(const CeParams& p, bool backward, hipStream_t st) {
-  Call<T> c(p, backward, st);
+  Call<T, SPLIT> c(p, backward, st);
   return backward ? c.backward() : c.forward();
 }
 
 hipError_t by_type(const CeParams& p, bool backward, hipStream_t st) {
-  if (p.dtype == 0) return run<float>(p, backward, st);
-  if (p.dtype == 1) return run<_Float16>(p, backward, st);
-  return run<__bf16>(p, backward, st);
+  if (p.dtype == 0) return p.n > kNativeRows ? run<float, true>(p, backward, st) : run<float, false>(p, backward, st);
+  if (p.dtype == 1) return run<_Float16, false>(p, backward, st);
+  return run<__bf16, false>(p, backward, st);
 }
 
 }  // namespace

@@ -1,13 +1,14 @@
-// Matrix products of 16-bit operands for the linear cross entropy: C[i][j] = sum_k A[i][k] B[j][k] on MFMA (gfx950).
+// Matrix products for the linear cross entropy: C[i][j] = sum_k A[i][k] B[j][k] on MFMA (gfx950).
 //
 // Either operand lies in memory "along k" (rows i, k contiguous) or "across k" (rows k, i contiguous); the second kind is
 // transposed on its way from LDS to registers (ds_read_b64_tr_b16), so that no transposed copy is ever made. A workgroup
-// owns a tile of TI x TJ results, walks k in steps of 64 and keeps two stages of both operands in LDS, filled by LDS DMA:
-// the next step's copies run while this step's products do.
+// owns a tile of TI x TJ results, walks k in steps of 128 bytes (64 elements of 16 bits) and keeps two stages of both
+// operands in LDS, filled by LDS DMA: the next step's copies run while this step's products do.
 //
-// float32 operands come as planes of 16-bit terms. Two each, x = h + m: three passes over k (m h, h m, h h). Three each, x = h
-// + m + l (split3): six passes (m m, l h, h l, m h, h m, h h), whose dropped terms are at most 2^-24 of the product. The
-// smallest come first.
+// float32 operands either go to v_mfma_f32_32x32x2_f32 as they are (H = float; a sixteenth of the 16-bit rate, but nothing
+// is laid out anew), or come as planes of 16-bit terms. Two each, x = h + m: three passes over k (m h, h m, h h). Three
+// each, x = h + m + l (split3): six passes (m m, l h, h l, m h, h m, h h), whose dropped terms are at most 2^-24 of the
+// product. The smallest come first.
 //
 // The accumulators have i along registers and j along lanes: lane l holds column j = l % 32 of a 32 x 32 block and four
 // consecutive i in each group of four registers, so sums over i stay inside a lane and i is written in pieces of four.
@@ -19,7 +20,21 @@ namespace theria {
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kGemmK = 64;  // k per step
+// Operand fragments of 32 x 32 results: 16 bytes a lane, 16 k (float32: 8 k, as four instructions of two).
+template <typename H>
+struct GemmMma {
+  using frag_t = typename Mfma<H>::frag_t;
+  __device__ __forceinline__ static f32x16_t mma(frag_t a, frag_t b, f32x16_t c) { return Mfma<H>::mma(a, b, c); }
+};
+template <>
+struct GemmMma<float> {
+  using frag_t = f32x4_t;
+  __device__ __forceinline__ static f32x16_t mma(frag_t a, frag_t b, f32x16_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
 
 struct GemmOperand {
   const char* base;
@@ -47,11 +62,18 @@ __device__ __forceinline__ void split3(float x, __bf16& h, __bf16& m, __bf16& l)
   l = (__bf16)(r - (float)m);
 }
 
-// Copies of one operand's tile: EXT x 64 elements, EXT / 8 wave instructions over NW waves. Every address is inside the
-// operand: a lane whose row, column or k lies outside uses an offset past the buffer's end and gets zeros.
-template <bool ACROSS, int EXT, int NW>
+// Slot of 16-byte chunk `chunk` in row k of an across-k tile of 128 columns, for elements of ES bytes. 16 bits: see swz<128>.
+// float32: rows 4 apart, which the two halves of a wave read at once, take different halves of the banks.
+template <int ES>
+__device__ __forceinline__ int across_slot(int k, int chunk) {
+  return ES == 2 ? chunk ^ swz<128>(k) : chunk ^ ((k >> 2 & 1) << 3);
+}
+
+// Copies of one operand's tile: EXT rows or columns of a step, EXT / 8 wave instructions over NW waves. Every address is
+// inside the operand: a lane whose row, column or k lies outside uses an offset past the buffer's end and gets zeros.
+template <int ES, bool ACROSS, int EXT, int NW>
 struct GemmLoader {
-  static constexpr int NQ = EXT / 8 / NW;
+  static constexpr int NQ = EXT / 8 / NW, kStep = 128 / ES, kChunk = 16 / ES, kLanes = 8 * ES;  // lanes of an across row
   static constexpr uint32_t kOut = 0x80000000u, kRange = 0x7fffffffu;
   static_assert(NQ * NW * 8 == EXT && (!ACROSS || EXT % 128 == 0));
   uint32_t off[NQ];
@@ -64,20 +86,20 @@ struct GemmLoader {
     for (int q = 0; q < NQ; ++q) {
       const int piece = q * NW + w;
       if constexpr (ACROSS) {
-        const int row = piece % 16 * 4 + lane / 16, col = piece / 16 * 128 + ((lane % 16) ^ swz<128>(row)) * 8;
-        off[q] = col < valid ? (uint32_t)(row * ld) + col * 2 : kOut;
+        const int row = piece % 16 * (64 / kLanes) + lane / kLanes, col = piece / 16 * 128 + across_slot<ES>(row, lane % kLanes) * kChunk;
+        off[q] = col < valid ? (uint32_t)(row * ld) + col * ES : kOut;
         at[q] = row;
       } else {
         const int row = piece * 8 + lane / 8, chunk = (lane % 8) ^ swz<64>(row);
         off[q] = row < valid ? (uint32_t)(row * ld) + chunk * 16 : kOut;
-        at[q] = chunk * 8;
+        at[q] = chunk * kChunk;
       }
     }
   }
   // base: the tile at this step's first k, of which `left` remain.
   __device__ __forceinline__ void issue(const char* base, char* lds, int left) const {
     const rsrc_t r = make_rsrc(base, kRange);
-    if (left >= kGemmK) {
+    if (left >= kStep) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) dma16(r, lds + (q * NW + wave) * 1024, off[q], 0);
     } else {
@@ -87,12 +109,14 @@ struct GemmLoader {
   }
 };
 
-// A lane's addresses in a tile for fragments of 32 rows from row r0 + 32 f, k chunk c of 16, in the KLIN order for both
-// kinds. The swizzles separate: along k it depends on c and the lane alone (32 f rows are a constant distance), across k
-// on f and the lane (a chunk of 16 rows is), so that a few offsets serve every fragment of a step.
+// A lane's addresses in a tile for fragments of 32 rows from row r0 + 32 f, k chunk c (a quarter of the step). Both kinds
+// hand lane half g the same k: 8 g + e of a 16-bit chunk, 4 g + e of a float32 one. The swizzles separate: along k it
+// depends on c and the lane alone (32 f rows are a constant distance), across k on f and the lane (a chunk's rows are),
+// so that a few offsets serve every fragment of a step.
 template <typename H, bool ACROSS, int NF>
 struct GemmFrags {
-  static constexpr int N = ACROSS ? 2 * NF : kGemmK / 16;
+  static constexpr int ES = sizeof(H), N = !ACROSS ? 4 : ES == 2 ? 2 * NF : NF;
+  using frag_t = typename GemmMma<H>::frag_t;
   uint32_t off[N];
 
   __device__ __forceinline__ void init(int r0) {
@@ -102,23 +126,35 @@ struct GemmFrags {
 #pragma unroll
       for (int c = 0; c < N; ++c) off[c] = row * 128 + (((2 * c + g) ^ swz<64>(row)) << 4);
     } else {
-      const int s = lane & 15, hh = (lane >> 4) & 1;
 #pragma unroll
-      for (int f = 0; f < NF; ++f)
+      for (int f = 0; f < NF; ++f) {
+        const int r = r0 + 32 * f, sub = r / 128 * 16384;
+        if constexpr (ES == 2) {
+          const int s = lane & 15, col = r % 128 + 16 * ((lane >> 4) & 1) + 4 * (s & 3);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int r = r0 + 32 * f, col = r % 128 + 16 * hh + 4 * (s & 3), k = 8 * g + 4 * b + (s >> 2);
-          off[2 * f + b] = r / 128 * (kGemmK * 256) + k * 256 + (((col >> 3) ^ swz<128>(k)) << 4) + (col & 7) * 2;
+          for (int b = 0; b < 2; ++b) {
+            const int k = 8 * g + 4 * b + (s >> 2);
+            off[2 * f + b] = sub + k * 256 + (across_slot<ES>(k, col >> 3) << 4) + (col & 7) * 2;
+          }
+        } else {
+          const int col = r % 128 + (lane & 31), k = 4 * g;
+          off[f] = sub + k * 512 + (across_slot<ES>(k, col >> 2) << 4) + (col & 3) * 4;
         }
+      }
     }
   }
-  __device__ __forceinline__ typename Mfma<H>::frag_t get(const char* tile, int f, int c) const {
+  __device__ __forceinline__ frag_t get(const char* tile, int f, int c) const {
     if constexpr (!ACROSS) {
-      return __builtin_bit_cast(typename Mfma<H>::frag_t, *reinterpret_cast<const i16x8_t*>(tile + off[c] + f * 4096));
-    } else {
+      return __builtin_bit_cast(frag_t, *reinterpret_cast<const i16x8_t*>(tile + off[c] + f * 4096));
+    } else if constexpr (ES == 2) {
       const i16x4_t a = ds_read_tr16(tile + off[2 * f] + c * 4096), b = ds_read_tr16(tile + off[2 * f + 1] + c * 4096);
       const i16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      return __builtin_bit_cast(typename Mfma<H>::frag_t, v);
+      return __builtin_bit_cast(frag_t, v);
+    } else {
+      frag_t v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(tile + off[f] + c * 4096 + e * 512);
+      return v;
     }
   }
 };
@@ -134,6 +170,7 @@ struct GemmTile {
 template <typename H_, int TI_, int TJ_, int WI_, int WJ_, bool A_, bool B_>
 struct GemmShape {
   using H = H_;
+  static constexpr int ES = sizeof(H_), K = 128 / ES;  // bytes of an element, k of a step
   static constexpr int TI = TI_, TJ = TJ_, WI = WI_, WJ = WJ_, NW = WI_ * WJ_;
   static constexpr bool A = A_, B = B_;
   static constexpr int FI = TI_ / WI_ / 32, FJ = TJ_ / WJ_ / 32;
@@ -182,7 +219,7 @@ __device__ __forceinline__ void gemm_zero(f32x16_t (&z)[S::FI][S::FJ]) {
 template <class S, class Epi>
 __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi) {
   using H = typename S::H;
-  constexpr int TI = S::TI, TJ = S::TJ, FI = S::FI, FJ = S::FJ, NW = S::NW;
+  constexpr int TI = S::TI, TJ = S::TJ, FI = S::FI, FJ = S::FJ, NW = S::NW, ES = S::ES;
   // two stages as arrays of their own, so that the reads of one are known not to wait for the copies into the other
   __shared__ __align__(1024) char a0[TI * 128], b0[TJ * 128], a1[TI * 128], b1[TJ * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -205,17 +242,17 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
   t.j0 = t.tile_j * TJ + t.wave_j * (TJ / S::WJ);
 
   // this part's k, in whole steps
-  const int steps_all = (K + kGemmK - 1) / kGemmK, steps_per = (steps_all + p.splits - 1) / p.splits;
+  const int steps_all = (K + S::K - 1) / S::K, steps_per = (steps_all + p.splits - 1) / p.splits;
   const int first = min(t.split * steps_per, steps_all), ksteps = min(steps_per, steps_all - first), steps = ksteps * p.segments;
 
   const int ti0 = t.tile_i * TI, tj0 = t.tile_j * TJ;
-  GemmLoader<S::A, TI, NW> la;
-  GemmLoader<S::B, TJ, NW> lb;
+  GemmLoader<ES, S::A, TI, NW> la;
+  GemmLoader<ES, S::B, TJ, NW> lb;
   la.init(wave, lane, p.a.ld, p.a.extent - ti0);
   lb.init(wave, lane, p.b.ld, (p.j_kept ? kept : p.b.extent) - tj0);
-  const int64_t astep = S::A ? kGemmK * p.a.ld : 2 * kGemmK, bstep = S::B ? kGemmK * p.b.ld : 2 * kGemmK;
-  const char* abase = p.a.base + (S::A ? (int64_t)ti0 * 2 : (int64_t)ti0 * p.a.ld) + first * astep;
-  const char* bbase = p.b.base + (S::B ? (int64_t)tj0 * 2 : (int64_t)tj0 * p.b.ld) + first * bstep;
+  const int64_t astep = S::A ? S::K * p.a.ld : 128, bstep = S::B ? S::K * p.b.ld : 128;
+  const char* abase = p.a.base + (S::A ? (int64_t)ti0 * ES : (int64_t)ti0 * p.a.ld) + first * astep;
+  const char* bbase = p.b.base + (S::B ? (int64_t)tj0 * ES : (int64_t)tj0 * p.b.ld) + first * bstep;
   // planes of the segments, two bits each, the first segment lowest: a = m l h m h h, b = m h l h m h; or m h h, h m h
   const uint32_t planes_a = p.segments == 6 ? 0x049u : p.segments == 3 ? 0x01u : 0u;
   const uint32_t planes_b = p.segments == 6 ? 0x121u : p.segments == 3 ? 0x04u : 0u;
@@ -224,7 +261,7 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
 
   int seg = 0, ks = 0;  // of the next step to copy
   auto copy = [&](char* a, char* b) {
-    const int left = K - (first + ks) * kGemmK;
+    const int left = K - (first + ks) * S::K;
     la.issue(abase + (int64_t)(planes_a >> (2 * seg) & 3) * p.a.plane + ks * astep, a, left);
     lb.issue(bbase + (int64_t)(planes_b >> (2 * seg) & 3) * p.b.plane + ks * bstep, b, left);
     if (++ks == ksteps) ks = 0, ++seg;
@@ -236,8 +273,8 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
   // A stage's products, chunk by chunk: chunk c + 1 is read while chunk c's products run, and no earlier (the barriers
   // bound the registers). The last chunk's products wait for the next stage, whose first chunk is read meanwhile: after
   // the workgroup's barrier every wave has products to run.
-  constexpr int NC = kGemmK / 16;
-  typename Mfma<H>::frag_t fa[2][FI], fb[2][FJ];
+  constexpr int NC = 4;
+  typename GemmMma<H>::frag_t fa[2][FI], fb[2][FJ];
   auto read = [&](const char* a, const char* b, int c) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < FI; ++i) fa[c & 1][i] = ra.get(a, i, c);
@@ -248,7 +285,7 @@ __global__ __launch_bounds__(S::NW * 64) void gemm_kernel(GemmParams p, Epi epi)
 #pragma unroll
     for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) acc[i][j] = Mfma<H>::mma(fa[c & 1][i], fb[c & 1][j], acc[i][j]);
+      for (int j = 0; j < FJ; ++j) acc[i][j] = GemmMma<H>::mma(fa[c & 1][i], fb[c & 1][j], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
   };
   auto stage = [&](const char* a, const char* b, bool first) __attribute__((always_inline)) {
