@@ -83,6 +83,19 @@ def test_wide_rows_take_large_tiles_in_both_gradients(hip_device):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("N", [16384, 16385, 40000])
+def test_many_rows_are_listed_by_several_workgroups(dt, N, hip_device):
+    """On both sides of the limit of one workgroup; ignored and invalid targets in runs, at both ends, and everywhere."""
+    x, w, t, b, g = _make(N, 20, 24, dt, hip_device, seed=4, bias=True, pad=0.3)
+    t[:5000], t[-3:] = IGNORE, IGNORE
+    t[9000:9100], t[N - 10] = 20, -7
+    _check(x, w, t, b, "none", g, f"{N} rows")
+    t[:] = IGNORE
+    got = _run(x, w, t, b, "sum")
+    assert not got["loss"].any() and not got["dx"].any() and not got["dw"].any()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 def test_ignored_rows_are_never_read(dt, reduction, hip_device):
     x, w, t, b, g = _make(300, 200, 72, dt, hip_device, seed=3, bias=True, pad=0.5)

@@ -22,7 +22,8 @@
 // + m to 2^-22, and three products of them (m m, 2^-22 of the product at most and 2^-25 on average, is dropped): each row of
 // x and W is first scaled by the power of two that brings its largest element to 2^13, which the epilogue takes back, so that
 // nothing leaves float16's range. For the gradients, whose sums run over rows of any size, three bfloat16 terms and six
-// products. XXNATIVE
+// products. ((48, 32000, 4096) forward and gradients: 0.76 ms as they are, 2 ms in planes; (2000, 10000, 1024): 0.87 ms in
+// planes, of six products throughout 1.25 ms.)
 #include <type_traits>
 
 #include "token_common.hpp"
@@ -43,34 +44,90 @@ struct Meta {
   float factor;  // of the float32 sums that become gradients
 };
 
-constexpr int kScanPer = 4;
+constexpr int kScanPer = 4, kScan = 1024 * kScanPer;  // rows of a thread and of a workgroup in a round
+
+struct RowTarget {
+  int64_t target;
+  bool keep, drop;
+};
+__device__ __forceinline__ RowTarget row_target(const CeParams& p, int64_t n) {
+  if (n >= p.n) return {0, false, false};
+  const int64_t t = p.target64 ? ((const int64_t*)p.target)[n] : (int64_t)((const int32_t*)p.target)[n];
+  const bool valid = t != p.ignore && t >= 0 && t < p.classes;
+  return {t, valid, !valid};
+}
+
+// Kept rows and largest finite |g| of each kScan rows, for the launch that lists them with several workgroups.
+struct RowCount {
+  int kept;
+  float most;
+};
+__device__ __forceinline__ float kept_gradient(const CeParams& p, int64_t n) {
+  const float g = fabsf(p.gout[n]);
+  return g < THERIA_INF ? g : 0.f;
+}
+// The sum of `kept` and the largest `most` over a workgroup of 16 waves, in every thread.
+__device__ __forceinline__ void block_count(int& kept, float& most, RowCount* red) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    kept += __shfl_xor(kept, o);
+    most = fmaxf(most, __shfl_xor(most, o));
+  }
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = {kept, most};
+  __syncthreads();
+  kept = 0;
+  for (int w = 0; w < 16; ++w) kept += red[w].kept, most = fmaxf(most, red[w].most);
+}
+__global__ __launch_bounds__(1024) void ce_count_kernel(CeParams p, bool gradients, RowCount* counts) {
+  __shared__ RowCount red[16];
+  int kept = 0;
+  float most = 0.f;
+#pragma unroll
+  for (int u = 0; u < kScanPer; ++u) {
+    const int64_t n = (int64_t)blockIdx.x * kScan + u * 1024 + threadIdx.x;
+    if (row_target(p, n).keep) {
+      ++kept;
+      if (gradients) most = fmaxf(most, kept_gradient(p, n));
+    }
+  }
+  block_count(kept, most, red);
+  if (threadIdx.x == 0) counts[blockIdx.x] = {kept, most};
+}
 
 // map: the kept rows in order, then from the end the dropped ones, ignored as n, invalid as -n - 1. target: of the kept.
-__global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward, int* map, int* target, Meta* meta) {
+// One workgroup for all rows, or with `counts` one for every kScan.
+__global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward, const RowCount* counts, int* map, int* target, Meta* meta) {
   __shared__ int wave_kept[2][16];
-  __shared__ float wave_most[16];
+  __shared__ RowCount red[2][16];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  int64_t kept = 0;  // before this round's rows
+  const bool gradients = backward && p.reduction == kCeNone;
+  int64_t first = 0, end = p.n;
+  int kept = 0;  // before this round's rows
+  int all_kept = 0;
   float most = 0.f;
+  if (counts) {
+    const int blocks = gridDim.x;
+    float none = 0.f;
+    for (int b = threadIdx.x; b < blocks; b += 1024) {
+      all_kept += counts[b].kept;
+      kept += b < (int)blockIdx.x ? counts[b].kept : 0;
+      most = fmaxf(most, counts[b].most);
+    }
+    block_count(all_kept, most, red[0]);
+    block_count(kept, none, red[1]);
+    first = (int64_t)blockIdx.x * kScan;
+    end = first + kScan < p.n ? first + kScan : p.n;
+  }
   int turn = 0;
-  for (int64_t base = 0; base < p.n; base += 1024 * kScanPer, turn ^= 1) {
+  for (int64_t base = first; base < end; base += kScan, turn ^= 1) {
     const int64_t n0 = base + threadIdx.x * kScanPer;
-    int64_t t[kScanPer];
-    bool keep[kScanPer], drop[kScanPer];
+    RowTarget t[kScanPer];
     int mine = 0;
 #pragma unroll
     for (int u = 0; u < kScanPer; ++u) {
-      const int64_t n = n0 + u;
-      const bool in = n < p.n;
-      t[u] = !in ? 0 : p.target64 ? ((const int64_t*)p.target)[n] : (int64_t)((const int32_t*)p.target)[n];
-      const bool valid = t[u] != p.ignore && t[u] >= 0 && t[u] < p.classes;
-      keep[u] = in && valid;
-      drop[u] = in && !valid;
-      mine += keep[u];
-      if (backward && p.reduction == kCeNone && keep[u]) {
-        const float g = fabsf(p.gout[n]);
-        if (g < THERIA_INF) most = fmaxf(most, g);
-      }
+      t[u] = row_target(p, n0 + u);
+      mine += t[u].keep;
+      if (gradients && !counts && t[u].keep) most = fmaxf(most, kept_gradient(p, n0 + u));
     }
     int upto = mine;  // inclusive sum over the wave's lanes
 #pragma unroll
@@ -89,29 +146,28 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParams p, bool backward
 #pragma unroll
     for (int u = 0; u < kScanPer; ++u) {
       const int64_t n = n0 + u;
-      if (keep[u]) {
+      if (t[u].keep) {
         map[at] = (int)n;
-        target[at] = (int)t[u];
+        target[at] = (int)t[u].target;
         ++at;
-      } else if (drop[u]) {
-        map[p.n - 1 - (n - at)] = t[u] == p.ignore ? (int)n : (int)(-n - 1);
+      } else if (t[u].drop) {
+        map[p.n - 1 - (n - at)] = t[u].target == p.ignore ? (int)n : (int)(-n - 1);
       }
     }
     kept += all;
   }
-  most = fmaxf(most, __shfl_xor(most, 1));
-#pragma unroll
-  for (int o = 2; o < 64; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
-  if (lane == 0) wave_most[wave] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < 16; ++w) most = fmaxf(most, wave_most[w]);
-    meta->kept = (int)kept;
+  if (!counts) {
+    int none = 0;
+    block_count(none, most, red[0]);
+    all_kept = kept;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    meta->kept = all_kept;
     meta->most = most;
     if (backward) {
       const float unit = p.dtype == 1 ? 0x1p-14f : 1.f;
       // no kept row: zero, not the zero over zero of an empty mean
-      meta->factor = kept == 0 ? 0.f : unit * (p.reduction == kCeNone ? most : p.reduction == kCeMean ? p.gout[0] / (float)kept : p.gout[0]);
+      meta->factor = all_kept == 0 ? 0.f : unit * (p.reduction == kCeNone ? most : p.reduction == kCeMean ? p.gout[0] / (float)all_kept : p.gout[0]);
     }
   }
 }
@@ -124,12 +180,21 @@ struct LayTo {
   int* exponent;
   int64_t plane;  // bytes from plane to plane
   int kp;
+  MutRows dx;     // with map: the dropped rows of this matrix become zero, NaN where the target is invalid; or absent
 };
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void ce_lay_kernel(Rows src, int64_t rows, int width, const int* map, const Meta* meta, LayTo to) {
   const int lane = threadIdx.x % 64;
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  if (i >= (map ? (int64_t)meta->kept : rows)) return;
+  if (i >= rows) return;
+  if (map && i >= meta->kept) {
+    const int m = map[i];
+    if (!to.dx.p) return;
+    const T fill = m < 0 ? (T)__builtin_nanf("") : (T)0.f;
+    T* row = (T*)to.dx.p + (m < 0 ? -(int64_t)m - 1 : (int64_t)m) * to.dx.sr;
+    for (int c = lane; c < width; c += 64) row[c] = fill;
+    return;
+  }
   const T* row = (const T*)src.p + (map ? (int64_t)map[i] : i) * src.sr;
   RawVec<T, 8> raw;
   int scale = 0;
@@ -448,12 +513,17 @@ struct SumTile {
   }
 };
 
-// The tile times the factor, in the output's type.
+// The tile times the factor, in the output's type. Rows j go to map[j] where there is a map, and `rest` is as in
+// ce_join_rows_kernel.
 template <typename T>
 struct OutTile {
   T* out;
   int64_t sr;
   const Meta* meta;
+  const int* map;
+  const float* rest;
+  const int* target;
+  Rows w;
 
   template <class S>
   __device__ __forceinline__ void start(f32x16_t (&z)[S::FI][S::FJ], const GemmTile&) const {
@@ -463,6 +533,25 @@ struct OutTile {
   __device__ __forceinline__ void run(f32x16_t (&z)[S::FI][S::FJ], const GemmTile& t, char* lds) const {
     const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
     const float f = meta->factor;
+    if (rest) {
+#pragma unroll
+      for (int fj = 0; fj < S::FJ; ++fj) {
+        const int j = t.j0 + 32 * fj + li;
+        const float left = j < t.J ? rest[j] : 0.f;
+        if (left == 0.f) continue;
+        const T* row = (const T*)w.p + target[j] * w.sr;
+#pragma unroll
+        for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int i = t.i0 + 32 * fi + 8 * q + 4 * g;
+            float f4[4];
+            load_quad(f4, row + i, t.I - i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[fi][fj][4 * q + e] += left * f4[e];
+          }
+      }
+    }
     using Stage = GemmStage<S, (int)sizeof(T)>;
     // the share holds every row of 16-bit results, or one block's rows of float32 ones
     constexpr int kBlocks = sizeof(T) == 2 ? S::FJ : 1, kPer = 16 / (int)sizeof(T);
@@ -482,7 +571,7 @@ struct OutTile {
       const int j0 = t.j0 + 32 * f0;
       Stage::each(lds, 32 * kBlocks, [&](int r, int i, const i32x4_t& c) {
         if (j0 + r >= t.J || t.i0 + i >= t.I) return;
-        T* to = out + (j0 + r) * sr + t.i0 + i;
+        T* to = out + (map ? (int64_t)map[j0 + r] : (int64_t)(j0 + r)) * sr + t.i0 + i;
         RawVec<T, kPer> v;
         __builtin_memcpy(v.v, &c, 16);
         v.store(to, t.I - t.i0 - i);
@@ -542,56 +631,41 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeParams p, int tiles, con
 __global__ __launch_bounds__(1024) void ce_total_kernel(CeParams p, const float* row_loss, const Meta* meta) {
   __shared__ float red[16];
   float s[1] = {0.f};
+#pragma unroll 8
   for (int64_t n = threadIdx.x; n < p.n; n += 1024) s[0] += row_loss[n];
   team_sum<1024, 1>(s, red);
   if (threadIdx.x == 0) p.loss[0] = p.reduction == kCeMean ? s[0] / (float)meta->kept : s[0];
 }
 
-// out[row] = the sum over the splits of sums[split][i], times the factor. map: rows as in ce_rows_kernel, dropped ones
-// zero (NaN where the target is invalid); without: row i. rest: what the rounding of the kept rows' target entries left, to
-// be added with the target's row of w.
+// out[row] = the sum over the splits of sums[split][i], times the factor. map: row map[i] for each kept row; without: row i.
+// rest: what the rounding of the kept rows' target entries left, to be added with the target's row of w.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_join_rows_kernel(const float* sums, int splits, int64_t rows, int ld, int width, const int* map,
                                                            const Meta* meta, T* out, int64_t sr, const float* rest,
                                                            const int* target, Rows w) {
   const int c = blockIdx.y * 512 + threadIdx.x % 64 * 8;
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  if (i >= rows || c >= width) return;
-  int64_t row = i;
-  bool have = true;
-  float fill = 0.f;
-  if (map) {
-    const int m = map[i];
-    have = i < meta->kept;
-    row = m < 0 ? -(int64_t)m - 1 : m;
-    fill = m < 0 ? __builtin_nanf("") : 0.f;
-  }
-  const float f = meta->factor;
-  const float left = rest && have ? rest[i] : 0.f;
-  const T* row_w = left != 0.f ? (const T*)w.p + target[i] * w.sr : nullptr;
-  float v[8];
-  RawVec<T, 8> o;
-  if (have) {
-    f32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;  // ld is a multiple of 8
+  if (i >= (map ? (int64_t)meta->kept : rows) || c >= width) return;
+  const float f = meta->factor, left = rest ? rest[i] : 0.f;
+  f32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;  // ld is a multiple of 8
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-      const f32x4_t* from = reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
-      a += from[0], b += from[1];
-    }
+  for (int s = 0; s < splits; ++s) {
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(sums + (s * rows + i) * ld + c);
+    a += from[0], b += from[1];
+  }
+  float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  RawVec<T, 8> o;
+  if (left != 0.f) {
+    float w8[8];
+    o.load((const T*)w.p + target[i] * w.sr + c, width - c);
+    o.get(w8);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
-    if (row_w) {
-      float w8[8];
-      o.load(row_w + c, width - c);
-      o.get(w8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += left * w8[e];
-    }
+    for (int e = 0; e < 8; ++e) v[e] += left * w8[e];
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = have ? v[e] * f : fill;
+  for (int e = 0; e < 8; ++e) v[e] *= f;
   o.set(v);
-  o.store(out + row * sr + c, width - c);
+  o.store(out + (map ? (int64_t)map[i] : i) * sr + c, width - c);
 }
 
 // Column sums of a piece's dz: a thread adds eight columns over its share of the kept rows.
@@ -622,7 +696,7 @@ int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // Product tiles, and parts of k for products with few of them. A workgroup of 256 x 256 holds a CU by itself and reads half
 // the operand bytes of 128 x 128 for each product; two of those share a CU, and one's epilogue runs beside the other's
-// products. Up to 64 rows: 128 x 64.
+// products. Up to 64 rows, and for float32 operands as they are: 128 x 64.
 enum class Tile { kFew, kMid, kLarge };
 int tile_i(Tile t) { return t == Tile::kLarge ? 256 : 128; }
 int tile_j(Tile t) { return t == Tile::kLarge ? 256 : t == Tile::kMid ? 128 : 64; }
@@ -636,21 +710,22 @@ struct Pick {
 // The pick with the least time for I x J results of K k by a model of the measured kernels, in us: a step of 64 k takes 1.65
 // in a large workgroup, 1.1 in two small ones on a CU and 0.9 in one alone, an epilogue 6 and 3, and a part's float32 sums
 // are written and read at 4.5 TB/s. (Before, large tiles wherever they alone filled the GPU, dx of (4096, 32000, 1024)
-// bfloat16 took XXPICK; forward of (2000, 10000, 512) takes 48 us in small tiles and 54 us in large ones, of (4096,
+// bfloat16 took 461 us, and takes 264 us in four parts; forward of (2000, 10000, 512) takes 48 us in small tiles and 54 us in large ones, of (4096,
 // 32000, 512) 181 and 172.) parts: most parts of k. Parts have at least 8 steps.
 Pick pick(int64_t I, int64_t J, int64_t K, int segments, bool few, bool large, bool parts) {
   const int64_t cus = device_cu_count();
-  if (I == 0 || J == 0) return {few && J <= 64 ? Tile::kFew : Tile::kMid, 1};
-  const int64_t most = !parts ? 1 : K / 512 < 1 ? 1 : K / 512 < 32 ? K / 512 : 32;
-  if ((few && J <= 64) || !large) {
+  const bool narrow = few && (J <= 64 || !large);
+  if (I == 0 || J == 0) return {narrow ? Tile::kFew : Tile::kMid, 1};
+  const int64_t most = !parts || K < 1024 ? 1 : K / 512 < 256 ? K / 512 : 256;
+  if (narrow || !large) {
     // bound by reading one operand, or by few products: parts until there are two workgroups for each CU
-    const Tile t = few && J <= 64 ? Tile::kFew : Tile::kMid;
+    const Tile t = narrow ? Tile::kFew : Tile::kMid;
     const int64_t tiles = tiles_of(t, I, J), want = tiles >= cus ? 1 : (2 * cus + tiles - 1) / tiles;
     return {t, (int)(want < most ? want : most)};
   }
   Pick best{Tile::kLarge, 1};
   double least = 1e30;
-  for (int s = 1; s <= (most < 16 ? most : 16); ++s) {
+  for (int s = 1; s <= most; s += s < 4 ? 1 : s < 16 ? s / 4 : s / 2) {
     const double steps = (double)((K + 64 * s - 1) / (64 * s)) * segments, sums = parts && s > 1 ? s * 8.0 * I * J / 4.5e6 : 0;
     const int64_t nl = tiles_of(Tile::kLarge, I, J) * s, nm = tiles_of(Tile::kMid, I, J) * s;
     const double tl = (double)((nl + cus - 1) / cus) * (1.65 * steps + 6) + sums;
@@ -669,10 +744,11 @@ struct Layout {
   int64_t piece;    // classes of a piece
   int ldz;          // of a piece's dz
   Pick f, x, w;     // of the logits, dx, dW
+  bool direct_x;    // dx leaves its product finished: one piece, one part
   int ldx;          // of the float32 sums
   int tiles;        // of classes, over all pieces
   int bias_parts;
-  int64_t map, target, meta, xs, xs_grad, ws_w, ws_w_grad, ex_x, ex_w, at_target, part, row_loss, rest, dz, sum_x, sum_w, bias_part, bytes;
+  int64_t map, target, counts, meta, xs, xs_grad, ws_w, ws_w_grad, ex_x, ex_w, at_target, part, row_loss, rest, dz, sum_x, sum_w, bias_part, bytes;
 };
 
 Layout layout_of(const CeParams& p, bool backward) {
@@ -696,6 +772,7 @@ Layout layout_of(const CeParams& p, bool backward) {
   l.f = pick(l.piece, p.n, p.width, segments_l, true, !native, false);
   l.x = pick(p.width, p.n, l.piece, segments_g, true, !native, true);
   l.w = pick(p.width, l.piece, p.n, segments_g, false, !native, true);
+  l.direct_x = l.piece >= p.classes && l.x.splits == 1;
   l.ldx = (int)up(p.width, 8);
   l.bias_parts = (int)(p.n < 64 ? 1 : p.n / 64 < 64 ? p.n / 64 : 64);
   for (int64_t v = 0; v < p.classes; v += l.piece)
@@ -708,6 +785,7 @@ Layout layout_of(const CeParams& p, bool backward) {
   l.meta = take(sizeof(Meta));
   l.map = take(4 * p.n);
   l.target = take(4 * p.n);
+  l.counts = take(sizeof(RowCount) * (p.n / kScan + 1));
   l.xs = take(bl * p.n * l.kp);
   if (l.lay_w) l.ws_w = take(bl * l.piece * l.kp);
   if (l.planes) {
@@ -722,7 +800,7 @@ Layout layout_of(const CeParams& p, bool backward) {
   } else {
     l.rest = take(4 * p.n);
     l.dz = take(bg * p.n * l.ldz);
-    if (p.dx.p) l.sum_x = take(4 * l.x.splits * p.n * l.ldx);
+    if (p.dx.p && !l.direct_x) l.sum_x = take(4 * l.x.splits * p.n * l.ldx);
     if (p.dw.p && l.w.splits > 1) l.sum_w = take(4 * l.w.splits * l.piece * l.ldx);
     if (p.db) l.bias_part = take(4 * (int64_t)l.bias_parts * l.ldz);
   }
@@ -780,21 +858,30 @@ struct Call {
     if (l.lay_w) return {ws + (across && SPLIT ? l.ws_w_grad : l.ws_w), ES * (int64_t)l.kp, plane_w(), across ? l.kp : have};
     return {(const char*)p.w.p + v * p.w.sr * ES, ES * p.w.sr, 0, across ? p.width : have};
   }
+  const float* rest() const { return sizeof(T) == 4 ? nullptr : (const float*)(ws + l.rest); }
   LogitBase<T, SPLIT> base(int64_t v) const {
     return {p.bias ? (const T*)p.bias + v : nullptr, v, target, (const int*)(ws + l.ex_w), (const int*)(ws + l.ex_x)};
   }
 
   hipError_t rows(bool backward) {
-    ce_rows_kernel<<<1, 1024, 0, st>>>(p, backward, map, target, meta);
+    // many rows: counted first, so that several workgroups can list them (100000: 87 -> 12 us)
+    if (p.n > 4 * kScan) {
+      const unsigned blocks = (unsigned)((p.n + kScan - 1) / kScan);
+      RowCount* counts = (RowCount*)(ws + l.counts);
+      ce_count_kernel<<<blocks, 1024, 0, st>>>(p, backward && p.reduction == kCeNone, counts);
+      ce_rows_kernel<<<blocks, 1024, 0, st>>>(p, backward, counts, map, target, meta);
+    } else {
+      ce_rows_kernel<<<1, 1024, 0, st>>>(p, backward, nullptr, map, target, meta);
+    }
     THERIA_TRY(hipGetLastError());
     if (p.n == 0) return hipSuccess;
-    ce_lay_kernel<T, SPLIT><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, LayTo{ws + l.xs, backward && SPLIT ? ws + l.xs_grad : nullptr, (int*)(ws + l.ex_x), plane_x(), l.kp});
+    ce_lay_kernel<T, SPLIT><<<dim3((unsigned)((p.n + 3) / 4)), 256, 0, st>>>(p.x, p.n, p.width, map, meta, LayTo{ws + l.xs, backward && SPLIT ? ws + l.xs_grad : nullptr, (int*)(ws + l.ex_x), plane_x(), l.kp, backward ? p.dx : MutRows{}});
     return hipGetLastError();
   }
   hipError_t lay_piece(bool backward, int64_t v, int have) {
     if (!l.lay_w) return hipSuccess;
     const Rows src{(const T*)p.w.p + v * p.w.sr, p.w.sr};
-    ce_lay_kernel<T, SPLIT><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, LayTo{ws + l.ws_w, backward && SPLIT ? ws + l.ws_w_grad : nullptr, (int*)(ws + l.ex_w), plane_w(), l.kp});
+    ce_lay_kernel<T, SPLIT><<<dim3((unsigned)((have + 3) / 4)), 256, 0, st>>>(src, have, p.width, nullptr, meta, LayTo{ws + l.ws_w, backward && SPLIT ? ws + l.ws_w_grad : nullptr, (int*)(ws + l.ex_w), plane_w(), l.kp, MutRows{}});
     return hipGetLastError();
   }
 
@@ -837,14 +924,18 @@ struct Call {
       }
       if (p.dx.p) {
         const GemmParams g{w_operand(true, v, have), z_operand(false), p.width, (int)p.n, have, l.x.splits, kGradSegments, &meta->kept, true, false};
-        const SumTile e{(float*)(ws + l.sum_x), p.n, l.ldx, v > 0};
-        THERIA_TRY((gemm<H, true, false>(l.x.tile, g, e, st)));
+        if (l.direct_x) {
+          THERIA_TRY((gemm<H, true, false>(l.x.tile, g, OutTile<T>{(T*)p.dx.p, p.dx.sr, meta, map, rest(), target, p.w}, st)));
+        } else {
+          const SumTile e{(float*)(ws + l.sum_x), p.n, l.ldx, v > 0};
+          THERIA_TRY((gemm<H, true, false>(l.x.tile, g, e, st)));
+        }
       }
       if (p.dw.p) {
         T* out = (T*)p.dw.p + v * p.dw.sr;
         const GemmParams g{x_operand(true), z_operand(true), p.width, have, (int)p.n, l.w.splits, kGradSegments, &meta->kept, false, true};
         if (l.w.splits == 1) {
-          THERIA_TRY((gemm<H, true, true>(l.w.tile, g, OutTile<T>{out, p.dw.sr, meta}, st)));
+          THERIA_TRY((gemm<H, true, true>(l.w.tile, g, OutTile<T>{out, p.dw.sr, meta, nullptr, nullptr, nullptr, Rows{}}, st)));
         } else {
           float* sums = (float*)(ws + l.sum_w);
           THERIA_TRY((gemm<H, true, true>(l.w.tile, g, SumTile{sums, l.piece, l.ldx, false}, st)));
@@ -860,8 +951,8 @@ struct Call {
         THERIA_TRY(hipGetLastError());
       }
     }
-    if (p.dx.p && p.n > 0) {
-      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4), (p.width + 511) / 512), 256, 0, st>>>((const float*)(ws + l.sum_x), l.x.splits, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, sizeof(T) == 4 ? nullptr : (const float*)(ws + l.rest), target, p.w);
+    if (p.dx.p && p.n > 0 && !l.direct_x) {
+      ce_join_rows_kernel<T><<<dim3((unsigned)((p.n + 3) / 4), (p.width + 511) / 512), 256, 0, st>>>((const float*)(ws + l.sum_x), l.x.splits, p.n, l.ldx, p.width, map, meta, (T*)p.dx.p, p.dx.sr, rest(), target, p.w);
       THERIA_TRY(hipGetLastError());
     }
     return hipSuccess;

@@ -91,6 +91,21 @@ struct RawVec {
   }
 };
 
+// Four consecutive values as float32, zeros behind the first `have`; memory aligned to its elements.
+template <typename T>
+__device__ __forceinline__ void load_quad(float (&f)[4], const T* p, int have) {
+  T t[4] = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
+  if (have >= 4) {
+    __builtin_memcpy(t, p, sizeof(t));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < have) t[e] = p[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = (float)t[e];
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float x) {
   return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
