@@ -50,6 +50,23 @@ def test_rows_and_gradient_match_float64(dt, N, V, D, hip_device):
         _check(_ids(N, V, kind, N).to(hip_device), w, g, 1.5, None, kind)
 
 
+@pytest.mark.parametrize("N,V", [(131072, 3000), (131073, 3000), (200003, 70000)])
+def test_many_tokens(N, V, hip_device):
+    """On both sides of the radix sort's change to tiles of 4096 tokens."""
+    gen = torch.Generator().manual_seed(N)
+    w, g = torch.randn(V, 8, generator=gen).to(hip_device), torch.randn(N, 8, generator=gen).to(hip_device)
+    for kind in ("uniform", "zipf"):
+        _check(_ids(N, V, kind, N).to(hip_device), w, g, 1.0, 1, f"{kind} {N}")
+
+
+def test_lookup_in_several_launches(hip_device):
+    """More ids than a launch takes (2^23)."""
+    N = 2**23 + 5
+    gen = torch.Generator().manual_seed(1)
+    w, ids = torch.randn(100, 3, generator=gen).half().to(hip_device), torch.randint(0, 100, (N,), generator=gen).int().to(hip_device)
+    assert torch.equal(hip_embedding(ids, w), w[ids.long()])
+
+
 @pytest.mark.parametrize("D", [16, 64, 200, 1500, 4096])
 @pytest.mark.parametrize("N", [64, 127, 5000, 20001])
 def test_one_id_for_every_token_and_rising_ids(N, D, hip_device):

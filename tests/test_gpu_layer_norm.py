@@ -123,6 +123,17 @@ def test_one_row_as_a_vector_and_no_rows(hip_device):
     assert gx.shape == (0, 5, 40) and not gw.any()
 
 
+def test_forward_in_several_launches(hip_device):
+    """More rows than a launch takes (2^21)."""
+    rows = 2**21 + 3
+    x, w, b, g, *_ = _make((rows, 2), torch.float32, torch.float32, hip_device, seed=9)
+    xl, wl, bl = _leaves(x, w, b)
+    y, first = _first(xl, wl, bl, g)
+    O.check(y, *O.norm_forward(x, w, b, EPS), "y")
+    for n, got, (v, t) in zip(("dx", "dw", "db"), first, O.norm_backward(x, w, g, EPS, torch.float32)):
+        O.check(got, v, t, n)
+
+
 def test_constant_rows_and_values_far_from_zero(hip_device):
     """A row without variance is all bias; a row around 1000 keeps its variance (no sum of squares)."""
     x = torch.full((3, 130), 7.0, device=hip_device)

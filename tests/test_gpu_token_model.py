@@ -111,6 +111,16 @@ def test_transforms_and_forward_mode_are_refused(hip_device):
             fwAD.unpack_dual(call(x, fwAD.make_dual(w, torch.ones_like(w)))).tangent.sum()
 
 
+def test_inference_mode_and_no_grad_give_the_same(hip_device):
+    x, w, calls = _calls(hip_device)
+    for call in calls:
+        ref = call(x, w.clone().requires_grad_(True))
+        with torch.no_grad():
+            assert torch.equal(call(x, w), ref.detach())
+        with torch.inference_mode():
+            assert torch.equal(call(x.clone(), w.clone()), ref.detach())
+
+
 def test_inputs_changed_after_the_forward_are_noticed(hip_device):
     x, w, calls = _calls(hip_device)
     for call, changed in zip(calls[:1] + calls[2:], (x, w)):
