@@ -23,38 +23,89 @@ namespace {
 template <int TPR>
 constexpr int kBlock = TPR > 256 ? TPR : 256;
 
-// TAIL: the width is no multiple of VEC, so that a row's last vector is partly filled (a template parameter, since the
-// branch costs whole vectors too: backward of (8192, 4096) bfloat16 56 us with it, 45 us without).
-//
+// How a row's last vector is filled (a template parameter: a branch around loads costs whole vectors too, backward of (8192, 4096)
+// bfloat16 56 us with one, 45 us without).
+enum Tail {
+  kWhole,  // the width is a multiple of VEC
+  kOver,   // it is not: the last vector is loaded from VEC before the row's end and shifted when it is used. Loads of
+           // single elements are waited for where they stand, and every load before them too: backward of (130000, 1001)
+           // bfloat16 170 us against 153 us, of (80000, 1500) 221 against 150.
+  kSingle  // the width is below VEC: single elements
+};
+
 // The columns that thread t of a team holds: NPT vectors of VEC, TPR vectors apart.
 template <int VEC, int TPR>
 __device__ __forceinline__ int col_of(int i, int t) {
   return (i * TPR + t) * VEC;
 }
 
-template <typename T, int VEC, int NPT, int TPR, bool TAIL>
+// The vector at column c of a row (zeros where there is none), and its values.
+template <Tail TAIL, typename T, int VEC>
+__device__ __forceinline__ void load_vec(RawVec<T, VEC>& raw, const T* row, int c, int width, bool live) {
+  if constexpr (TAIL == kOver)
+    raw.template load<false>(row + (c + VEC > width ? width - VEC : c), live ? width - c : 0);
+  else
+    raw.template load<TAIL == kSingle>(row + c, live ? width - c : 0);
+}
+template <Tail TAIL, typename T, int VEC>
+__device__ __forceinline__ void values_of(float (&f)[VEC], RawVec<T, VEC> raw, int c, int width) {
+  if (TAIL == kOver && c < width && c + VEC > width) raw.shift_down(VEC - width % VEC);
+  raw.get(f);
+}
+
+template <typename T, int VEC, int NPT, int TPR, Tail TAIL>
 __device__ __forceinline__ void load_row(RawVec<T, VEC> (&raw)[NPT], const T* row, int t, int width, bool live) {
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) {
-    const int c = col_of<VEC, TPR>(i, t);
-    raw[i].template load<TAIL>(row + c, live ? width - c : 0);
-  }
+  for (int i = 0; i < NPT; ++i) load_vec<TAIL>(raw[i], row, col_of<VEC, TPR>(i, t), width, live);
+}
+template <typename T, int VEC, int NPT, int TPR, Tail TAIL>
+__device__ __forceinline__ void values(float (&f)[NPT][VEC], const RawVec<T, VEC> (&raw)[NPT], int t, int width) {
+#pragma unroll
+  for (int i = 0; i < NPT; ++i) values_of<TAIL>(f[i], raw[i], col_of<VEC, TPR>(i, t), width);
 }
 
 // VEC parameters from column c, or the given constant where the parameter is absent.
-template <typename WT, int VEC, bool TAIL>
+template <typename WT, int VEC, Tail TAIL>
 __device__ __forceinline__ void load_param(float (&f)[VEC], const void* p, int c, int width, float absent) {
   if (p) {
     RawVec<WT, VEC> r;
-    r.template load<TAIL>((const WT*)p + c, width - c);
-    r.get(f);
+    load_vec<TAIL>(r, (const WT*)p, c, width, true);
+    values_of<TAIL>(f, r, c, width);
   } else {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = absent;
   }
 }
 
-template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
+// A parameter's columns of a thread: held in registers (HOLD) by a team that walks its rows with the next row's loads on
+// their way. Vector memory answers in order, so that a load behind those would wait for that row, too. Backward of (65536,
+// 2048) bfloat16 173 -> 151 us, float32 301 -> 285 us.
+template <typename WT, int VEC, int NPT, int TPR, Tail TAIL, bool HOLD>
+struct HeldParam {
+  const void* p;
+  int t, width;
+  float absent;
+  RawVec<WT, VEC> raw[HOLD ? NPT : 1];
+
+  __device__ __forceinline__ HeldParam(const void* p_, int t_, int width_, float absent_) : p(p_), t(t_), width(width_), absent(absent_) {
+    if constexpr (HOLD) {
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        float f[VEC];
+        load_param<WT, VEC, TAIL>(f, p, col_of<VEC, TPR>(i, t), width, absent);
+        raw[i].set(f);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[VEC], int i) const {
+    if constexpr (HOLD)
+      raw[i].get(f);
+    else
+      load_param<WT, VEC, TAIL>(f, p, col_of<VEC, TPR>(i, t), width, absent);
+  }
+};
+
+template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
   constexpr int TEAMS = kBlock<TPR> / TPR;
   __shared__ float red[2][16];
@@ -64,13 +115,12 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
   RawVec<T, VEC> raw[NPT];
   load_row<T, VEC, NPT, TPR, TAIL>(raw, (const T*)p.x.p + row * p.x.sr, t, p.width, live);
   float x[NPT][VEC];
+  values<T, VEC, NPT, TPR, TAIL>(x, raw, t, p.width);
   float s[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) {
-    raw[i].get(x[i]);
+  for (int i = 0; i < NPT; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s[0] += x[i][e];
-  }
   team_sum<TPR, 1>(s, red[0]);
   const float mean = s[0] / (float)p.width;
   // the variance from the centred values: no cancellation for rows far from zero
@@ -81,7 +131,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       x[i][e] -= mean;
-      q[0] += e * TAIL < have ? x[i][e] * x[i][e] : 0.f;
+      q[0] += (TAIL == kWhole ? have > 0 : e < have) ? x[i][e] * x[i][e] : 0.f;
     }
   }
   team_sum<TPR, 1>(q, red[1]);
@@ -98,7 +148,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
     for (int e = 0; e < VEC; ++e) x[i][e] = x[i][e] * rstd * w[e] + b[e];
     RawVec<T, VEC> out;
     out.set(x[i]);
-    out.template store<TAIL>((T*)p.y.p + row * p.y.sr + c, p.width - c);
+    out.template store<TAIL != kWhole>((T*)p.y.p + row * p.y.sr + c, p.width - c);
   }
   if (t == 0) {
     p.mean[row] = mean;
@@ -146,9 +196,10 @@ __device__ __forceinline__ void write_partial(float (&acc)[NPT][VEC], float* out
 template <int VEC, int NPT, int TPR>
 constexpr int kPartialLds = TPR <= 64 ? 4 * VEC * NPT * TPR : 1;
 
-template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
+template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   constexpr int TEAMS = kBlock<TPR> / TPR;
+  constexpr bool HOLD = !(TPR == 1024 && NPT == 4);  // which has no registers left for the weight
   __shared__ float red[2][2 * 16];
   __shared__ float lds[kPartialLds<VEC, NPT, TPR>];
   const int t = threadIdx.x % TPR, width = p.width;
@@ -160,33 +211,34 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
 
+  const HeldParam<WT, VEC, NPT, TPR, TAIL, HOLD> weight(p.weight, t, width, 1.f);
   const int64_t step = (int64_t)gridDim.x * TEAMS;
   int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
   RawVec<T, VEC> rx[NPT], rg[NPT];
-  load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + row * p.x.sr, t, width, row < p.rows);
-  load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + row * p.dout.sr, t, width, row < p.rows);
+  float next_mean = 0.f, next_rstd = 0.f;
+  const auto fetch = [&](int64_t r) {
+    const bool live = r < p.rows;
+    if (live) next_mean = p.mean[r], next_rstd = p.rstd[r];
+    load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + r * p.x.sr, t, width, live);
+    load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + r * p.dout.sr, t, width, live);
+  };
+  fetch(row);
   int turn = 0;
   // teams of a wave leave the loop apart; a workgroup-wide team leaves it as one (its row is the workgroup's)
 #pragma unroll 1
-  while (row < p.rows) {
+  for (; row < p.rows; row += step) {
     float x[NPT][VEC], g[NPT][VEC];
-#pragma unroll
-    for (int i = 0; i < NPT; ++i) {
-      rx[i].get(x[i]);
-      rg[i].get(g[i]);
-    }
-    // the next row's loads go out before this row's sums
-    const int64_t next = row + step;
-    load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + next * p.x.sr, t, width, next < p.rows);
-    load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + next * p.dout.sr, t, width, next < p.rows);
-    const float mean = p.mean[row], rstd = p.rstd[row];
+    values<T, VEC, NPT, TPR, TAIL>(x, rx, t, width);
+    values<T, VEC, NPT, TPR, TAIL>(g, rg, t, width);
+    const float mean = next_mean, rstd = next_rstd;
+    fetch(row + step);  // before this row's sums
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NPT; ++i) {
       const int c = col_of<VEC, TPR>(i, t);
       if (c < width) {
         float w[VEC];
-        load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
+        weight.get(w, i);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[i][e] = (x[i][e] - mean) * rstd;
@@ -210,11 +262,10 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
           for (int e = 0; e < VEC; ++e) g[i][e] = rstd * (g[i][e] - m1 - x[i][e] * m2);
           RawVec<T, VEC> out;
           out.set(g[i]);
-          out.template store<TAIL>((T*)p.dx.p + row * p.dx.sr + c, width - c);
+          out.template store<TAIL != kWhole>((T*)p.dx.p + row * p.dx.sr + c, width - c);
         }
       }
     }
-    row = next;
   }
   if (!sums) return;
   float* part = p.ws + (int64_t)blockIdx.x * 2 * width;
@@ -222,9 +273,10 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   write_partial<VEC, NPT, TPR>(db, part + width, width, lds);
 }
 
-template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
+template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
 __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p) {
   constexpr int TEAMS = kBlock<TPR> / TPR;
+  constexpr bool AHEAD = TPR < 1024;  // the next row's loads and the parameters in registers: 1024 threads have too few
   __shared__ float red[2][7 * 16];
   __shared__ float lds[kPartialLds<VEC, NPT, TPR>];
   const int t = threadIdx.x % TPR, width = p.width;
@@ -235,27 +287,38 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) gw_sum[i][e] = 0.f;
 
+  const HeldParam<WT, VEC, NPT, TPR, TAIL, AHEAD> weight(p.weight, t, width, 1.f), gdw(p.gdw, t, width, 0.f), gdb(p.gdb, t, width, 0.f);
+  const int64_t step = (int64_t)gridDim.x * TEAMS;
+  int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
+  RawVec<T, VEC> rx[NPT], rg[NPT], ru[NPT];
+  float next_mean = 0.f, next_rstd = 0.f;
+  const auto fetch = [&](int64_t r) {
+    const bool live = r < p.rows;
+    if (live) next_mean = p.mean[r], next_rstd = p.rstd[r];
+    load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + r * p.x.sr, t, width, live);
+    load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + r * p.dout.sr, t, width, live);
+    load_row<T, VEC, NPT, TPR, TAIL>(ru, (const T*)p.gdx.p + r * p.gdx.sr, t, width, live && p.gdx.p);
+  };
+  if constexpr (AHEAD) fetch(row);
   int turn = 0;
 #pragma unroll 1
-  for (int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * TEAMS) {
-    RawVec<T, VEC> rx[NPT], rg[NPT], ru[NPT];
-    load_row<T, VEC, NPT, TPR, TAIL>(rx, (const T*)p.x.p + row * p.x.sr, t, width, true);
-    load_row<T, VEC, NPT, TPR, TAIL>(rg, (const T*)p.dout.p + row * p.dout.sr, t, width, true);
-    load_row<T, VEC, NPT, TPR, TAIL>(ru, (const T*)p.gdx.p + row * p.gdx.sr, t, width, p.gdx.p != nullptr);
-    const float mean = p.mean[row], rstd = p.rstd[row];
+  for (; row < p.rows; row += step) {
+    if constexpr (!AHEAD) fetch(row);
     float x[NPT][VEC], g[NPT][VEC], u[NPT][VEC];
+    values<T, VEC, NPT, TPR, TAIL>(x, rx, t, width);
+    values<T, VEC, NPT, TPR, TAIL>(g, rg, t, width);
+    values<T, VEC, NPT, TPR, TAIL>(u, ru, t, width);
+    const float mean = next_mean, rstd = next_rstd;
+    if constexpr (AHEAD) fetch(row + step);
     // sums over the row: gw, gw xh, u, u xh, u gw, a dout, a dout xh
     float s[7] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NPT; ++i) {
       const int c = col_of<VEC, TPR>(i, t);
-      rx[i].get(x[i]);
-      rg[i].get(g[i]);
-      ru[i].get(u[i]);
       if (c < width) {
         float w[VEC], a[VEC];
-        load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
-        load_param<WT, VEC, TAIL>(a, p.gdw, c, p.width, 0.f);
+        weight.get(w, i);
+        gdw.get(a, i);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[i][e] = (x[i][e] - mean) * rstd;
@@ -282,9 +345,9 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
       const int c = col_of<VEC, TPR>(i, t);
       if (c >= width) continue;
       float w[VEC], a[VEC], b[VEC];
-      load_param<WT, VEC, TAIL>(w, p.weight, c, p.width, 1.f);
-      load_param<WT, VEC, TAIL>(a, p.gdw, c, p.width, 0.f);
-      load_param<WT, VEC, TAIL>(b, p.gdb, c, p.width, 0.f);
+      weight.get(w, i);
+      gdw.get(a, i);
+      gdb.get(b, i);
       float gx[VEC], gg[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -297,11 +360,11 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
       RawVec<T, VEC> out;
       if (p.out_gx.p) {
         out.set(gx);
-        out.template store<TAIL>((T*)p.out_gx.p + row * p.out_gx.sr + c, width - c);
+        out.template store<TAIL != kWhole>((T*)p.out_gx.p + row * p.out_gx.sr + c, width - c);
       }
       if (p.out_gdout.p) {
         out.set(gg);
-        out.template store<TAIL>((T*)p.out_gdout.p + row * p.out_gdout.sr + c, width - c);
+        out.template store<TAIL != kWhole>((T*)p.out_gdout.p + row * p.out_gdout.sr + c, width - c);
       }
     }
   }
@@ -323,23 +386,28 @@ Plan plan_of(const NormParams& p) {
 // Teams of a workgroup.
 int teams_of(const Plan& pl) { return pl.tpr >= 256 ? 1 : 256 / pl.tpr; }
 
-// Workgroups of a launch that sums over the rows. More hide more latency and write more partial rows, eight bytes of traffic
-// a column each: two a CU while those are over a fourteenth of the rows' own bytes, up to four (16-bit) or three. Teams of
-// 1024 threads, one a CU. Backward in us with 1, 2, 3, 4, 6 a CU: (8192, 4096) bfloat16 69, 53, 56, 60, 74; (65536, 2048)
-// bfloat16 371, 214, 175, 169, 168, float32 399, 302, 303, 310, 318; (400000, 64) float32 102, 62, 56, 57, 62; (4096, 16384)
-// bfloat16 109, 131, 159, 188, 244. Fewer where a team would get fewer than two rows.
+// Workgroups of a launch that sums over the rows. A workgroup has the next rows of its teams on their way, 8 KiB of each
+// tensor on a CU hide what latency there is, and every further workgroup writes another partial row: one a CU from
+// 8 KiB of rows on, more below it, and two at least with 16-bit rows, whose unpacking takes longer. Backward in us with 1, 2, 3, 4 a CU:
+// bfloat16 (65536, 2048) 217, 149, 149, 162; (80000, 1500) 326, 193, 149, 144; (130000, 1001) 182, 154, 163, 168; (16384,
+// 4096) 86, 91, 97, 103, its double backward 162, 141, 149, 147; (10^6, 50) 120, 77, 65, 69; float32 (65000, 1001) 143, 157,
+// 161, 164; (200000, 256) 169, 119, 120, 121. With few rows the partial rows count more: (2048, 4096) bfloat16 21, 26, 32, 39,
+// so that a further one has to have six rows for each team (two for the first).
 int walkers(const NormParams& p, const Plan& pl) {
-  const int64_t cus = device_cu_count(), two = 2 * teams_of(pl), want = (p.rows + two - 1) / two;
-  int64_t most = cus;
+  const int64_t cus = device_cu_count(), teams = teams_of(pl), bytes = teams * p.width * (p.dtype == 0 ? 4 : 2);
+  int64_t each = 1;
   if (pl.tpr < 1024) {
-    const int64_t few = 2 * cus, many = (p.dtype == 0 ? pl.tpr == 256 ? 2 : 3 : 4) * cus, cheap = p.rows * (p.dtype == 0 ? 4 : 2) / 76;
-    most = cheap < few ? few : cheap < many ? cheap : many;
+    each = (8192 + bytes - 1) / bytes;
+    if (p.dtype != 0 && each < 2) each = 2;
+    if (each > 4) each = 4;
+    while (each > 1 && p.rows < 6 * teams * each * cus) --each;
   }
+  const int64_t want = (p.rows + 2 * teams - 1) / (2 * teams), most = each * cus;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 struct Fwd {
-  template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
+  template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
   static hipError_t run(const NormParams& p, hipStream_t st) {
     constexpr int TEAMS = kBlock<TPR> / TPR;
     constexpr int64_t most = int64_t(1) << 21;  // rows: a launch holds fewer than 2^32 threads
@@ -364,7 +432,7 @@ hipError_t finish(const NormParams& p, int parts, int64_t cols, void* out0, void
 }
 
 struct Bwd {
-  template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
+  template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
   static hipError_t run(const NormParams& p, hipStream_t st) {
     const int n = walkers(p, Plan{NPT, TPR});
     norm_bwd_kernel<T, WT, VEC, NPT, TPR, TAIL><<<n, kBlock<TPR>, 0, st>>>(p);
@@ -375,7 +443,7 @@ struct Bwd {
 };
 
 struct BwdBwd {
-  template <typename T, typename WT, int VEC, int NPT, int TPR, bool TAIL>
+  template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
   static hipError_t run(const NormParams& p, hipStream_t st) {
     const int n = walkers(p, Plan{NPT, TPR});
     norm_bwd_bwd_kernel<T, WT, VEC, NPT, TPR, TAIL><<<n, kBlock<TPR>, 0, st>>>(p);
@@ -389,9 +457,10 @@ template <typename L, typename T, typename WT>
 hipError_t by_plan(const NormParams& p, hipStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const Plan pl = plan_of(p);
+  if (p.width < V) return L::template run<T, WT, V, 1, 8, kSingle>(p, st);
 #define THERIA_NORM_CASE(NPT, TPR)               \
   if (pl.npt == NPT && pl.tpr == TPR)            \
-    return p.width % V ? L::template run<T, WT, V, NPT, TPR, true>(p, st) : L::template run<T, WT, V, NPT, TPR, false>(p, st);
+    return p.width % V ? L::template run<T, WT, V, NPT, TPR, kOver>(p, st) : L::template run<T, WT, V, NPT, TPR, kWhole>(p, st);
   THERIA_NORM_CASE(1, 8)
   THERIA_NORM_CASE(1, 16)
   THERIA_NORM_CASE(1, 32)

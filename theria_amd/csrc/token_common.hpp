@@ -59,6 +59,21 @@ struct RawVec {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) __builtin_nontemporal_store(v[i], reinterpret_cast<piece_t*>(p) + i);
   }
+  // Values n < VEC places down, zeros behind them.
+  __device__ __forceinline__ void shift_down(int n) {
+    constexpr int N = 4 * kPieces;
+    n *= (int)sizeof(T);
+#pragma unroll
+    for (int by = N / 2; by >= 1; by /= 2) {  // in registers
+      if (!(n & 4 * by)) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i / 4][i % 4] = i + by < N ? v[(i + by) / 4 % kPieces][(i + by) % 4] : 0;
+    }
+    if (sizeof(T) == 2 && (n & 2)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i / 4][i % 4] = v[i / 4][i % 4] >> 16 | (i + 1 < N ? v[(i + 1) / 4 % kPieces][(i + 1) % 4] << 16 : 0);
+    }
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) v[i] = u32x4_t{0, 0, 0, 0};
@@ -161,10 +176,14 @@ __device__ __forceinline__ void team_sum(float (&s)[K], float* red) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float t = red[k * NW];
+      if constexpr (NW == 16) {
+        s[k] = lane_sum<16>(red[k * NW + threadIdx.x % 16]);  // one read for each sum, not sixteen: they would fill the registers
+      } else {
+        float t = red[k * NW];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) t += red[k * NW + w];
-      s[k] = t;
+        for (int w = 1; w < NW; ++w) t += red[k * NW + w];
+        s[k] = t;
+      }
     }
   }
 }
