@@ -14,6 +14,8 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <functional>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -277,9 +279,11 @@ py::tuple bwd_bwd(at::Tensor q, at::Tensor k, at::Tensor v, OptT o, const at::Te
 struct ContractError : std::runtime_error {
   using std::runtime_error::runtime_error;
 };
-void must(bool ok, const std::string& msg) {
-  if (!ok) throw ContractError(msg);
-}
+// The message is only put together where it is thrown: the strings of one operator's checks cost as much as its launch.
+#define THERIA_MUST(ok, msg) \
+  do {                       \
+    if (!(ok)) throw ContractError(msg); \
+  } while (0)
 void token_rc(int rc, const char* what) {
   if (rc == THERIA_OK) return;
   const std::string msg = std::string(what) + ": " + theria_last_error();
@@ -302,23 +306,23 @@ std::string shape_text(const Tensor& t) {
 }
 
 // A torch.func transform wraps its tensors; the C++ Functions know nothing of that.
-void check_plain(const Tensor& t, const char* what) { must(t.has_storage(), std::string(what) + " does not run under torch.func transforms"); }
+void check_plain(const Tensor& t, const char* what) { THERIA_MUST(t.has_storage(), std::string(what) + " does not run under torch.func transforms"); }
 
 // Device, dtype and size contract of the operators' matrices.
 void check_matrix(const Tensor& t, const char* name, const char* what) {
-  must(t.defined(), std::string(what) + ": " + name + " must be a tensor");
-  must(t.is_cuda(), std::string(what) + " requires GPU (HIP) tensors; " + name + " is on " + t.device().str());
+  THERIA_MUST(t.defined(), std::string(what) + ": " + name + " must be a tensor");
+  THERIA_MUST(t.is_cuda(), std::string(what) + " requires GPU (HIP) tensors; " + name + " is on " + t.device().str());
   check_plain(t, what);
   const auto st = t.scalar_type();
-  must(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, std::string("Unsupported dtype for ") + name + ": " + c10::toString(st));
-  must(t.dim() == 0 || t.size(-1) == 0 || t.numel() / t.size(-1) <= kMaxRows, std::string(what) + ": " + name + " has more rows than 32-bit indexes reach");
+  THERIA_MUST(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, std::string("Unsupported dtype for ") + name + ": " + c10::toString(st));
+  THERIA_MUST(t.dim() == 0 || t.size(-1) == 0 || t.numel() / t.size(-1) <= kMaxRows, std::string(what) + ": " + name + " has more rows than 32-bit indexes reach");
 }
 // Ids or targets.
 void check_indexes(const Tensor& t, const char* name, const Tensor& like, const char* what) {
-  must(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, std::string(what) + ": " + name + " must be an int32 or int64 tensor");
-  must(t.device() == like.device(), std::string(what) + ": " + name + " must be on " + like.device().str() + ", got " + t.device().str());
+  THERIA_MUST(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, std::string(what) + ": " + name + " must be an int32 or int64 tensor");
+  THERIA_MUST(t.device() == like.device(), std::string(what) + ": " + name + " must be on " + like.device().str() + ", got " + t.device().str());
   check_plain(t, what);
-  must(t.numel() <= kMaxRows, std::string(what) + ": " + name + " has more elements than 32-bit indexes reach");
+  THERIA_MUST(t.numel() <= kMaxRows, std::string(what) + ": " + name + " has more elements than 32-bit indexes reach");
 }
 
 // A tensor's rows of `width` as a matrix; a copy only where no view with a contiguous last dimension exists.
@@ -331,7 +335,7 @@ Tensor rows_of(const Tensor& t_in, int64_t width) {
 // A gradient or cotangent in the shape and type of `like`; undefined stays undefined.
 Tensor rows_like(const Tensor& t, const Tensor& like, const char* what) {
   if (!t.defined()) return t;
-  must(t.sizes() == like.sizes() && t.device() == like.device(), std::string(what) + ": a gradient must have the shape of its input");
+  THERIA_MUST(t.sizes() == like.sizes() && t.device() == like.device(), std::string(what) + ": a gradient must have the shape of its input");
   return rows_of(t.scalar_type() == like.scalar_type() ? t : t.to(like.scalar_type()), like.size(-1));
 }
 Tensor flat(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
@@ -383,6 +387,14 @@ variable_list unpacked(const variable_list& some, const std::vector<bool>& want)
 Tensor or_empty(const Tensor& t, const Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
 Tensor or_absent(const Tensor& t) { return t.numel() ? t : Tensor(); }
 
+// Whether a call is outside autograd altogether, so that it runs without a Function (0.7 us of its 4 to 6). A forward-mode
+// tangent is not: the Function refuses it.
+bool outside_autograd(std::initializer_list<std::reference_wrapper<const Tensor>> inputs) {
+  for (const Tensor& t : inputs)
+    if (t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())) return false;
+  return true;
+}
+
 std::vector<bool> needed(AutogradContext* ctx) {
   const auto list = ctx->saved_data["need"].toBoolList();
   return std::vector<bool>(list.begin(), list.end());
@@ -393,7 +405,7 @@ theria_layer_norm_problem_t norm_problem(const Tensor& x, at::ScalarType param, 
   return {token_dtype(x.scalar_type()), token_dtype(param), (int32_t)x.size(1), (float)eps, x.size(0)};
 }
 
-variable_list norm_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& dy_in, const Tensor& mean, const Tensor& rstd, double eps,
+variable_list norm_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& dy_in, const Tensor& stats, double eps,
                        at::ScalarType param, bool need_dx, bool need_dw, bool need_db) {
   const int64_t width = x_in.size(-1);
   const Tensor dy = rows_like(dy_in, x_in, "hip_layer_norm"), x = rows_of(x_in, width), weight = flat(weight_in);
@@ -409,13 +421,13 @@ variable_list norm_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor
     if (need_dw || need_db) ws = at::empty({theria_layer_norm_ws_floats(&p)}, x.options().dtype(at::kFloat));
     const auto vx = rows_view(x), vg = rows_view(dy);
     const theria_rows_t vdx{ptr(dx), width};
-    token_rc(theria_layer_norm_bwd(&p, &vx, ptr(weight), &vg, floats(mean), floats(rstd), &vdx, ptr(dw), ptr(db), floats(ws), stream_of(x)),
+    token_rc(theria_layer_norm_bwd(&p, &vx, ptr(weight), &vg, floats(stats), floats(stats) + x.size(0), &vdx, ptr(dw), ptr(db), floats(ws), stream_of(x)),
              "theria_layer_norm_bwd");
   }
   return {dx, dw, db};
 }
 
-variable_list norm_bwd_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& dy_in, const Tensor& mean, const Tensor& rstd, double eps,
+variable_list norm_bwd_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& dy_in, const Tensor& stats, double eps,
                            at::ScalarType param, const Tensor& u_in, const Tensor& a_in, const Tensor& c_in, bool need_gx, bool need_gw,
                            bool need_gdy) {
   const int64_t width = x_in.size(-1);
@@ -423,7 +435,7 @@ variable_list norm_bwd_bwd(const Tensor& x_in, const Tensor& weight_in, const Te
                weight = flat(weight_in);
   auto param_like = [&](const Tensor& t) {
     if (!t.defined()) return t;
-    must(t.numel() == width && t.device() == x.device(), "hip_layer_norm: a cotangent must have the shape of its parameter");
+    THERIA_MUST(t.numel() == width && t.device() == x.device(), "hip_layer_norm: a cotangent must have the shape of its parameter");
     return flat(t.scalar_type() == param ? t : t.to(param));
   };
   const Tensor a = param_like(a_in), c = param_like(c_in);
@@ -439,7 +451,7 @@ variable_list norm_bwd_bwd(const Tensor& x_in, const Tensor& weight_in, const Te
     if (need_gw) ws = at::empty({theria_layer_norm_ws_floats(&p)}, x.options().dtype(at::kFloat));
     const auto vx = rows_view(x), vg = rows_view(dy), vu = rows_view(u);
     const theria_rows_t vgx{ptr(gx), width}, vgdy{ptr(gdy), width};
-    token_rc(theria_layer_norm_bwd_bwd(&p, &vx, ptr(weight), &vg, floats(mean), floats(rstd), &vu, ptr(a), ptr(c), &vgx, ptr(gw), &vgdy,
+    token_rc(theria_layer_norm_bwd_bwd(&p, &vx, ptr(weight), &vg, floats(stats), floats(stats) + x.size(0), &vu, ptr(a), ptr(c), &vgx, ptr(gw), &vgdy,
                                        floats(ws), stream_of(x)),
              "theria_layer_norm_bwd_bwd");
   }
@@ -460,21 +472,21 @@ variable_list norm_map(const variable_list& in, double eps) {
   return {dx.reshape(x_in.sizes()).to(x_in.scalar_type()), (dy * xh).sum(0), dy.sum(0)};
 }
 
-// (x, weight, dy, mean, rstd) -> (dx, dweight, dbias). mean and rstd are functions of x, whose part in the derivative the
+// (x, weight, dy, stats) -> (dx, dweight, dbias). The statistics are functions of x, whose part in the derivative the
 // double backward's kernel includes.
 struct NormBackwardFn : torch::autograd::Function<NormBackwardFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight_in, const Tensor& dy, const Tensor& mean,
-                               const Tensor& rstd, double eps, int64_t param, bool need_dx, bool need_dw, bool need_db) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight_in, const Tensor& dy, const Tensor& stats,
+                               double eps, int64_t param, bool need_dx, bool need_dw, bool need_db) {
     const Tensor weight = or_absent(weight_in);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x, weight_in, dy, mean, rstd});
+    ctx->save_for_backward({x, weight_in, dy, stats});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["param"] = param;
     ctx->saved_data["need"] = std::vector<bool>{need_dx, need_dw, need_db};
-    return packed(norm_bwd(x, weight, dy, mean, rstd, eps, (at::ScalarType)param, need_dx, need_dw, need_db));
+    return packed(norm_bwd(x, weight, dy, stats, eps, (at::ScalarType)param, need_dx, need_dw, need_db));
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& some) {
-    variable_list out(10);
+    variable_list out(9);
     const variable_list g = unpacked(some, needed(ctx));
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
     const auto saved = ctx->get_saved_variables();
@@ -483,25 +495,30 @@ struct NormBackwardFn : torch::autograd::Function<NormBackwardFn> {
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), ny = ctx->needs_input_grad(2);
     const bool keep = at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(dy) || wants(g[0]) || wants(g[1]) || wants(g[2]));
     const variable_list r = keep ? through_map({x, weight, dy}, {nx, nw, ny}, {g[0], g[1], g[2]}, true, [&](const variable_list& in) { return norm_map(in, eps); })
-                                 : norm_bwd_bwd(x, weight, dy, saved[3], saved[4], eps, (at::ScalarType)ctx->saved_data["param"].toInt(), g[0], g[1], g[2], nx, nw, ny);
+                                 : norm_bwd_bwd(x, weight, dy, saved[3], eps, (at::ScalarType)ctx->saved_data["param"].toInt(), g[0], g[1], g[2], nx, nw, ny);
     out[0] = r[0], out[1] = r[1], out[2] = r[2];
     return out;
   }
 };
 
+// y and the statistics (mean, rstd) of each row.
+std::pair<Tensor, Tensor> norm_fwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, double eps, at::ScalarType param) {
+  const int64_t width = x_in.size(-1);
+  const Tensor x = rows_of(x_in, width), weight = flat(weight_in), bias = flat(bias_in);
+  const c10::hip::HIPGuard guard(x.get_device());
+  const Tensor y = at::empty(x_in.sizes(), x.options()), stats = at::empty({2, x.size(0)}, x.options().dtype(at::kFloat));
+  const auto p = norm_problem(x, param, eps);
+  const auto vx = rows_view(x);
+  const theria_rows_t vy{ptr(y), width};
+  token_rc(theria_layer_norm_fwd(&p, &vx, ptr(weight), ptr(bias), &vy, floats(stats), floats(stats) + x.size(0), stream_of(x)), "theria_layer_norm_fwd");
+  return {y, stats};
+}
+
 struct NormFn : torch::autograd::Function<NormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, double eps, int64_t param) {
-    const int64_t width = x_in.size(-1);
-    const Tensor x = rows_of(x_in, width), weight = flat(or_absent(weight_in)), bias = flat(or_absent(bias_in));
-    const c10::hip::HIPGuard guard(x.get_device());
-    const Tensor y = at::empty(x_in.sizes(), x.options());
-    const Tensor mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
-    const auto p = norm_problem(x, (at::ScalarType)param, eps);
-    const auto vx = rows_view(x);
-    const theria_rows_t vy{ptr(y), width};
-    token_rc(theria_layer_norm_fwd(&p, &vx, ptr(weight), ptr(bias), &vy, floats(mean), floats(rstd), stream_of(x)), "theria_layer_norm_fwd");
+    const auto [y, stats] = norm_fwd(x_in, or_absent(weight_in), or_absent(bias_in), eps, (at::ScalarType)param);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x_in, weight_in, mean, rstd});
+    ctx->save_for_backward({x_in, weight_in, stats});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["param"] = param;
     return y;
@@ -515,8 +532,8 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const int64_t param = ctx->saved_data["param"].toInt();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2);
     const variable_list r = at::GradMode::is_enabled()
-                                ? unpacked(NormBackwardFn::apply(x, saved[1], g[0], saved[2], saved[3], eps, param, nx, nw, nb), {nx, nw, nb})
-                                : norm_bwd(x, weight, g[0], saved[2], saved[3], eps, (at::ScalarType)param, nx, nw, nb);
+                                ? unpacked(NormBackwardFn::apply(x, saved[1], g[0], saved[2], eps, param, nx, nw, nb), {nx, nw, nb})
+                                : norm_bwd(x, weight, g[0], saved[2], eps, (at::ScalarType)param, nx, nw, nb);
     out[0] = r[0], out[1] = r[1], out[2] = r[2];
     return out;
   }
@@ -526,19 +543,20 @@ Tensor layer_norm(const Tensor& x, const OptT& weight_in, const OptT& bias_in, d
   const char* what = "hip_layer_norm";
   const Tensor weight = weight_in.value_or(Tensor()), bias = bias_in.value_or(Tensor());
   check_matrix(x, "x", what);
-  must(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxNormWidth,
+  THERIA_MUST(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxNormWidth,
        std::string(what) + " supports rows of 1 to " + std::to_string(kMaxNormWidth) + " elements, got shape " + shape_text(x));
   for (const auto& [name, t] : {std::pair<const char*, const Tensor&>("weight", weight), std::pair<const char*, const Tensor&>("bias", bias)}) {
     if (!t.defined()) continue;
     check_plain(t, what);
-    must(t.dim() == 1 && t.size(0) == x.size(-1), std::string(name) + " must have shape (" + std::to_string(x.size(-1)) + ",), got " + shape_text(t));
-    must((t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat) && t.device() == x.device(),
+    THERIA_MUST(t.dim() == 1 && t.size(0) == x.size(-1), std::string(name) + " must have shape (" + std::to_string(x.size(-1)) + ",), got " + shape_text(t));
+    THERIA_MUST((t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat) && t.device() == x.device(),
          std::string(what) + ": " + name + " must be on " + x.device().str() + " in " + c10::toString(x.scalar_type()) + " or float32, got " +
              c10::toString(t.scalar_type()) + " on " + t.device().str());
   }
-  must(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), std::string(what) + ": weight and bias must have one dtype");
-  must(eps >= 0 && std::isfinite(eps), std::string(what) + ": eps must be finite and not negative, got " + std::to_string(eps));
+  THERIA_MUST(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), std::string(what) + ": weight and bias must have one dtype");
+  THERIA_MUST(eps >= 0 && std::isfinite(eps), std::string(what) + ": eps must be finite and not negative, got " + std::to_string(eps));
   const auto param = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type();
+  if (outside_autograd({x, weight, bias})) return norm_fwd(x, weight, bias, eps, param).first;
   return NormFn::apply(x, or_empty(weight, x), or_empty(bias, x), eps, (int64_t)param);
 }
 
@@ -550,7 +568,7 @@ theria_embedding_problem_t embed_problem(const Tensor& ids, const Tensor& rows, 
 Tensor embed_bwd(const Tensor& ids_in, const Tensor& dout_in, int64_t classes, double scale, int64_t padding) {
   const int64_t width = dout_in.size(-1);
   const Tensor ids = ids_in.contiguous(), dout = rows_of(dout_in, width);
-  must(dout.size(0) == ids.numel() && dout.device() == ids.device(), "hip_embedding: the gradient must have one row for each id");
+  THERIA_MUST(dout.size(0) == ids.numel() && dout.device() == ids.device(), "hip_embedding: the gradient must have one row for each id");
   const c10::hip::HIPGuard guard(dout.get_device());
   const Tensor out = at::empty({classes, width}, dout.options());
   const auto p = embed_problem(ids, dout, classes, scale, padding);
@@ -570,18 +588,23 @@ struct EmbedBackwardFn : torch::autograd::Function<EmbedBackwardFn> {
   static variable_list backward(AutogradContext* ctx, const variable_list& g);
 };
 
+Tensor embed_fwd(const Tensor& table_in, const Tensor& ids_in, double scale, int64_t padding, bool zero_padding) {
+  const int64_t width = table_in.size(1);
+  const Tensor table = rows_of(table_in, width), ids = ids_in.contiguous();
+  const c10::hip::HIPGuard guard(table.get_device());
+  at::DimVector sizes(ids_in.sizes());
+  sizes.push_back(width);
+  const Tensor out = at::empty(sizes, table.options());
+  const auto p = embed_problem(ids, table, table.size(0), scale, padding);
+  const auto vt = rows_view(table);
+  const theria_rows_t vo{ptr(out), width};
+  token_rc(theria_embedding_fwd(&p, ids.data_ptr(), &vt, zero_padding, &vo, stream_of(table)), "theria_embedding_fwd");
+  return out;
+}
+
 struct EmbedFn : torch::autograd::Function<EmbedFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& table_in, const Tensor& ids_in, double scale, int64_t padding, bool zero_padding) {
-    const int64_t width = table_in.size(1);
-    const Tensor table = rows_of(table_in, width), ids = ids_in.contiguous();
-    const c10::hip::HIPGuard guard(table.get_device());
-    auto sizes = ids_in.sizes().vec();
-    sizes.push_back(width);
-    const Tensor out = at::empty(sizes, table.options());
-    const auto p = embed_problem(ids, table, table.size(0), scale, padding);
-    const auto vt = rows_view(table);
-    const theria_rows_t vo{ptr(out), width};
-    token_rc(theria_embedding_fwd(&p, ids.data_ptr(), &vt, zero_padding, &vo, stream_of(table)), "theria_embedding_fwd");
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids_in, double scale, int64_t padding, bool zero_padding) {
+    const Tensor out = embed_fwd(table, ids_in, scale, padding, zero_padding);
     ctx->save_for_backward({ids_in});
     ctx->saved_data["classes"] = table.size(0);
     ctx->saved_data["scale"] = scale;
@@ -607,16 +630,17 @@ variable_list EmbedBackwardFn::backward(AutogradContext* ctx, const variable_lis
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
   const char* what = "hip_embedding";
   check_matrix(weight, "weight", what);
-  must(weight.dim() == 2 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
+  THERIA_MUST(weight.dim() == 2 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
        std::string(what) + ": weight must be (V, D) with 1 <= D <= " + std::to_string(kMaxRowWidth) + ", got shape " + shape_text(weight));
   check_indexes(ids, "ids", weight, what);
   int64_t padding = -1;
   if (padding_idx) {
     padding = *padding_idx < 0 ? *padding_idx + weight.size(0) : *padding_idx;
-    must(padding >= 0 && padding < weight.size(0), std::string(what) + ": padding_idx " + std::to_string(*padding_idx) + " is outside the table of " +
+    THERIA_MUST(padding >= 0 && padding < weight.size(0), std::string(what) + ": padding_idx " + std::to_string(*padding_idx) + " is outside the table of " +
                                                        std::to_string(weight.size(0)) + " rows");
   }
-  must(std::isfinite(scale) && std::isfinite((float)scale), std::string(what) + ": scale must be finite, got " + std::to_string(scale));
+  THERIA_MUST(std::isfinite(scale) && std::isfinite((float)scale), std::string(what) + ": scale must be finite, got " + std::to_string(scale));
+  if (outside_autograd({weight})) return embed_fwd(weight, ids, scale, padding, false);
   return EmbedFn::apply(weight, ids, scale, padding, false);
 }
 
@@ -635,7 +659,7 @@ variable_list ce_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& 
   const int64_t width = x_in.size(-1);
   const Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = target_in.contiguous(), bias = flat(bias_in);
   const Tensor dloss = dloss_in.to(at::kFloat).contiguous();
-  must(dloss.numel() == (reduction == THERIA_REDUCE_NONE ? x.size(0) : 1) && dloss.device() == x.device(),
+  THERIA_MUST(dloss.numel() == (reduction == THERIA_REDUCE_NONE ? x.size(0) : 1) && dloss.device() == x.device(),
        "hip_linear_cross_entropy: the loss's gradient must have the shape of the loss");
   const c10::hip::HIPGuard guard(x.get_device());
   Tensor dx, dw, db;
@@ -697,21 +721,26 @@ struct CeBackwardFn : torch::autograd::Function<CeBackwardFn> {
   }
 };
 
+// The loss, and the rows' statistics for the backward.
+std::pair<Tensor, Tensor> ce_fwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, const Tensor& target_in, int64_t ignore,
+                                 int64_t reduction) {
+  const Tensor x = rows_of(x_in, x_in.size(-1)), weight = rows_of(weight_in, weight_in.size(1)), target = target_in.contiguous(), bias = flat(bias_in);
+  const c10::hip::HIPGuard guard(x.get_device());
+  const auto f = x.options().dtype(at::kFloat);
+  const Tensor loss = reduction == THERIA_REDUCE_NONE ? at::empty(target_in.sizes(), f) : at::empty({}, f);
+  const Tensor stats = at::empty({2, x.size(0)}, f);
+  const auto p = ce_problem(x, weight, target, ignore, reduction);
+  const auto vx = rows_view(x), vw = rows_view(weight);
+  const Tensor ws = ce_workspace(p, vw, x, false, false, false, false);
+  token_rc(theria_linear_ce_fwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), floats(loss), floats(stats), ws.data_ptr(), stream_of(x)),
+           "theria_linear_ce_fwd");
+  return {loss, stats};
+}
+
 struct CeFn : torch::autograd::Function<CeFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, const Tensor& target_in,
                         int64_t ignore, int64_t reduction) {
-    const int64_t width = x_in.size(-1);
-    const Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = target_in.contiguous(),
-                 bias = flat(or_absent(bias_in));
-    const c10::hip::HIPGuard guard(x.get_device());
-    const auto f = x.options().dtype(at::kFloat);
-    const Tensor loss = reduction == THERIA_REDUCE_NONE ? at::empty(target_in.sizes(), f) : at::empty({}, f);
-    const Tensor stats = at::empty({2, x.size(0)}, f);
-    const auto p = ce_problem(x, weight, target, ignore, reduction);
-    const auto vx = rows_view(x), vw = rows_view(weight);
-    const Tensor ws = ce_workspace(p, vw, x, false, false, false, false);
-    token_rc(theria_linear_ce_fwd(&p, &vx, &vw, ptr(bias), target.data_ptr(), floats(loss), floats(stats), ws.data_ptr(), stream_of(x)),
-             "theria_linear_ce_fwd");
+    const auto [loss, stats] = ce_fwd(x_in, weight_in, or_absent(bias_in), target_in, ignore, reduction);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x_in, weight_in, bias_in, target_in, stats});
     ctx->saved_data["ignore"] = ignore;
@@ -738,20 +767,21 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   const Tensor bias = bias_in.value_or(Tensor());
   check_matrix(x, "x", what);
   check_matrix(weight, "weight", what);
-  must(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
+  THERIA_MUST(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
        w + ": x must be (..., D) and weight (V, D), got " + shape_text(x) + " and " + shape_text(weight));
-  must(weight.size(0) >= 1 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
+  THERIA_MUST(weight.size(0) >= 1 && weight.size(1) >= 1 && weight.size(1) <= kMaxRowWidth,
        w + " supports V >= 1 and 1 <= D <= " + std::to_string(kMaxRowWidth) + ", got weight " + shape_text(weight));
-  must(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(), w + ": weight must match x in dtype and device");
+  THERIA_MUST(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(), w + ": weight must match x in dtype and device");
   if (bias.defined()) check_plain(bias, what);
-  must(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0) && bias.scalar_type() == x.scalar_type() &&
+  THERIA_MUST(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0) && bias.scalar_type() == x.scalar_type() &&
                            bias.device() == x.device()),
        w + ": bias must be (" + std::to_string(weight.size(0)) + ",) and match x in dtype and device");
   check_indexes(target, "target", x, what);
-  must(target.sizes() == x.sizes().slice(0, x.dim() - 1), w + ": target must have shape " + "x's without its last dimension, got " + shape_text(target) +
+  THERIA_MUST(target.sizes() == x.sizes().slice(0, x.dim() - 1), w + ": target must have shape " + "x's without its last dimension, got " + shape_text(target) +
                                                               " for x " + shape_text(x));
-  must(reduction == "none" || reduction == "mean" || reduction == "sum", w + ": reduction must be 'none', 'mean' or 'sum', got '" + reduction + "'");
+  THERIA_MUST(reduction == "none" || reduction == "mean" || reduction == "sum", w + ": reduction must be 'none', 'mean' or 'sum', got '" + reduction + "'");
   const int64_t r = reduction == "none" ? THERIA_REDUCE_NONE : reduction == "mean" ? THERIA_REDUCE_MEAN : THERIA_REDUCE_SUM;
+  if (outside_autograd({x, weight, bias})) return ce_fwd(x, weight, bias, target, ignore, r).first;
   return CeFn::apply(x, weight, or_empty(bias, x), target, ignore, r);
 }
 

@@ -29,7 +29,7 @@ enum Tail {
   kWhole,  // the width is a multiple of VEC
   kOver,   // it is not: the last vector is loaded from VEC before the row's end and shifted when it is used. Loads of
            // single elements are waited for where they stand, and every load before them too: backward of (130000, 1001)
-           // bfloat16 170 us against 153 us, of (80000, 1500) 221 against 150.
+           // bfloat16 168 us against 153 us.
   kSingle  // the width is below VEC: single elements
 };
 
