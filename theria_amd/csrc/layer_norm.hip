@@ -156,6 +156,47 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_fwd_kernel(NormParams p) {
   }
 }
 
+// A thread's sums over its rows. For float32 parameters every sixteen rows are added up first (TWO): one sum over 256 rows
+// after the other loses half as much again as a library's tree (mean error of dweight of (65536, 2048) 2.9e-7 against
+// 2.1e-7, with TWO 1.7e-7). 16-bit parameters round by far more, and 1024 threads with 16 columns each have no registers left.
+template <int VEC, int NPT, bool TWO>
+struct RowSums {
+  float s[NPT][VEC], far[TWO ? NPT : 1][TWO ? VEC : 1];
+  int rows = 0;
+  __device__ __forceinline__ RowSums() {
+#pragma unroll
+    for (int i = 0; i < NPT; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        s[i][e] = 0.f;
+        if constexpr (TWO) far[i][e] = 0.f;
+      }
+  }
+  __device__ __forceinline__ void end_row() {
+    if constexpr (TWO) {
+      if (++rows % 16 == 0) join();
+    }
+  }
+  __device__ __forceinline__ void join() {
+    if constexpr (TWO) {
+#pragma unroll
+      for (int i = 0; i < NPT; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) far[i][e] += s[i][e], s[i][e] = 0.f;
+    }
+  }
+  __device__ __forceinline__ float (&total())[NPT][VEC] {
+    if constexpr (TWO) {
+      join();
+      return far;
+    } else {
+      return s;
+    }
+  }
+};
+template <typename WT, int VEC, int NPT, int TPR>
+constexpr bool kTwo = sizeof(WT) == 4 && !(TPR == 1024 && NPT * VEC == 16);
+
 // A workgroup's column sums: the teams' sums added and written as one partial row. acc: the thread's columns.
 template <int VEC, int NPT, int TPR>
 __device__ __forceinline__ void write_partial(float (&acc)[NPT][VEC], float* out, int width, float* lds) {
@@ -205,11 +246,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   const int t = threadIdx.x % TPR, width = p.width;
   const float inv = 1.0f / (float)width;
   const bool sums = p.dw || p.db;
-  float dw[NPT][VEC], db[NPT][VEC];
-#pragma unroll
-  for (int i = 0; i < NPT; ++i)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
+  RowSums<VEC, NPT, kTwo<WT, VEC, NPT, TPR>> dw, db;
 
   const HeldParam<WT, VEC, NPT, TPR, TAIL, HOLD> weight(p.weight, t, width, 1.f);
   const int64_t step = (int64_t)gridDim.x * TEAMS;
@@ -242,14 +279,15 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[i][e] = (x[i][e] - mean) * rstd;
-          dw[i][e] += g[i][e] * x[i][e];
-          db[i][e] += g[i][e];
+          dw.s[i][e] += g[i][e] * x[i][e];
+          db.s[i][e] += g[i][e];
           g[i][e] *= w[e];
           s[0] += g[i][e];
           s[1] += g[i][e] * x[i][e];
         }
       }
     }
+    dw.end_row(), db.end_row();
     if (p.dx.p) {
       team_sum<TPR, 2>(s, red[turn]);
       turn ^= 1;
@@ -269,8 +307,8 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_kernel(NormParams p) {
   }
   if (!sums) return;
   float* part = p.ws + (int64_t)blockIdx.x * 2 * width;
-  write_partial<VEC, NPT, TPR>(dw, part, width, lds);
-  write_partial<VEC, NPT, TPR>(db, part + width, width, lds);
+  write_partial<VEC, NPT, TPR>(dw.total(), part, width, lds);
+  write_partial<VEC, NPT, TPR>(db.total(), part + width, width, lds);
 }
 
 template <typename T, typename WT, int VEC, int NPT, int TPR, Tail TAIL>
@@ -281,12 +319,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
   __shared__ float lds[kPartialLds<VEC, NPT, TPR>];
   const int t = threadIdx.x % TPR, width = p.width;
   const float inv = 1.0f / (float)width;
-  float gw_sum[NPT][VEC];
-#pragma unroll
-  for (int i = 0; i < NPT; ++i)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) gw_sum[i][e] = 0.f;
-
+  RowSums<VEC, NPT, kTwo<WT, VEC, NPT, TPR>> gw_sum;
   const HeldParam<WT, VEC, NPT, TPR, TAIL, AHEAD> weight(p.weight, t, width, 1.f), gdw(p.gdw, t, width, 0.f), gdb(p.gdb, t, width, 0.f);
   const int64_t step = (int64_t)gridDim.x * TEAMS;
   int64_t row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
@@ -355,7 +388,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
         const float h = a[e] * g[i][e] - rstd * (u[i][e] * m_gx + g[i][e] * w[e] * m_ux);
         gx[e] = rstd * (h - m_h - x[i][e] * (m_hx + m_udx));
         gg[e] = w[e] * pu + a[e] * x[i][e] + b[e];
-        gw_sum[i][e] += g[i][e] * pu;
+        gw_sum.s[i][e] += g[i][e] * pu;
       }
       RawVec<T, VEC> out;
       if (p.out_gx.p) {
@@ -367,8 +400,9 @@ __global__ __launch_bounds__(kBlock<TPR>) void norm_bwd_bwd_kernel(NormParams p)
         out.template store<TAIL != kWhole>((T*)p.out_gdout.p + row * p.out_gdout.sr + c, width - c);
       }
     }
+    gw_sum.end_row();
   }
-  if (p.out_gw) write_partial<VEC, NPT, TPR>(gw_sum, p.ws + (int64_t)blockIdx.x * width, width, lds);
+  if (p.out_gw) write_partial<VEC, NPT, TPR>(gw_sum.total(), p.ws + (int64_t)blockIdx.x * width, width, lds);
 }
 
 // Teams by width, in vectors of 16 bytes: at most 16 elements of a tensor for each thread.
