@@ -323,8 +323,18 @@ struct LogitBase {
   }
 };
 
-// Forward: of each row (column j of the tile) the largest logit over the tile's classes and the sum of
-// exp(logit - largest), and the target's logit where it lies in the tile.
+// What a softmax's sum is kept as: the largest logit, and the sum of exp(logit - largest) without the largest one's 1 (-1 where
+// there is nothing but -inf). So the loss of a row that is well predicted, log1p of it, keeps its digits: next to the 1 they
+// would be rounded off with every term.
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+  const bool swap = b.x > a.x;
+  const float2 hi = swap ? b : a, lo = swap ? a : b;
+  const float off = hi.x == -THERIA_INF ? 0.f : hi.x;
+  return float2{hi.x, hi.y + (1.f + lo.y) * fast_exp2((lo.x - off) * kLog2e)};
+}
+
+// Forward: of each row (column j of the tile) that pair over the tile's classes, and the target's logit where it lies in the
+// tile.
 template <typename T, bool SCALED>
 struct LogitStats : LogitBase<T, SCALED> {
   float* at_target;   // one of each kept row
@@ -359,29 +369,28 @@ struct LogitStats : LogitBase<T, SCALED> {
         for (int r = 0; r < 16; ++r) top = fmaxf(top, z[fi][fj][r]);
       top = pair_max(top);
       const float off = top == -THERIA_INF ? 0.f : top;  // nothing but -inf: a sum of zeros
-      float sum = 0.f;
+      float part4[4] = {0.f, 0.f, 0.f, 0.f};
+      int tops = 0;
 #pragma unroll
       for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += fast_exp2((z[fi][fj][r] - off) * kLog2e);
-      sum = pair_sum(sum);
-      if (g == 0) red[t.wave_i][t.wave_j * (S::TJ / S::WJ) + 32 * fj + li] = float2{top, sum};
+        for (int r = 0; r < 16; ++r) {
+          const bool it = z[fi][fj][r] == top;
+          part4[r & 3] += it ? 0.f : fast_exp2((z[fi][fj][r] - off) * kLog2e);
+          tops += it;
+        }
+      const float others = pair_sum((part4[0] + part4[1]) + (part4[2] + part4[3])), more = pair_sum((float)tops) - 1.f;
+      const float rest = top == THERIA_INF ? __builtin_nanf("") : others + (top == -THERIA_INF ? -1.f : more);
+      if (g == 0) red[t.wave_i][t.wave_j * (S::TJ / S::WJ) + 32 * fj + li] = float2{top, rest};
     }
     __syncthreads();
     for (int c = threadIdx.x; c < S::TJ; c += S::NW * 64) {
       const int j = t.tile_j * S::TJ + c;
       if (j >= t.J) continue;
-      float top = red[0][c].x;
+      float2 all = red[0][c];
 #pragma unroll
-      for (int w = 1; w < S::WI; ++w) top = fmaxf(top, red[w][c].x);
-      const float off = top == -THERIA_INF ? 0.f : top;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < S::WI; ++w) {
-        const float2 v = red[w][c];
-        sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));  // v.y is 0 there, or NaN
-      }
-      part[(int64_t)(tile0 + t.tile_i) * n + j] = float2{top, sum};
+      for (int w = 1; w < S::WI; ++w) all = joined(all, red[w][c]);
+      part[(int64_t)(tile0 + t.tile_i) * n + j] = all;
     }
   }
 };
@@ -590,29 +599,28 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeParams p, int tiles, con
   const int r = threadIdx.x % R, s = threadIdx.x / R;
   const int64_t j = (int64_t)blockIdx.x * R + r;
   const int kept = meta->kept;
-  float top = -THERIA_INF, sum = 0.f;
+  float2 all{-THERIA_INF, -1.f};
   if (j < kept) {
+    float top = -THERIA_INF, rest = 0.f;
+    bool seen = false;
 #pragma unroll 4
     for (int k = s; k < tiles; k += S) top = fmaxf(top, part[(int64_t)k * p.n + j].x);
     const float off = top == -THERIA_INF ? 0.f : top;
 #pragma unroll 4
     for (int k = s; k < tiles; k += S) {
       const float2 v = part[(int64_t)k * p.n + j];
-      sum += v.y * (v.x == -THERIA_INF ? 1.f : fast_exp2((v.x - off) * kLog2e));
+      const bool it = v.x == top && !seen;
+      rest += it ? v.y : (1.f + v.y) * fast_exp2((v.x - off) * kLog2e);
+      seen = seen || it;
     }
+    all = float2{top, seen ? rest : -1.f};
   }
-  red[s][r] = float2{top, sum};
+  red[s][r] = all;
   // halves of the slices joined in turn, in an order that does not depend on the run
 #pragma unroll
   for (int o = S / 2; o > 0; o /= 2) {
     __syncthreads();
-    if (s < o) {
-      const float2 a = red[s][r], b = red[s + o][r];
-      top = fmaxf(a.x, b.x);
-      const float off = top == -THERIA_INF ? 0.f : top;
-      sum = a.y * (a.x == -THERIA_INF ? 1.f : fast_exp2((a.x - off) * kLog2e)) + b.y * (b.x == -THERIA_INF ? 1.f : fast_exp2((b.x - off) * kLog2e));
-      red[s][r] = float2{top, sum};
-    }
+    if (s < o) red[s][r] = all = joined(red[s][r], red[s + o][r]);
   }
   if (s != 0 || j >= p.n) return;
   if (j >= kept) {
@@ -622,9 +630,9 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeParams p, int tiles, con
     }
     return;
   }
-  p.stats[j] = top;
-  p.stats[p.n + j] = sum;
-  if (row_loss) row_loss[map[j]] = logf(sum) - (at_target[j] - top);
+  p.stats[j] = all.x;
+  p.stats[p.n + j] = 1.f + all.y;
+  if (row_loss) row_loss[map[j]] = log1pf(all.y) - (at_target[j] - all.x);
 }
 
 // The mean or sum of the rows' losses, by one workgroup in a fixed order.
