@@ -320,8 +320,8 @@ typedef struct {
 /* Bytes of the 256-byte-aligned workspace of a call on these matrices. Nothing in it is kept between calls. */
 int64_t theria_linear_ce_ws_bytes(const theria_linear_ce_problem_t* p, const theria_rows_t* weight, int32_t backward,
                                   int32_t need_dx, int32_t need_dweight, int32_t need_dbias);
-/* loss (float32: n of them, or one) and, for the backward, stats (2 n floats: of the i-th row that is not left out, the
- * largest logit and the sum of exp(logit - largest)). Rows left out have loss 0 and are not read; a target outside
+/* loss (float32: n of them, or one) and stats: 2 n floats for the backward of the same problem and inputs, which alone knows what
+ * they hold. Rows left out have loss 0 and are not read; a target outside
  * [0, classes) gives a loss of NaN. The mean is over the rows that are not left out, NaN if there are none. bias may be NULL. */
 int theria_linear_ce_fwd(const theria_linear_ce_problem_t* p, const theria_rows_t* x, const theria_rows_t* weight, const void* bias,
                          const void* target, float* loss, float* stats, void* ws, void* stream);

@@ -5,7 +5,8 @@ Layout mirrors the reference package so callers switch by import name:
   theria_amd.attention               fused forward / explicit backward / frozen-stats JVP on HIP,
                                      sdpa_custom dispatcher, pure-PyTorch references, FD HVP
   theria_amd.autograd                SDPAOp / SDPABackwardOp (HIP, exact to second order),
-                                     SDPAFunction, SDPACustom
+                                     SDPAFunction, SDPACustom; hip_layer_norm, hip_embedding,
+                                     hip_linear_cross_entropy
   theria_amd.maml / models / tasks   the MAML loops and tiny models that drive double backward
 """
 

@@ -19,7 +19,9 @@ namespace theria {
 namespace {
 
 constexpr int kPiece = 64;         // sorted tokens of a piece
-constexpr int kRankTokens = 8192;  // most tokens ordered by counting
+// Most tokens ordered by counting: 12 us for 4096 and 20 us for 8192 tokens, where two passes of the sort take 25 us; 16384
+// tokens would take 35 us against 25 us.
+constexpr int kRankTokens = 8192;
 constexpr int kSortMost = 1024;     // digits of a radix sort's pass
 
 __device__ __forceinline__ int64_t load_id(const void* ids, bool ids64, int64_t n) {
