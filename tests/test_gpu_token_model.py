@@ -176,3 +176,33 @@ def test_a_thread_of_its_own(hip_device):
     for th in threads:
         th.join()
     assert not wrong
+
+
+def test_views_of_negated_values(hip_device):
+    """The imaginary part of a conjugate is a view whose values stand in memory with the other sign."""
+    gen = torch.Generator().manual_seed(3)
+    part = lambda *shape: torch.complex(torch.zeros(shape), torch.randn(*shape, generator=gen)).to(hip_device).conj().imag  # noqa: E731
+    x, w, b, g = part(6, 5), part(5), part(5), part(6, 5)
+    assert x.is_neg() and not x.clone().is_neg()
+    table, ids, targets = part(7, 5), torch.tensor([0, 6, 3], device=hip_device), torch.tensor([0, 6, 3, 3, 1, 2], device=hip_device)
+    up = part(6)
+    calls = (
+        (lambda x, w, b: hip_layer_norm(x, w, b), (x, w, b), g),
+        (lambda t: hip_embedding(ids, t), (table,), g[:3]),
+        (lambda x, t: hip_linear_cross_entropy(x, t, targets, reduction="none"), (x, table), up),
+    )
+    for call, args, cot in calls:
+        got = [call(*args)] + list(torch.autograd.grad(call(*(leaves := [a.detach().requires_grad_(True) for a in args])), leaves, cot))
+        plain = [a.clone() for a in args]
+        want = [call(*plain)] + list(torch.autograd.grad(call(*(leaves := [a.requires_grad_(True) for a in plain])), leaves, cot.clone()))
+        for a, e in zip(got, want):
+            assert torch.equal(a, e)
+
+
+def test_forward_mode_is_refused_without_a_graph_too(hip_device):
+    import torch.autograd.forward_ad as fwAD
+
+    x, w, calls = _calls(hip_device)
+    for call in calls:
+        with torch.no_grad(), fwAD.dual_level(), pytest.raises(RuntimeError):
+            fwAD.unpack_dual(call(x, fwAD.make_dual(w, torch.ones_like(w)))).tangent.sum()

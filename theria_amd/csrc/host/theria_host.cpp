@@ -325,9 +325,10 @@ void check_indexes(const Tensor& t, const char* name, const Tensor& like, const 
   THERIA_MUST(t.numel() <= kMaxRows, std::string(what) + ": " + name + " has more elements than 32-bit indexes reach");
 }
 
-// A tensor's rows of `width` as a matrix; a copy only where no view with a contiguous last dimension exists.
+// A tensor's rows of `width` as a matrix; a copy only where no view with a contiguous last dimension exists, or where the
+// view is one of negated values (the imaginary part of a conjugate).
 Tensor rows_of(const Tensor& t_in, int64_t width) {
-  Tensor t = t_in;
+  Tensor t = t_in.resolve_neg();
   if (t.dim() != 2) t = t.reshape({t.numel() / width, width});
   if (width > 1 && t.stride(1) != 1) t = t.contiguous();
   return t;
@@ -338,7 +339,7 @@ Tensor rows_like(const Tensor& t, const Tensor& like, const char* what) {
   THERIA_MUST(t.sizes() == like.sizes() && t.device() == like.device(), std::string(what) + ": a gradient must have the shape of its input");
   return rows_of(t.scalar_type() == like.scalar_type() ? t : t.to(like.scalar_type()), like.size(-1));
 }
-Tensor flat(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor flat(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 theria_rows_t rows_view(const Tensor& t) { return t.defined() ? theria_rows_t{t.data_ptr(), t.stride(0)} : theria_rows_t{nullptr, 0}; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
@@ -658,7 +659,7 @@ variable_list ce_bwd(const Tensor& x_in, const Tensor& weight_in, const Tensor& 
                      const Tensor& dloss_in, int64_t ignore, int64_t reduction, bool need_dx, bool need_dw, bool need_db) {
   const int64_t width = x_in.size(-1);
   const Tensor x = rows_of(x_in, width), weight = rows_of(weight_in, width), target = target_in.contiguous(), bias = flat(bias_in);
-  const Tensor dloss = dloss_in.to(at::kFloat).contiguous();
+  const Tensor dloss = dloss_in.to(at::kFloat).resolve_neg().contiguous();
   THERIA_MUST(dloss.numel() == (reduction == THERIA_REDUCE_NONE ? x.size(0) : 1) && dloss.device() == x.device(),
        "hip_linear_cross_entropy: the loss's gradient must have the shape of the loss");
   const c10::hip::HIPGuard guard(x.get_device());
