@@ -50,6 +50,22 @@ def test_rows_and_gradient_match_float64(dt, N, V, D, hip_device):
         _check(_ids(N, V, kind, N).to(hip_device), w, g, 1.5, None, kind)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 63, 64, 65, 255, 256, 257, 511, 512, 513])
+@pytest.mark.parametrize("V,D", [(1, 40), (16, 64), (17, 200), (40000, 72), (9000, 520)])
+def test_few_tokens(N, V, D, dt, hip_device):
+    """On both sides of the gradient in one launch, whose workgroups order their rows' tokens themselves."""
+    gen = torch.Generator().manual_seed(N + V)
+    w, g = torch.randn(V, D, generator=gen).to(dt).to(hip_device), torch.randn(N, D, generator=gen).to(dt).to(hip_device)
+    for kind in ("uniform", "zipf", "one", "rising"):
+        _check(_ids(N, V, kind, N).to(hip_device), w, g, 0.5, 0 if V > 1 else None, f"{kind} {N}")
+    ids = _ids(N, V, "uniform", 1)
+    ids[::3] = torch.tensor([-1, V, 2**40])[torch.arange(len(ids[::3])) % 3]
+    _, dw = _run(ids.to(hip_device), w, g)
+    known = (ids >= 0) & (ids < V)
+    O.check(dw, *O.embed_backward(ids[known], g[known.to(hip_device)], V, 1.0, None), "ids outside the table")
+
+
 @pytest.mark.parametrize("N,V", [(131072, 3000), (131073, 3000), (200003, 70000)])
 def test_many_tokens(N, V, hip_device):
     """On both sides of the radix sort's change to tiles of 4096 tokens."""

@@ -75,6 +75,14 @@ def test_float32_parameters_beside_16_bit_rows(dt, shape, hip_device):
     _check_all(x, w, b, g, u, a, c, f"{dt} wide {shape}")
 
 
+@pytest.mark.parametrize("dt,pt", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("shape", [(40000, 21), (9000, 203), (5000, 1500), (4200, 4101), (600, 8195)])
+def test_many_rows_of_odd_widths(dt, pt, shape, hip_device):
+    """Teams of every size that walk many rows, the last vector of each partly filled."""
+    x, w, b, g, u, a, c = _make(shape, dt, pt, hip_device, seed=shape[1])
+    _check_all(x, w, b, g, u, a, c, f"{dt} {shape}")
+
+
 @pytest.mark.parametrize("weight,bias", [(True, False), (False, True), (False, False)])
 def test_parameters_are_optional(weight, bias, hip_device):
     x, w, b, g, u, a, c = _make((12, 96), torch.bfloat16, torch.bfloat16, hip_device, weight=weight, bias=bias)

@@ -84,6 +84,25 @@ def test_large_tiles_in_both_gradients(N, V, D, hip_device):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("N,V", [(30, 5), (100, 13), (40, 60), (300, 100), (300, 700), (1100, 1030)])
+def test_small_losses_keep_their_digits(dt, N, V, hip_device):
+    """Rows whose target stands far above the other classes, with logits that every type holds exactly: loss log1p(sum of
+    exp(z - top)). The exponent of at most 16 log2(e) = 23.1 has two roundings (its constant's and the product's), 2 * 23.1 ln 2 u
+    = 32 u of the exponential, which is good to 2 u itself; V terms are added and log1p good to 4 u: 38 u and V u."""
+    gen = torch.Generator().manual_seed(V)
+    t = torch.randint(0, V, (N,), generator=gen)
+    x = torch.randint(-8, 9, (N, V), generator=gen) / 8.0
+    x[torch.arange(N), t] = 3.0
+    z = 4.0 * x.double()
+    z -= 12.0
+    others = torch.exp(z).scatter(1, t.unsqueeze(1), 0.0).sum(1)
+    want = torch.log1p(others)
+    got = hip_linear_cross_entropy(x.to(dt).to(hip_device), (4.0 * torch.eye(V)).to(dt).to(hip_device), t.to(hip_device), reduction="none")
+    off = ((got.double().cpu() - want).abs() / want).max()
+    assert float(off) <= (V + 38) * O.U, f"{float(off) / O.U:.3g} u"
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("N", [16384, 16385, 40000])
 def test_many_rows_are_listed_by_several_workgroups(dt, N, hip_device):
     """On both sides of the limit of one workgroup; ignored and invalid targets in runs, at both ends, and everywhere."""

@@ -11,7 +11,8 @@
 //           of LDS, spread over the GPU). More: a stable radix sort, digits of at most 10 bits, two launches a digit.
 //   pieces  frequent ids: every aligned run of 64 sorted tokens that holds one id alone is summed by a workgroup of its
 //           own into a float32 row of the workspace, so that an id with thousands of tokens is spread over the GPU.
-//   rows    every table row: the tokens before its first whole piece, the pieces, and the tokens after its last one.
+//   rows    every table row: the tokens before its first whole piece, the pieces, and the tokens after its last one. Of
+//           few tokens and rows this launch is the only one (own_launch): each workgroup finds its rows' tokens itself.
 #include "token_common.hpp"
 #include "token_params.hpp"
 
@@ -288,19 +289,73 @@ __global__ __launch_bounds__(256) void embed_piece_kernel(EmbedParams p, const u
 }
 
 constexpr int kRowsMost = 16;   // table rows of a workgroup
+constexpr int kOwnTokens = 512;  // most tokens whose gradient may be one launch instead of three
 constexpr int kTeamTokens = 8;  // most tokens that a team sums alone
 
-// `rows` table rows of a workgroup, one for each team in turn; rows with more tokens take all the teams.
-template <typename T, int VEC, int TPR>
-__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const uint32_t* __restrict__ order, const int2* __restrict__ bounds,
+// The tokens of table rows v0 to v0 + have, in order, and each row's run of them, found by the workgroup itself: every one
+// looks at every id, which takes less than a launch while they are few.
+__device__ __forceinline__ void own_order(const EmbedParams& p, int64_t v0, int have, uint32_t* order, int2* bound, int (&count)[kOwnTokens / 64][kRowsMost]) {
+  constexpr int PER = kOwnTokens / 256;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  int row[PER], before[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int n = u * 256 + threadIdx.x;
+    const int64_t at = n < p.n ? (int64_t)key_of(p, n) - v0 : -1;
+    row[u] = at >= 0 && at < have ? (int)at : -1;
+    before[u] = 0;
+    for (int r = 0; r < have; ++r) {
+      const uint64_t all = __ballot(row[u] == r);
+      if (lane == 0) count[4 * u + wave][r] = __popcll(all);
+      if (row[u] == r) before[u] = __popcll(all & ((uint64_t(1) << lane) - 1));
+    }
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < kRowsMost) {  // each row's counts to places in it, and its tokens
+    int sum = 0;
+    if ((int)threadIdx.x < have)
+#pragma unroll
+      for (int k = 0; k < kOwnTokens / 64; ++k) {
+        const int c = count[k][threadIdx.x];
+        count[k][threadIdx.x] = sum;
+        sum += c;
+      }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < kRowsMost; o *= 2) {
+      const int add = __shfl_up(upto, o, kRowsMost);
+      if ((int)threadIdx.x >= o) upto += add;
+    }
+    bound[threadIdx.x] = int2{upto - sum, upto};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    if (row[u] >= 0) order[bound[row[u]].x + count[4 * u + wave][row[u]] + before[u]] = u * 256 + threadIdx.x;
+  __syncthreads();
+}
+
+// `rows` table rows of a workgroup, one for each team in turn; rows with more tokens take all the teams. OWN: the gradient of at
+// most kOwnTokens tokens, in this launch alone.
+template <typename T, int VEC, int TPR, bool OWN>
+__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, int64_t first, const uint32_t* __restrict__ sorted, const int2* __restrict__ bounds,
                                                          const float* __restrict__ pieces, int rows, int cols) {
   constexpr int TEAMS = 256 / TPR;
   __shared__ float lds[256 * (VEC + 1)];
   __shared__ int2 bound[kRowsMost];
-  const int64_t v0 = (int64_t)(blockIdx.x / cols) * rows;
-  const int have = (int)min((int64_t)rows, p.classes - v0);
-  if ((int)threadIdx.x < have) bound[threadIdx.x] = p.n ? bounds[v0 + threadIdx.x] : int2{0, 0};
-  __syncthreads();
+  const int64_t v0 = (int64_t)(blockIdx.x / cols) * rows;  // from `first`
+  const int have = (int)min((int64_t)rows, p.classes - first - v0);
+  __shared__ uint32_t own[OWN ? kOwnTokens : 1];
+  __shared__ int count[OWN ? kOwnTokens / 64 : 1][kRowsMost];
+  const uint32_t* order;
+  if constexpr (OWN) {
+    own_order(p, first + v0, have, own, bound, count);
+    order = own;
+  } else {
+    if ((int)threadIdx.x < have) bound[threadIdx.x] = bounds[first + v0 + threadIdx.x];
+    __syncthreads();
+    order = sorted;
+  }
   const int t = threadIdx.x % TPR, team = threadIdx.x / TPR, c = ((int)(blockIdx.x % cols) * TPR + t) * VEC;
   auto write = [&](const float(&acc)[VEC], int64_t v) {
     if (c >= p.width) return;
@@ -323,7 +378,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedParams p, const ui
     if (e - s <= kTeamTokens) continue;
     const int a = (s + kPiece - 1) / kPiece, b = e / kPiece;  // whole pieces [a, b)
     float acc[VEC] = {};
-    if (a < b) {
+    if (!OWN && a < b) {
       add_tokens<T, VEC>(acc, p, order, s, a * kPiece, team, TEAMS, c);
       if (c < p.width) {
 #pragma unroll 4
@@ -396,7 +451,6 @@ hipError_t sort_tokens(const EmbedParams& p, Order& o, hipStream_t st) {
   const Space at(p);
   uint32_t *key[2] = {(uint32_t*)ws, (uint32_t*)(ws + at.each)}, *ord[2] = {(uint32_t*)(ws + 2 * at.each), (uint32_t*)(ws + 3 * at.each)};
   o = {key[0], ord[0], (int2*)(ws + at.bounds), (float*)(ws + at.pieces)};
-  if (p.n == 0) return hipSuccess;
   if (p.n <= kRankTokens) {
     rank_kernel<<<dim3((unsigned)((p.n + 63) / 64)), 1024, 0, st>>>(p, o.keys, o.order, o.bounds);
     return hipGetLastError();
@@ -420,28 +474,42 @@ hipError_t sort_tokens(const EmbedParams& p, Order& o, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Columns of workgroups of the gradient, and its table rows for each (several once they fill the GPU).
+int grad_team(const EmbedParams& p) { return p.width <= 16 * (p.dtype == 0 ? 4 : 8) ? 16 : 64; }
+int64_t grad_cols(const EmbedParams& p) {
+  const int64_t cols = (int64_t)grad_team(p) * (p.dtype == 0 ? 4 : 8);
+  return (p.width + cols - 1) / cols;
+}
+int64_t grad_rows(const EmbedParams& p) {
+  const int64_t per = p.classes * grad_cols(p) / (16 * (int64_t)device_cu_count());
+  return per < 1 ? 1 : per < kRowsMost ? per : kRowsMost;
+}
+// Whether the gradient is one launch. (512, 32 to 1000, up to 4096) bfloat16: 44 us a call with its lookup against 50 us, 6 to 7 us
+// against 12 to 13 in a graph; an id that all 512 tokens share 21 us against 17. More workgroups than those with fewer
+// than kRowsMost rows each lose it again, (512, 128000, 1024) 62 us against 58; more tokens than these wait for the one id.
+bool own_launch(const EmbedParams& p) { return p.n <= kOwnTokens && grad_rows(p) < kRowsMost; }
+
 template <typename T, int VEC, int TPR>
 hipError_t bwd(const EmbedParams& p, hipStream_t st) {
-  constexpr int COLS = TPR * VEC;
-  const unsigned cols = (unsigned)((p.width + COLS - 1) / COLS);
-  Order o;
-  hipError_t e = sort_tokens(p, o, st);
-  if (e != hipSuccess) return e;
-  if (p.n > 0) {
+  const unsigned cols = (unsigned)grad_cols(p);
+  const bool own = own_launch(p) || p.n == 0;
+  Order o{};
+  if (!own) {
+    hipError_t e = sort_tokens(p, o, st);
+    if (e != hipSuccess) return e;
     embed_piece_kernel<T, VEC, TPR><<<dim3((unsigned)((p.n + kPiece - 1) / kPiece), cols), 256, 0, st>>>(p, o.keys, o.order, o.bounds, o.pieces);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  // several rows for a workgroup once they fill the GPU
-  const int64_t per = p.classes * cols / (16 * (int64_t)device_cu_count());
-  const int rows = (int)(per < 1 ? 1 : per < kRowsMost ? per : kRowsMost);
+  const int rows = (int)grad_rows(p);
   const int64_t most = (int64_t(1) << 23) / cols * rows;  // table rows: a launch holds fewer than 2^32 threads
   for (int64_t v = 0; v < p.classes; v += most) {
+    const int64_t have = p.classes - v < most ? p.classes - v : most;
     EmbedParams q = p;
-    q.classes = p.classes - v < most ? p.classes - v : most;
     q.out.p = (T*)p.out.p + v * p.out.sr;
-    embed_rows_kernel<T, VEC, TPR><<<dim3((unsigned)((q.classes + rows - 1) / rows * cols)), 256, 0, st>>>(q, o.order, o.bounds + v, o.pieces, rows, (int)cols);
-    e = hipGetLastError();
+    const auto kernel = own ? embed_rows_kernel<T, VEC, TPR, true> : embed_rows_kernel<T, VEC, TPR, false>;
+    kernel<<<dim3((unsigned)((have + rows - 1) / rows * cols)), 256, 0, st>>>(q, v, o.order, o.bounds, o.pieces, rows, (int)cols);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
@@ -452,7 +520,7 @@ hipError_t by_width(const EmbedParams& p, hipStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const int n = (p.width + V - 1) / V;
   if constexpr (GRAD) {
-    return n <= 16 ? bwd<T, V, 16>(p, st) : bwd<T, V, 64>(p, st);
+    return grad_team(p) == 16 ? bwd<T, V, 16>(p, st) : bwd<T, V, 64>(p, st);
   } else {
     if (n <= 16) return fwd<T, V, 16>(p, st);
     return n <= 128 ? fwd<T, V, 64>(p, st) : fwd<T, V, 256>(p, st);
