@@ -37,6 +37,9 @@ constexpr int64_t kPieceBytes = int64_t(256) << 20;  // most of a piece's dz
 constexpr int64_t kLayBytes = int64_t(1) << 30;      // most of a piece of W laid out anew
 constexpr int64_t kNativeRows = 256;                 // most rows of float32 products without planes
 
+// The workspace's layout and the kernels that use it ask the same question.
+bool takes_planes(const CeParams& p) { return p.dtype == 0 && p.n > kNativeRows; }
+
 // ------------------------------------------------------------------------------------------ rows
 struct Meta {
   int kept;
@@ -761,7 +764,7 @@ struct Layout {
 
 Layout layout_of(const CeParams& p, bool backward) {
   Layout l{};
-  l.planes = p.dtype == 0 && p.n > kNativeRows;
+  l.planes = takes_planes(p);
   const bool f32 = p.dtype == 0, native = f32 && !l.planes;
   // bytes of an element of the logits' operands and of the gradients', all planes
   const int es = f32 ? 4 : 2, bl = es, bg = l.planes ? 6 : es, per = 16 / es;
@@ -974,7 +977,7 @@ hipError_t run(const CeParams& p, bool backward, hipStream_t st) {
 }
 
 hipError_t by_type(const CeParams& p, bool backward, hipStream_t st) {
-  if (p.dtype == 0) return p.n > kNativeRows ? run<float, true>(p, backward, st) : run<float, false>(p, backward, st);
+  if (p.dtype == 0) return takes_planes(p) ? run<float, true>(p, backward, st) : run<float, false>(p, backward, st);
   if (p.dtype == 1) return run<_Float16, false>(p, backward, st);
   return run<__bf16, false>(p, backward, st);
 }
