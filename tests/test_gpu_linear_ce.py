@@ -57,6 +57,14 @@ def test_loss_and_gradients_match_float64(dt, N, V, D, hip_device):
         _check(x, w, t, b, reduction, g if reduction == "none" else None, f"{reduction} bias={bias}")
 
 
+@pytest.mark.parametrize("N", [257, 1300, 4100])
+@pytest.mark.parametrize("V,D", [(5, 700), (17, 64), (40, 1030), (128, 300), (129, 520), (256, 65), (257, 65)])
+def test_float32_of_many_rows_and_few_classes(N, V, D, hip_device):
+    x, w, t, b, g = _make(N, V, D, torch.float32, hip_device, seed=N + V, bias=True, pad=0.2)
+    _check(x, w, t, b, "none", g, f"{N} {V} {D}")
+    _check(x, w, t, None, "mean", None, f"{N} {V} {D} mean")
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_large_tiles(dt, hip_device):
     """Enough tiles for the 256 x 256 shape in all three products (205 and more), with ragged edges."""
